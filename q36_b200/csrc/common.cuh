@@ -1,5 +1,6 @@
 // Shared device/host helpers for the MXFP4 x E4M3 MoE expert path (sm_100a).
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>

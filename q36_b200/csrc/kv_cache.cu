@@ -1,0 +1,311 @@
+// The paged 4-bit cache: tables of a step from its request lengths, the writer and the reader of cache rows.
+#include "attn.cuh"
+
+namespace q36 {
+
+constexpr int TB_THREADS = 512;
+constexpr int TB_MAX_SEQ = 16384;
+
+// ---------------------------------------------------------------- tables
+// Two prefix sums over the requests (rows, new blocks), then one pass over all rows and all new blocks, each of which finds
+// its request by bisection.  Sums saturate just above what is available (min(a + b, cap) is associative for a, b >= 0), so
+// that no lengths overflow them.  Every CTA makes the sums for itself: 16 KB of lengths at 2000 requests come out of L2 in
+// less time than a second launch takes.
+struct TbReq { int rows, need, ok; };
+__device__ __forceinline__ TbReq tb_request(int old, int q, int bs, int max_blocks, int row_cap, int blk_cap, int &flags) {
+    TbReq r;
+    r.ok = 1;
+    r.rows = min(max(q, 0), row_cap);
+    r.need = 0;
+    if (old < 0 || q < 0) { flags |= 4; r.ok = 0; return r; }
+    const long long held = ((long long)old + bs - 1) / bs, all = ((long long)old + q + bs - 1) / bs;
+    if (all > max_blocks) { flags |= 2; r.ok = 0; return r; }
+    r.need = (int)min(all - held, (long long)blk_cap);
+    return r;
+}
+__device__ __forceinline__ int sat_add(int a, int b, int cap) { return min(a + b, cap); }
+
+// largest b in [0, n) with pre[b] <= v (pre[0] <= v)
+__device__ __forceinline__ int bisect(const int *pre, int n, int v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (pre[m] <= v) lo = m; else hi = m;
+    }
+    return lo;
+}
+
+__global__ void __launch_bounds__(TB_THREADS)
+k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int bs, int n_blocks, const int *__restrict__ free_blocks,
+            int n_free, const int *free_head, int *block_table, int max_blocks, int *__restrict__ cu_q, int *kv_len,
+            int *__restrict__ slots, int *__restrict__ positions, int T, int *free_head_out, int *status) {
+    Q36_GDS();
+    extern __shared__ int sm[];
+    int *pre_r = sm, *pre_b = sm + B + 1;     // exclusive prefix sums; entry B: the total
+    __shared__ int wr[TB_THREADS / 32], wb[TB_THREADS / 32], fl;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int head = min(max(*free_head, 0), n_free), avail = n_free - head;
+    const int row_cap = T + 1, blk_cap = avail + 1;
+    if (tid == 0) fl = 0;
+    const int per = (B + TB_THREADS - 1) / TB_THREADS, b0 = min(tid * per, B), b1 = min(b0 + per, B);
+    int flags = 0, sr = 0, sb = 0;
+    for (int b = b0; b < b1; b++) {
+        const TbReq r = tb_request(kv_old[b], q_len[b], bs, max_blocks, row_cap, blk_cap, flags);
+        pre_r[b] = sr;
+        pre_b[b] = sb;
+        sr = sat_add(sr, r.rows, row_cap);
+        sb = sat_add(sb, r.need, blk_cap);
+    }
+    int ir = sr, ib = sb;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int r = __shfl_up_sync(0xffffffffu, ir, o), n = __shfl_up_sync(0xffffffffu, ib, o);
+        if (lane >= o) { ir = sat_add(ir, r, row_cap); ib = sat_add(ib, n, blk_cap); }
+    }
+    if (lane == 31) { wr[warp] = ir; wb[warp] = ib; }
+    int er = __shfl_up_sync(0xffffffffu, ir, 1), eb = __shfl_up_sync(0xffffffffu, ib, 1);
+    if (lane == 0) er = eb = 0;
+    __syncthreads();
+    for (int w = 0; w < warp; w++) { er = sat_add(er, wr[w], row_cap); eb = sat_add(eb, wb[w], blk_cap); }
+    for (int b = b0; b < b1; b++) { pre_r[b] = sat_add(pre_r[b], er, row_cap); pre_b[b] = sat_add(pre_b[b], eb, blk_cap); }
+    if (tid == TB_THREADS - 1) { pre_r[B] = sat_add(er, sr, row_cap); pre_b[B] = sat_add(eb, sb, blk_cap); }
+    __syncthreads();
+    const int total_rows = min(pre_r[B], T), total_new = pre_b[B];
+    auto served = [&](int b, const TbReq &r) { return r.ok && (r.need == 0 || pre_b[b] + r.need <= avail) && (r.rows == 0 || pre_r[b + 1] <= T); };
+
+    const int stride = gridDim.x * TB_THREADS, first = blockIdx.x * TB_THREADS + tid;
+    int dummy = 0;
+    // new table entries
+    for (int i = first; i < min(total_new, avail); i += stride) {
+        const int b = bisect(pre_b, B, i);
+        const int old = kv_old[b];
+        const TbReq r = tb_request(old, q_len[b], bs, max_blocks, row_cap, blk_cap, dummy);
+        if (!served(b, r)) continue;
+        const int held = (old + bs - 1) / bs;
+        block_table[(size_t)b * max_blocks + held + (i - pre_b[b])] = free_blocks[head + i];
+    }
+    // rows; a row's block is an old table entry or a free-list entry (the table's new entries may not be written yet)
+    for (int t = first; t < T; t += stride) {
+        int slot = -1, pos = -1;
+        if (t < total_rows) {
+            const int b = bisect(pre_r, B, t);
+            const int old = kv_old[b];
+            const TbReq r = tb_request(old, q_len[b], bs, max_blocks, row_cap, blk_cap, dummy);
+            if (served(b, r)) {
+                pos = old + (t - pre_r[b]);
+                const int held = (old + bs - 1) / bs, col = pos / bs;
+                const int blk = col < held ? block_table[(size_t)b * max_blocks + col] : free_blocks[head + pre_b[b] + (col - held)];
+                if (blk >= 0 && blk < n_blocks) slot = blk * bs + pos % bs;
+            }
+        }
+        slots[t] = slot;
+        positions[t] = pos;
+    }
+    // The requests' own outputs: block 0, after everything that reads the lengths and the head (kv_len and free_head_out may be
+    // kv_old and free_head, with one block).
+    if (blockIdx.x == 0) {
+        __syncthreads();
+        int used = 0;
+        for (int b = tid; b < B; b += TB_THREADS) {
+            const int old = kv_old[b], q = q_len[b];
+            const TbReq r = tb_request(old, q, bs, max_blocks, row_cap, blk_cap, flags);
+            const bool s = served(b, r);
+            if (r.ok && r.need > 0 && pre_b[b] + r.need > avail) flags |= 1;
+            if (r.rows > 0 && pre_r[b + 1] > T) flags |= 8;
+            cu_q[b] = min(pre_r[b], T);
+            kv_len[b] = s ? old + q : 0;
+            // (from the first unserved request on that needs blocks or rows none of that kind is served: no holes)
+            if (s && r.need > 0) used = max(used, pre_b[b] + r.need);
+        }
+        if (tid == 0) cu_q[B] = total_rows;
+        used = (int)__reduce_max_sync(0xffffffffu, (unsigned)used);
+        flags = (int)__reduce_or_sync(0xffffffffu, (unsigned)flags);
+        if (lane == 0) { wr[warp] = used; atomicOr(&fl, flags); }
+        __syncthreads();
+        if (tid == 0) {
+            for (int w = 1; w < TB_THREADS / 32; w++) used = max(used, wr[w]);
+            *free_head_out = head + used;
+            *status = fl;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- rows in and out
+// Smallest e with amax <= 6 * 2^e in [-126, 125]; 6 = 1.5 * 2^2.
+__device__ __forceinline__ int e2_of_amax_fp4(float amax) {
+    const uint32_t u = __float_as_uint(amax);
+    const int e = (int)(u >> 23) - 129 + ((u & 0x7FFFFFu) > 0x400000u ? 1 : 0);
+    return max(-126, min(125, e));
+}
+// eight f32 -> eight E2M1 nibbles, element 0 in the low one; round to nearest even, saturating at 6
+__device__ __forceinline__ uint32_t f32x8_to_e2m1(const float (&v)[8]) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\tcvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\tcvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+        "mov.b32 %0, {a, b, c, d};\n\t}"
+        : "=r"(r)
+        : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
+    return r;
+}
+__device__ __forceinline__ void load8(const void *p, size_t e, int bf16, float (&v)[8]) {
+    if (bf16) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + e);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+        const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + e);
+        const float4 a = f[0], b = f[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+}
+
+constexpr int KVC_THREADS = 256;
+// Four lanes per 32-element block, eight elements each: a row is read and its K codes are written in whole sectors.
+// blockIdx.y: 0 K, 1 V.
+__global__ void __launch_bounds__(KVC_THREADS)
+k_kv_append(const void *__restrict__ k, const void *__restrict__ v, int bf16, long long ks, long long vs, const int *__restrict__ slots,
+            KvGeom g, long long n8) {
+    Q36_GDS();
+    const long long i = (long long)blockIdx.x * KVC_THREADS + threadIdx.x;
+    const bool is_v = blockIdx.y;
+    const int row8 = g.Hkv * g.Dh / 8;
+    const bool in = i < n8;
+    const int t = in ? (int)(i / row8) : 0, r = in ? (int)(i - (long long)t * row8) : 0;
+    const int head = r / (g.Dh / 8), c = r - head * (g.Dh / 8), b = c >> 2, j = c & 3;
+    const int slot = in ? slots[t] : -1;
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (slot >= 0) load8(is_v ? v : k, (size_t)t * (is_v ? vs : ks) + (size_t)r * 8, bf16, x);
+    float am = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        x[e] = x[e] == x[e] ? x[e] : 0.f;
+        am = fmaxf(am, fabsf(x[e]));
+    }
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
+    am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
+    if (slot < 0 || (slot >> g.log_bs) >= g.n_blocks) return;
+    const int e2 = e2_of_amax_fp4(am);
+    const float inv = inv_scale_of_e2(e2);
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] *= inv;
+    const uint32_t codes = f32x8_to_e2m1(x);
+    uint8_t *reg = const_cast<uint8_t *>(g.at(slot >> g.log_bs, head));
+    const int tok = slot & (g.bs - 1), half = g.bs * g.Dh / 2;
+    if (!is_v) {
+        *reinterpret_cast<uint32_t *>(reg + kv_k_off(tok, j, b, g.Dh)) = codes;
+    } else {
+        *reinterpret_cast<uint16_t *>(reg + half + kv_v_off(tok, 2 * j, b, g.Dh)) = (uint16_t)codes;
+        *reinterpret_cast<uint16_t *>(reg + half + kv_v_off(tok, 2 * j + 1, b, g.Dh)) = (uint16_t)(codes >> 16);
+    }
+    if (j == 0) reg[2 * half + (is_v ? g.bs * (g.Dh / 32) : 0) + tok * (g.Dh / 32) + b] = (uint8_t)(127 + e2);
+}
+
+__global__ void __launch_bounds__(KVC_THREADS)
+k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *__restrict__ v, int bf16, long long n8) {
+    Q36_GDS();
+    const long long i = (long long)blockIdx.x * KVC_THREADS + threadIdx.x;
+    if (i >= n8) return;
+    const bool is_v = blockIdx.y;
+    const int row8 = g.Hkv * g.Dh / 8;
+    const int t = (int)(i / row8), r = (int)(i - (long long)t * row8);
+    const int head = r / (g.Dh / 8), c = r - head * (g.Dh / 8), b = c >> 2, j = c & 3;
+    const int slot = slots[t];
+    uint32_t codes = 0;
+    float sc = 0.f;
+    if (slot >= 0 && (slot >> g.log_bs) < g.n_blocks) {
+        const uint8_t *reg = g.at(slot >> g.log_bs, head);
+        const int tok = slot & (g.bs - 1), half = g.bs * g.Dh / 2;
+        if (!is_v) {
+            codes = *reinterpret_cast<const uint32_t *>(reg + kv_k_off(tok, j, b, g.Dh));
+        } else {
+            codes = *reinterpret_cast<const uint16_t *>(reg + half + kv_v_off(tok, 2 * j, b, g.Dh)) |
+                    (uint32_t)*reinterpret_cast<const uint16_t *>(reg + half + kv_v_off(tok, 2 * j + 1, b, g.Dh)) << 16;
+        }
+        sc = ue8m0_to_f32(reg[2 * half + (is_v ? g.bs * (g.Dh / 32) : 0) + tok * (g.Dh / 32) + b]);
+    }
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const float2 f = e2m1x2_to_f32x2((codes >> (8 * e)) & 0xff);
+        x[2 * e] = f.x * sc;
+        x[2 * e + 1] = f.y * sc;
+    }
+    void *dst = is_v ? v : k;
+    const size_t at = (size_t)i * 8;
+    if (bf16) {      // exact: a code has two significant bits
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = (__float_as_uint(x[2 * e]) >> 16) | (__float_as_uint(x[2 * e + 1]) & 0xffff0000u);
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(dst) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + at);
+        o[0] = make_float4(x[0], x[1], x[2], x[3]);
+        o[1] = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+
+int launch_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g, int T, cudaStream_t st) {
+    const long long n8 = (long long)T * g.Hkv * g.Dh / 8;
+    launch_k(k_kv_append, dim3((unsigned)((n8 + KVC_THREADS - 1) / KVC_THREADS), 2), dim3(KVC_THREADS), 0, st, k, v, bf16, ks, vs, slots, g, n8);
+    return check_launch();
+}
+
+}  // namespace q36
+
+using namespace q36;
+
+static bool off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
+
+extern "C" {
+
+uint64_t q36_kv_block_bytes(int block_size, int n_kv_head, int head_dim) {
+    if (!kv_geom_ok(block_size, n_kv_head, head_dim)) return 0;
+    return (uint64_t)block_size * head_dim * 17 / 16 * n_kv_head;
+}
+
+int q36_kv_tables(const int *kv_old, const int *q_len, int n_seq, int block_size, int n_blocks, const int *free_blocks, int n_free,
+                  const int *free_head, int *block_table, int max_blocks, int *cu_q, int *kv_len, int *slots, int *positions, int T,
+                  int *free_head_out, int *status, void *stream) {
+    if (!kv_old || !q_len || !free_head || !block_table || !cu_q || !kv_len || !free_head_out || !status) return Q36_MOE_EINVAL;
+    if ((n_free > 0 && !free_blocks) || (T > 0 && (!slots || !positions))) return Q36_MOE_EINVAL;
+    if (n_seq <= 0 || n_seq > TB_MAX_SEQ || T < 0 || T > (1 << 29) || n_free < 0 || n_free > (1 << 29) || max_blocks <= 0 || n_blocks <= 0) return Q36_MOE_EINVAL;
+    if (!kv_geom_ok(block_size, 1, 64) || (int64_t)n_blocks * block_size > INT32_MAX || (int64_t)max_blocks * block_size > (1 << 30)) return Q36_MOE_EINVAL;
+    const int smem = 2 * (n_seq + 1) * 4;
+    static bool attr_done[MAX_DEVICES] = {false};
+    int rc;
+    if (smem > 48 * 1024 && (rc = ensure_smem_attr((const void *)k_kv_tables, 2 * (TB_MAX_SEQ + 1) * 4, attr_done))) return rc;
+    const long work = (long)T + n_seq;
+    // in place: one block, since another could read what it has written
+    const bool in_place = kv_len == kv_old || free_head_out == free_head;
+    const int grid = in_place ? 1 : (int)min((work + 2 * TB_THREADS - 1) / (2 * TB_THREADS), (long)sm_count());
+    launch_k(k_kv_tables, dim3(grid), dim3(TB_THREADS), smem, (cudaStream_t)stream, kv_old, q_len, n_seq, block_size, n_blocks, free_blocks, n_free,
+             free_head, block_table, max_blocks, cu_q, kv_len, slots, positions, T, free_head_out, status);
+    return check_launch();
+}
+
+int q36_kv_append(const void *k, const void *v, int x_is_bf16, int64_t k_stride, int64_t v_stride, const int *slots, void *cache,
+                  int n_blocks, int block_size, int n_kv_head, int head_dim, int T, void *stream) {
+    if ((T && (!k || !v || !slots)) || !cache || !kv_geom_ok(block_size, n_kv_head, head_dim) || T < 0) return Q36_MOE_EINVAL;
+    const int64_t row = (int64_t)n_kv_head * head_dim, vec = x_is_bf16 ? 8 : 4;
+    if (n_blocks <= 0 || (int64_t)n_blocks * block_size > INT32_MAX || k_stride < row || v_stride < row || k_stride % vec || v_stride % vec) return Q36_MOE_EINVAL;
+    if (off16(k) || off16(v) || off16(cache)) return Q36_MOE_EINVAL;
+    if (T == 0) return Q36_MOE_OK;
+    const KvGeom g{(const uint8_t *)cache, n_blocks, block_size, log2_of(block_size), n_kv_head, head_dim};
+    return launch_kv_append(k, v, x_is_bf16, k_stride, v_stride, slots, g, T, (cudaStream_t)stream);
+}
+
+int q36_kv_read(const void *cache, int n_blocks, int block_size, int n_kv_head, int head_dim, const int *slots, void *k, void *v,
+                int x_is_bf16, int T, void *stream) {
+    if ((T && (!k || !v || !slots)) || !cache || !kv_geom_ok(block_size, n_kv_head, head_dim) || T < 0) return Q36_MOE_EINVAL;
+    if (n_blocks <= 0 || (int64_t)n_blocks * block_size > INT32_MAX || off16(k) || off16(v) || off16(cache)) return Q36_MOE_EINVAL;
+    if (T == 0) return Q36_MOE_OK;
+    const KvGeom g{(const uint8_t *)cache, n_blocks, block_size, log2_of(block_size), n_kv_head, head_dim};
+    const long long n8 = (long long)T * n_kv_head * head_dim / 8;
+    launch_k(k_kv_read, dim3((unsigned)((n8 + KVC_THREADS - 1) / KVC_THREADS), 2), dim3(KVC_THREADS), 0, (cudaStream_t)stream, g, slots, k, v,
+             x_is_bf16, n8);
+    return check_launch();
+}
+
+}  // extern "C"

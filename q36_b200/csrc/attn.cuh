@@ -40,6 +40,20 @@ __device__ __forceinline__ void seq_span(const AttnArgs &a, int b, int &t0, int 
     len = min(max(a.kv_len[b], 0), a.max_blocks << a.kv.log_bs);
 }
 
+// eight elements from element e on
+__device__ __forceinline__ void load8(const void *p, size_t e, int bf16, float (&v)[8]) {
+    if (bf16) {
+        const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + e);
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else {
+        const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + e);
+        const float4 a = f[0], b = f[1];
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    }
+}
+
 int launch_attention(const AttnArgs &a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st);
 uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q);
 int launch_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g, int T, cudaStream_t st);

@@ -1,79 +1,76 @@
 // Attention over the paged 4-bit cache.
 #include <math.h>
 
-#include "attn.cuh"
+#include "attn_plan.cuh"
 
 namespace q36 {
 
-constexpr int SA_THREADS = 128;
+constexpr int JOIN_THREADS = 128;
 
-// One block per (row, query head): each warp takes every fourth token and keeps its own running maximum and sum.
+// Block (i, y): row y of the span whose first piece CTA i had, if it had one of a cut span.  Piece p counts l_p 2^(m_p - m).
 template <int DH>
-__global__ void __launch_bounds__(SA_THREADS) k_attn_simple(AttnArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS)
+k_attn_join(AttnArgs a, int tile_rows, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
     Q36_GDS();
-    constexpr int NB = DH / 32;
-    __shared__ float qs[DH], sm_o[4][DH], sm_m[4], sm_l[4];
-    const int t = blockIdx.x, hq = blockIdx.y, hk = hq / a.G, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int b = -1, t0 = 0, n = 0, len = 0;
-    for (int s = 0; s < a.B; s++) {
-        seq_span(a, s, t0, n, len);
-        if (t >= t0 && t < t0 + n) { b = s; break; }
-    }
-    if (b < 0) return;
-    const int pos = len - n + (t - t0), lo = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-    for (int d = tid; d < DH; d += SA_THREADS) {
-        const size_t e = (size_t)t * a.q_stride + (size_t)hq * DH + d;
-        qs[d] = (a.q_bf16 ? __uint_as_float((uint32_t)reinterpret_cast<const uint16_t *>(a.q)[e] << 16) : reinterpret_cast<const float *>(a.q)[e]) * a.scale2;
-    }
+    constexpr int C4 = DH / 4, LANES = JOIN_THREADS / C4;      // threads over the dims, and pieces in parallel
+    extern __shared__ float w[];                               // one weight per piece
+    __shared__ float red[JOIN_THREADS / 32];
+    __shared__ float4 acc[LANES][C4];
+    const AttnPart d = desc[blockIdx.x];
+    const int r = blockIdx.y, tid = threadIdx.x;
+    if (d.parts == 0 || d.rt * tile_rows + r >= d.n * a.G) return;
+    const int stride = attn_part_floats(tile_rows, DH);
+    auto slot = [&](int p) { return part + (size_t)(p == 0 ? d.slot : 2 * ((int)blockIdx.x + p)) * stride; };
+    float m = -3.0e38f;
+    for (int p = tid; p < d.parts; p += JOIN_THREADS) m = fmaxf(m, slot(p)[2 * r]);
+    m = warp_max(m);
+    if ((tid & 31) == 0) red[tid >> 5] = m;
     __syncthreads();
-    float m = -INFINITY, l = 0.f, o[NB] = {};
-    for (int j = lo + warp; j <= pos; j += 4) {
-        const int blk = a.table[(size_t)b * a.max_blocks + (j >> a.kv.log_bs)];
-        if (blk < 0 || blk >= a.kv.n_blocks) continue;
-        const uint8_t *reg = a.kv.at(blk, hk);
-        const int tok = j & (a.kv.bs - 1), half = a.kv.bs * DH / 2;
-        float s = 0.f, v[NB];
-#pragma unroll
-        for (int c = 0; c < NB; c++) {     // lane = dim inside block c
-            const uint8_t kb = reg[kv_k_off(tok, lane >> 3, c, DH) + ((lane & 7) >> 1)];
-            const uint8_t vb = reg[half + kv_v_off(tok, lane >> 2, c, DH) + ((lane & 3) >> 1)];
-            const float2 kf = e2m1x2_to_f32x2(kb), vf = e2m1x2_to_f32x2(vb);
-            s += qs[32 * c + lane] * ((lane & 1) ? kf.y : kf.x) * ue8m0_to_f32(reg[2 * half + tok * NB + c]);
-            v[c] = ((lane & 1) ? vf.y : vf.x) * ue8m0_to_f32(reg[2 * half + a.kv.bs * NB + tok * NB + c]);
-        }
-        s = warp_sum(s);
-        const float mn = fmaxf(m, s), f = exp2f(m - mn), p = exp2f(s - mn);
-        m = mn;
-        l = l * f + p;
-#pragma unroll
-        for (int c = 0; c < NB; c++) o[c] = o[c] * f + p * v[c];
-    }
-#pragma unroll
-    for (int c = 0; c < NB; c++) sm_o[warp][32 * c + lane] = o[c];
-    if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
+    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     __syncthreads();
-    float M = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3])), L = 0.f, w[4];
-    for (int i = 0; i < 4; i++) { w[i] = M == -INFINITY ? 0.f : exp2f(sm_m[i] - M); L += w[i] * sm_l[i]; }
-    for (int d = tid; d < DH; d += SA_THREADS) {
-        float acc = 0.f;
-        for (int i = 0; i < 4; i++) acc += w[i] * sm_o[i][d];
-        acc = L > 0.f ? acc / L : 0.f;
-        const size_t e = (size_t)t * a.o_stride + (size_t)hq * DH + d;
-        if (a.o_bf16) reinterpret_cast<__nv_bfloat16 *>(a.out)[e] = __float2bfloat16_rn(acc);
-        else reinterpret_cast<float *>(a.out)[e] = acc;
+    float l = 0.f;
+    for (int p = tid; p < d.parts; p += JOIN_THREADS) {
+        const float *s = slot(p);
+        l += w[p] = s[2 * r + 1] * exp2f(s[2 * r] - m);
     }
-    if (a.lse && tid == 0) a.lse[(size_t)t * a.Hq + hq] = L > 0.f ? (M + log2f(L)) * 0.6931471805599453f : -INFINITY;
+    l = warp_sum(l);
+    if ((tid & 31) == 0) red[tid >> 5] = l;
+    __syncthreads();
+    l = red[0] + red[1] + red[2] + red[3];
+    const int c = tid % C4, lane = tid / C4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = lane; p < d.parts; p += LANES) {
+        const float4 v = *reinterpret_cast<const float4 *>(slot(p) + 2 * tile_rows + r * DH + 4 * c);
+        const float f = w[p];
+        o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+    }
+    acc[lane][c] = o;
+    __syncthreads();
+    if (lane == 0) {
+#pragma unroll
+        for (int i = 1; i < LANES; i++) { const float4 v = acc[i][c]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        attn_store(a, d.b_t0, d.n, d.hk, d.rt * tile_rows + r, 4 * c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+        if (c == 0) attn_store_lse(a, d.b_t0, d.n, d.hk, d.rt * tile_rows + r, m, l);
+    }
 }
 
-uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) { (void)Hq; (void)Hkv; (void)Dh; (void)max_q; return 256; }
+int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st) {
+    const dim3 blocks(grid, tile_rows), threads(JOIN_THREADS);
+    if (a.kv.Dh == 64) launch_k(k_attn_join<64>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
+    else if (a.kv.Dh == 128) launch_k(k_attn_join<128>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
+    else launch_k(k_attn_join<256>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
+    return check_launch();
+}
+
+static int rows_of(int Hq, int Hkv, int max_q) { return (int)min((long)(Hq / Hkv) * max_q, (long)INT32_MAX); }
+
+uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) { return decode_ws_bytes(Dh, rows_of(Hq, Hkv, max_q)); }
 
 int launch_attention(const AttnArgs &a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st) {
-    (void)max_q; (void)ws; (void)ws_bytes;
-    const dim3 grid(a.T, a.Hq), block(SA_THREADS);
-    if (a.kv.Dh == 64) launch_k(k_attn_simple<64>, grid, block, 0, st, a);
-    else if (a.kv.Dh == 128) launch_k(k_attn_simple<128>, grid, block, 0, st, a);
-    else launch_k(k_attn_simple<256>, grid, block, 0, st, a);
-    return check_launch();
+    (void)ws_bytes;
+    return launch_decode(a, rows_of(a.Hq, a.kv.Hkv, max_q), INT32_MAX, ws, st);
 }
 
 }  // namespace q36

@@ -148,19 +148,6 @@ __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float (&v)[8]) {
         : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
-__device__ __forceinline__ void load8(const void *p, size_t e, int bf16, float (&v)[8]) {
-    if (bf16) {
-        const uint4 u = *reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(p) + e);
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    } else {
-        const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(p) + e);
-        const float4 a = f[0], b = f[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-    }
-}
-
 constexpr int KVC_THREADS = 256;
 // Four lanes per 32-element block, eight elements each: a row is read and its K codes are written in whole sectors.
 // blockIdx.y: 0 K, 1 V.

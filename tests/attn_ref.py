@@ -42,8 +42,8 @@ def region_bytes(kc, ks, vc, vs):
 
 
 def attention(q, k, v, n, scale, window=0, drop=None):
-    """Rows q [n, Hq, Dh] over k, v [len, Hkv, Dh] -> (out, lse, A, delta) with A = softmax-weighted |v| and delta = the
-    largest scaled sum of |q||k| of a row: what the error bounds are made of.  drop [len]: tokens left out."""
+    """Rows q [n, Hq, Dh] over k, v [len, Hkv, Dh] -> (out, lse, A, delta, V) with A = softmax-weighted |v|, delta = the largest
+    sum of |q||k| of a row, V = the sum of |v| over the tokens a row sees: what the error bounds are made of.  drop [len]: tokens left out."""
     q, k, v = (np.asarray(x, np.float64) for x in (q, k, v))
     L, Hkv = k.shape[:2]
     Hq, Dh = q.shape[1:]
@@ -56,7 +56,7 @@ def attention(q, k, v, n, scale, window=0, drop=None):
     if drop is not None:
         seen &= ~drop[None]
     out, lse = np.zeros((n, Hq, Dh)), np.full((n, Hq), -np.inf)
-    A, delta = np.zeros((n, Hq, Dh)), np.zeros((n, Hq))
+    A, delta, V = np.zeros((n, Hq, Dh)), np.zeros((n, Hq)), np.zeros((n, Hq, Dh))
     for h in range(Hq):
         kk, vv = k[:, h // G], v[:, h // G]
         s = np.where(seen, q[:, h] @ kk.T * scale, -np.inf)
@@ -66,8 +66,9 @@ def attention(q, k, v, n, scale, window=0, drop=None):
         l = p.sum(-1, keepdims=True)
         out[ok, h], A[ok, h] = p @ vv / l, p @ np.abs(vv) / l
         lse[ok, h] = m[ok] + np.log(l[:, 0])
+        V[:, h] = seen @ np.abs(vv)
         delta[:, h] = np.where(seen, np.abs(q[:, h]) @ np.abs(kk).T * scale, 0).max(-1, initial=0)
-    return out, lse, A, delta
+    return out, lse, A, delta, V
 
 
 def tables(old, new, bs, free, head, table, T, n_blocks):

@@ -8,6 +8,9 @@ its reference does too.  With |q.k| the sum of |q_d k_d| and A the softmax-weigh
   (n + 64) 2^-24; numerator and denominator both: twice that, times A.
   bf16 inputs: the weights are rounded once for the product with V (half a step of bf16: 2^-8 A, which covers f16's 2^-11),
   and the output is (2^-8 of the value).
+  small weights: f16 has no step finer than 2^-24, so a weight w against a largest one of 2^7 is off by up to 2^-25 before and
+  2^-25 after its factor f = 2^(exponent of v - anchor), 2^-8 <= f <= 2^4.  That is 2^-25 (1 + f) / f |v| <= 2^-24 2^7 |v| of a
+  normaliser of at least 2^7: 2^-24 |v| for every token seen, which shows where the strong tokens' v are 0.
 """
 import itertools
 
@@ -203,10 +206,10 @@ class Setup:
         t0 = j0 = 0
         for b, (n, kv) in enumerate(self.lens):
             if rows is None or b in rows:
-                o, l, A, d = R.attention(q[t0:t0 + n], self.k[j0:j0 + kv], self.v[j0:j0 + kv], n, scale, window, None if drop is None else drop[b])
+                o, l, A, d, V = R.attention(q[t0:t0 + n], self.k[j0:j0 + kv], self.v[j0:j0 + kv], n, scale, window, None if drop is None else drop[b])
                 d = abs(d) * abs(scale) * (self.Dh + 8) * 2.0 ** -24
                 sums = (kv + 64) * 2.0 ** -24
-                tol = A * (2 * (4 * d + 2.0 ** -20 + sums))[..., None] + 1e-30
+                tol = A * (2 * (4 * d + 2.0 ** -20 + sums))[..., None] + 2.0 ** -24 * V + 1e-30
                 tol += 2.0 ** -8 * (np.abs(o) + A) if self.x == "bf16" else 2.0 ** -24 * np.abs(o)
                 err = np.abs(out[t0:t0 + n] - o)
                 assert (err <= tol).all(), (b, n, kv, float((err / tol).max()))
@@ -275,11 +278,10 @@ def test_rows_that_see_nothing(attn, x):
         s = Setup(attn, rng, [(nq, 3), (1, 0), (nq, 0), (2, 50), (nq, 40)], 16, 2, 128, 16, x)
         s.check(s.run())
     s = Setup(attn, rng, [(1, 30), (1, 48)], 16, 2, 128, 16, x)
-    want = s.run()
     s.kv_len = ints([-5, 1 << 30])
     out, lse = s.run()
     assert (out[0] == 0).all() and (lse[0] == -torch.inf).all()
-    assert torch.equal(out[1], want[0][1]) and torch.equal(lse[1], want[1][1])     # cut at the table's width: 48 tokens
+    s.check((out, lse), rows=[1])                                                  # cut at the table's width: 48 tokens
 
 
 @pytest.mark.parametrize("x", ["bf16", "f32"])
@@ -490,7 +492,7 @@ def test_decoding_steps_of_a_layer(attn, moe):
             keys[b].append([R.quantise(bufs[x][r].float().cpu().numpy())[2] for x in ("k", "v")])
             k, v = (np.concatenate([p[i] for p in keys[b]]) for i in (0, 1))
             assert int(out.kv_len[b]) == len(k)
-            o, _, A, _ = R.attention(bufs["q"][r].double().cpu().numpy(), k, v, nb, Dh ** -0.5)
+            o, _, A, _, _ = R.attention(bufs["q"][r].double().cpu().numpy(), k, v, nb, Dh ** -0.5)
             w = w_o.double().cpu().numpy()
             want[r] += o.reshape(nb, Hq * Dh) @ w.T
             tol[r] = (2.0 ** -8 * (np.abs(o) + A) * 1.02).reshape(nb, Hq * Dh) @ np.abs(w).T + 1e-5 * (1 + np.abs(want[r]))

@@ -1,5 +1,6 @@
 // y = act(x W^T + bias) + residual, bf16 operands, f32 sums.
 #include "attn.cuh"
+#include "tc_ptx.cuh"
 
 namespace q36 {
 
@@ -11,50 +12,390 @@ struct Epilogue {
     long long rs, ys;
     int act, res_bf16, y_bf16;
 };
-__device__ __forceinline__ float activate(float v, int act) {
+// An activation over N sums (the choice outside the loop).  x / (1 + e^-x) with e^-x kept finite: beyond 2^100 the quotient
+// is below any f32 step of the result's neighbours.  0.5 (1 + tanh u) = 1 / (1 + e^-2u).
+__device__ __forceinline__ float over_1p_exp(float x, float u) { return __fdividef(x, 1.f + fminf(__expf(-u), 1.2676506e30f)); }
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
     switch (act) {
-        case Q36_ACT_RELU: return v < 0.f ? 0.f : v;
-        case Q36_ACT_SILU: return v / (1.f + expf(-v));
-        case Q36_ACT_GELU: return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-        case Q36_ACT_GELU_TANH: return 0.5f * v * (1.f + tanhf(0.79788456080286536f * (v + 0.044715f * v * v * v)));
-        default: return v;
+        case Q36_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
+            break;
+        case Q36_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = over_1p_exp(v[i], v[i]);
+            break;
+        case Q36_ACT_GELU:
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = 0.5f * v[i] * (1.f + erff(v[i] * 0.70710678118654752f));
+            break;
+        case Q36_ACT_GELU_TANH:
+#pragma unroll
+            for (int i = 0; i < N; i++) v[i] = over_1p_exp(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+            break;
+        default: break;
     }
 }
-__device__ __forceinline__ void finish(const Epilogue &e, int t, int n, float v) {
-    if (e.bias) v += e.bias[n];
-    v = activate(v, e.act);
+// Sums of column n, rows t .. t + N - 1 (those below `rows`), to their place.
+template <int N>
+__device__ __forceinline__ void finish(const Epilogue &e, int n, float bias, int t, int rows, float (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] += bias;
+    float r[N];
     if (e.res) {
-        const size_t i = (size_t)t * e.rs + n;
-        v += e.res_bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16 *>(e.res)[i]) : reinterpret_cast<const float *>(e.res)[i];
+        if (e.res_bf16) {
+            const __nv_bfloat16 *p = reinterpret_cast<const __nv_bfloat16 *>(e.res) + (size_t)t * e.rs + n;
+#pragma unroll
+            for (int i = 0; i < N; i++, p += e.rs) r[i] = t + i < rows ? __bfloat162float(*p) : 0.f;
+        } else {
+            const float *p = reinterpret_cast<const float *>(e.res) + (size_t)t * e.rs + n;
+#pragma unroll
+            for (int i = 0; i < N; i++, p += e.rs) r[i] = t + i < rows ? *p : 0.f;
+        }
     }
-    const size_t i = (size_t)t * e.ys + n;
-    if (e.y_bf16) reinterpret_cast<__nv_bfloat16 *>(e.y)[i] = __float2bfloat16_rn(v);
-    else reinterpret_cast<float *>(e.y)[i] = v;
+    activate(v, e.act);
+    if (e.res) {
+#pragma unroll
+        for (int i = 0; i < N; i++) v[i] += r[i];
+    }
+    if (e.y_bf16) {
+        __nv_bfloat16 *p = reinterpret_cast<__nv_bfloat16 *>(e.y) + (size_t)t * e.ys + n;
+#pragma unroll
+        for (int i = 0; i < N; i++, p += e.ys)
+            if (t + i < rows) *p = __float2bfloat16_rn(v[i]);
+    } else {
+        float *p = reinterpret_cast<float *>(e.y) + (size_t)t * e.ys + n;
+#pragma unroll
+        for (int i = 0; i < N; i++, p += e.ys)
+            if (t + i < rows) *p = v[i];
+    }
 }
 
-// 16 x 16 outputs per block, K in steps of 16.
-__global__ void __launch_bounds__(256)
-k_linear_simple(const uint16_t *__restrict__ x, long long xs, const uint16_t *__restrict__ w, Epilogue e, int T, int N, int K, const int *rows_used) {
+// ---------------------------------------------------------------- few rows: the weights' stream
+// Up to 16 rows.  A block has 16 columns of y (rows of W) and splits K over its warps; a lane reads 16 bytes of two rows of W
+// and of one row of x, which is a fragment of m16n8k16 with k permuted alike on both sides.
+constexpr int LS_WARPS = 8, LS_THREADS = 32 * LS_WARPS, LS_COLS = 16;
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+template <int NT>
+__global__ void __launch_bounds__(LS_THREADS)
+k_linear_few(const uint16_t *__restrict__ x, long long xs, const uint16_t *__restrict__ w, Epilogue e, int T, int N, int K, const int *rows_used) {
+    constexpr int U = 4;      // steps of 32 k in flight
     Q36_GDS();
-    __shared__ float sx[16][17], sw[16][17];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, n0 = blockIdx.x * 16, t0 = blockIdx.y * 16;
-    const int rows = rows_used ? min(T, *rows_used) : T;
-    float acc = 0.f;
-    for (int k0 = 0; k0 < K; k0 += 16) {
-        sx[ty][tx] = (t0 + ty < rows && k0 + tx < K) ? __uint_as_float((uint32_t)x[(size_t)(t0 + ty) * xs + k0 + tx] << 16) : 0.f;
-        sw[ty][tx] = (n0 + ty < N && k0 + tx < K) ? __uint_as_float((uint32_t)w[(size_t)(n0 + ty) * K + k0 + tx] << 16) : 0.f;
-        __syncthreads();
-        for (int k = 0; k < 16; k++) acc = fmaf(sx[ty][k], sw[tx][k], acc);
-        __syncthreads();
+    __shared__ float red[LS_WARPS][8 * NT][LS_COLS + 1];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
+    const int n0 = blockIdx.x * LS_COLS, rows = rows_used ? min(T, *rows_used) : T;
+    const int steps = (K + 31) / 32;
+    const uint16_t *wp[2] = {w + (size_t)min(n0 + g, N - 1) * K + 8 * j, w + (size_t)min(n0 + g + 8, N - 1) * K + 8 * j};
+    const uint16_t *xp[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) xp[nt] = x + (size_t)min(nt * 8 + g, T - 1) * xs + 8 * j;
+    float c[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) c[nt][i] = 0.f;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    for (int s0 = warp; s0 < steps; s0 += LS_WARPS * U) {
+        uint4 a[U][2], b[U][NT];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = (s0 + u * LS_WARPS) * 32;
+            const bool in = k + 8 * j < K;     // K is a multiple of 8
+#pragma unroll
+            for (int h = 0; h < 2; h++) a[u][h] = in ? __ldcs(reinterpret_cast<const uint4 *>(wp[h] + k)) : zero;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) b[u][nt] = in ? *reinterpret_cast<const uint4 *>(xp[nt] + k) : zero;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                mma_bf16(c[nt], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][nt].x, b[u][nt].y);
+                mma_bf16(c[nt], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][nt].z, b[u][nt].w);
+            }
     }
-    if (t0 + ty < rows && n0 + tx < N) finish(e, t0 + ty, n0 + tx, acc);
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) red[warp][nt * 8 + 2 * j + (i & 1)][g + 8 * (i >> 1)] = c[nt][i];
+    __syncthreads();
+    if (tid < 8 * NT * LS_COLS) {
+        const int t = tid / LS_COLS, n = tid % LS_COLS;
+        float v[1] = {0.f};
+#pragma unroll
+        for (int k = 0; k < LS_WARPS; k++) v[0] += red[k][t][n];
+        if (t < rows && n0 + n < N) finish(e, n0 + n, e.bias ? e.bias[n0 + n] : 0.f, t, rows, v);
+    }
+}
+
+// ---------------------------------------------------------------- tiles on tcgen05
+// A tile is 128 columns of y (rows of W, the 128 lanes of the accumulator) by BN rows (its columns): in the epilogue a thread is
+// one column of y, so that bias is a register and a warp's accesses to residual and y are 32 neighbours.
+// SPLIT > 1: a cluster shares a tile, each CTA a part of K; the parts are added in rank order over distributed shared memory.
+constexpr int LT_M = 128, LT_K = 64, LT_EPI_WARPS = 8, LT_THREADS = 32 * (2 + LT_EPI_WARPS);
+template <int BN>
+struct LtCfg {
+    static constexpr int STAGE = LT_M * LT_K * 2 + BN * LT_K * 2;
+    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int SMEM = STAGE * STAGES + 1024;
+};
+struct LtMaps { CUtensorMap w, x; };
+__device__ int g_linear_status;      // where a wait gave up (0: nowhere)
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
+    float v;
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+
+template <int BN, int SPLIT>
+__global__ void __launch_bounds__(LT_THREADS, 1)
+k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K, const int *rows_used, int t_tiles, int n_tiles) {
+    using C = LtCfg<BN>;
+    constexpr int TM_COLS = SPLIT == 1 ? 2 * BN : BN;
+    constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(LT_M >> 4) << 24);
+    Q36_GDS();
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    __shared__ uint64_t full_b[C::STAGES], empty_b[C::STAGES], acc_full_b[2], acc_empty_b[2];
+    __shared__ uint32_t tmem_s;
+    __shared__ volatile int abort_flag;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t full0 = smem_u32(full_b), empty0 = smem_u32(empty_b), accf0 = smem_u32(acc_full_b), acce0 = smem_u32(acc_empty_b);
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < C::STAGES; i++) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(accf0 + 8 * i, 1); mbar_init(acce0 + 8 * i, LT_EPI_WARPS); }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(TM_COLS) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;
+    const int rows = rows_used ? min(T, *rows_used) : T;
+    const int tiles = t_tiles * n_tiles, all_steps = (K + LT_K - 1) / LT_K;
+    const int rank = SPLIT == 1 ? 0 : (int)(blockIdx.x % SPLIT);
+    const int k0 = all_steps * rank / SPLIT, k_steps = all_steps * (rank + 1) / SPLIT - k0;
+    const int first = SPLIT == 1 ? blockIdx.x : blockIdx.x / SPLIT, step = SPLIT == 1 ? gridDim.x : tiles;
+    // Order of tiles: eight row tiles by all column tiles at a time, rows fastest, so that what runs at one time shares W and x in L2.
+    auto place = [&](int i, int &n0, int &t0) {
+        constexpr int GT = 8;
+        const int grp = i / (GT * n_tiles), in = i - grp * GT * n_tiles, gt = min(GT, t_tiles - grp * GT);
+        n0 = in / gt * LT_M;
+        t0 = (grp * GT + in % gt) * BN;
+    };
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            for (int i = first; i < tiles && ok; i += step) {
+                int n0, t0;
+                place(i, n0, t0);
+                if (t0 >= rows) continue;
+                for (int k = 0; k < k_steps; k++, it++) {
+                    const uint32_t s = it % C::STAGES, ph = (it / C::STAGES) & 1;
+                    if (!(ok = mbar_wait(empty0 + 8 * s, ph ^ 1, &abort_flag, &g_linear_status, 0x100 + s, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                    const uint32_t sa = smem_u32(smem + s * C::STAGE);
+                    mbar_expect_tx(full0 + 8 * s, C::STAGE);
+                    tma_load_2d(sa, &maps.w, (k0 + k) * LT_K, n0, full0 + 8 * s);
+                    tma_load_2d(sa + LT_M * LT_K * 2, &maps.x, (k0 + k) * LT_K, t0, full0 + 8 * s);
+                }
+            }
+            // gave up: let the copies in flight land before the block ends
+            if (!ok)
+                for (uint32_t i = it > C::STAGES ? it - C::STAGES : 0; i < it; i++)
+                    for (uint32_t n = 0; n < TC_SPIN_LIMIT && !mbar_try(full0 + 8 * (i % C::STAGES), (i / C::STAGES) & 1); n++) {}
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            uint32_t it = 0, tc = 0;
+            bool ok = true;
+            for (int i = first; i < tiles && ok; i += step) {
+                int n0, t0;
+                place(i, n0, t0);
+                if (t0 >= rows) continue;
+                const uint32_t buf = SPLIT == 1 ? tc & 1 : 0;
+                if (!(ok = mbar_wait(acce0 + 8 * buf, ((tc >> 1) & 1) ^ 1, &abort_flag, &g_linear_status, 0x200 + buf))) break;
+                tc_fence_after();
+                for (int k = 0; k < k_steps; k++, it++) {
+                    const uint32_t s = it % C::STAGES, ph = (it / C::STAGES) & 1;
+                    if (!(ok = mbar_wait(full0 + 8 * s, ph, &abort_flag, &g_linear_status, 0x300 + s))) break;
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(smem + s * C::STAGE);
+#pragma unroll
+                    for (int kk = 0; kk < LT_K / 16; kk++)
+                        mma_f16_ss(tmem + buf * BN, desc_sw128(sa + kk * 32), desc_sw128(sa + LT_M * LT_K * 2 + kk * 32), IDESC, (k | kk) ? 1u : 0u);
+                    tc_commit(empty0 + 8 * s);
+                }
+                if (ok) tc_commit(accf0 + 8 * buf);
+                tc++;
+            }
+        }
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        uint32_t tc = 0;
+        for (int i = first; i < tiles; i += step) {
+            int n0, t0;
+            place(i, n0, t0);
+            if (t0 >= rows) continue;
+            const uint32_t buf = SPLIT == 1 ? tc & 1 : 0;
+            if (!mbar_wait(accf0 + 8 * buf, SPLIT == 1 ? (tc >> 1) & 1 : 0, &abort_flag, &g_linear_status, 0x400 + buf, TC_SPIN_LIMIT, TC_BACKOFF_NS)) break;
+            __syncwarp();
+            tc_fence_after();
+            const int n = n0 + 32 * q + lane;
+            const float bias = e.bias && n < N ? e.bias[n] : 0.f;
+#pragma unroll 1
+            for (int c = half * (BN / 2); c < (half + 1) * (BN / 2); c += 16) {
+                if (SPLIT == 1 && t0 + c >= rows) break;
+                uint32_t r[16];
+                tc_ld16(tmem + buf * BN + ((uint32_t)(32 * q) << 16) + c, r);
+                tc_ld_wait();
+                float v[16];
+#pragma unroll
+                for (int x = 0; x < 16; x++) v[x] = __uint_as_float(r[x]);
+                if constexpr (SPLIT == 1) {
+                    if (n < N) finish(e, n, bias, t0 + c, rows, v);
+                } else {
+                    // every MMA of this CTA is over: the stages are free to hold its sums, [row][column]
+                    float *p = reinterpret_cast<float *>(smem) + c * LT_M + 32 * q + lane;
+#pragma unroll
+                    for (int x = 0; x < 16; x++) p[x * LT_M] = v[x];
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acce0 + 8 * buf);
+            tc++;
+        }
+    }
+    if constexpr (SPLIT > 1) {
+        cluster_sync();
+        int n0, t0;
+        place(first, n0, t0);
+        if (warp >= 2 && t0 < rows && !abort_flag) {
+            const int f = (tid - 64) % LT_M, half = (tid - 64) / LT_M, n = n0 + f;
+            constexpr int PER = BN / SPLIT;       // rows of the tile this CTA finishes, by two groups of threads
+            constexpr int CH = PER >= 16 ? 8 : PER / 2;
+            const float bias = e.bias && n < N ? e.bias[n] : 0.f;
+            for (int c = rank * PER + half * (PER / 2); c < rank * PER + (half + 1) * (PER / 2); c += CH) {
+                if (t0 + c >= rows) break;
+                float v[CH];
+#pragma unroll
+                for (int x = 0; x < CH; x++) {
+                    float part[SPLIT];
+#pragma unroll
+                    for (int r = 0; r < SPLIT; r++) part[r] = ld_cluster(smem_u32(smem) + ((c + x) * LT_M + f) * 4, r);
+                    v[x] = part[0];
+#pragma unroll
+                    for (int r = 1; r < SPLIT; r++) v[x] += part[r];
+                }
+                if (n < N) finish(e, n, bias, t0 + c, rows, v);
+            }
+        }
+        cluster_sync();      // nobody leaves while its sums are read
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
+}
+
+static int make_map_bf16(CUtensorMap *m, const void *base, long rows, long cols, long long stride, int box_rows) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static Encode fn = nullptr;
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return Q36_MOE_ECUDA;
+        fn = (Encode)p;
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)stride * 2};
+    const cuuint32_t box[2] = {LT_K, (cuuint32_t)box_rows}, el[2] = {1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void *>(base), dims, strides, box, el, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { last_cuda_error() = 100000 + (int)r; return Q36_MOE_ECUDA; }
+    return Q36_MOE_OK;
+}
+
+template <int BN, int SPLIT>
+static int run_tc(const LtMaps &maps, const Epilogue &e, int T, int N, int K, const int *rows_used, cudaStream_t st) {
+    using C = LtCfg<BN>;
+    static bool attr_done[MAX_DEVICES] = {false};
+    int rc;
+    if ((rc = ensure_smem_attr((const void *)k_linear_tc<BN, SPLIT>, C::SMEM, attr_done))) return rc;
+    const int t_tiles = (T + BN - 1) / BN, n_tiles = (N + LT_M - 1) / LT_M;
+    const long tiles = (long)t_tiles * n_tiles;
+    if (SPLIT == 1) {
+        launch_k(k_linear_tc<BN, SPLIT>, dim3((unsigned)min(tiles, (long)sm_count())), dim3(LT_THREADS), C::SMEM, st, maps, e, T, N, K, rows_used, t_tiles, n_tiles);
+        return check_launch();
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(tiles * SPLIT));
+    cfg.blockDim = dim3(LT_THREADS);
+    cfg.dynamicSmemBytes = C::SMEM;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = SPLIT;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, k_linear_tc<BN, SPLIT>, maps, e, T, N, K, rows_used, t_tiles, n_tiles);
+    return check_launch();
+}
+template <int BN>
+static int run_split(int split, const LtMaps &maps, const Epilogue &e, int T, int N, int K, const int *rows_used, cudaStream_t st) {
+    if (split == 8) return run_tc<BN, 8>(maps, e, T, N, K, rows_used, st);
+    if (split == 4) return run_tc<BN, 4>(maps, e, T, N, K, rows_used, st);
+    if (split == 2) return run_tc<BN, 2>(maps, e, T, N, K, rows_used, st);
+    return run_tc<BN, 1>(maps, e, T, N, K, rows_used, st);
 }
 
 int launch_linear(const void *x, long long xs, const void *w, const float *bias, int act, const void *res, int res_bf16, long long rs,
                   void *y, int y_bf16, long long ys, int T, int N, int K, const int *rows_used, cudaStream_t st) {
     const Epilogue e{bias, res, y, rs, ys, act, res_bf16, y_bf16};
-    launch_k(k_linear_simple, dim3((N + 15) / 16, (T + 15) / 16), dim3(256), 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
-    return check_launch();
+    if (T <= 16) {
+        const dim3 grid((N + LS_COLS - 1) / LS_COLS), block(LS_THREADS);
+        if (T <= 8) launch_k(k_linear_few<1>, grid, block, 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
+        else launch_k(k_linear_few<2>, grid, block, 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
+        return check_launch();
+    }
+    const int bn = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+    // K is split while a cluster's CTAs still find an SM each and have two steps of 64 at least
+    const long tiles = (long)((T + bn - 1) / bn) * ((N + LT_M - 1) / LT_M);
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sm_count() && (K + LT_K - 1) / LT_K >= split * 4) split *= 2;
+    LtMaps maps;
+    int rc;
+    if ((rc = make_map_bf16(&maps.w, w, N, K, K, LT_M)) || (rc = make_map_bf16(&maps.x, x, T, K, xs, bn))) return rc;
+    if (bn == 32) return run_split<32>(split, maps, e, T, N, K, rows_used, st);
+    if (bn == 64) return run_split<64>(split, maps, e, T, N, K, rows_used, st);
+    if (bn == 128) return run_split<128>(split, maps, e, T, N, K, rows_used, st);
+    return run_split<256>(split, maps, e, T, N, K, rows_used, st);
+}
+
+// Where a bounded wait of the tile kernel gave up since the process began (0: nowhere).
+int linear_wait_status(int *out, cudaStream_t st) {
+    if (cudaMemcpyFromSymbolAsync(out, g_linear_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess) return check_launch();
+    return cudaStreamSynchronize(st) == cudaSuccess ? Q36_MOE_OK : check_launch();
 }
 
 }  // namespace q36

@@ -73,7 +73,7 @@ __device__ __forceinline__ void finish(const Epilogue &e, int n, float bias, int
 }
 
 // ---------------------------------------------------------------- few rows: the weights' stream
-// Up to 16 rows.  A block has 16 columns of y (rows of W) and splits K over its warps; a lane reads 16 bytes of two rows of W
+// Up to 8 rows.  A block has 16 columns of y (rows of W) and splits K over its warps; a lane reads 16 bytes of two rows of W
 // and of one row of x, which is a fragment of m16n8k16 with k permuted alike on both sides.
 constexpr int LS_WARPS = 8, LS_THREADS = 32 * LS_WARPS, LS_COLS = 16;
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -81,50 +81,47 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-template <int NT>
+__device__ __forceinline__ void prefetch_l2(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __global__ void __launch_bounds__(LS_THREADS)
 k_linear_few(const uint16_t *__restrict__ x, long long xs, const uint16_t *__restrict__ w, Epilogue e, int T, int N, int K, const int *rows_used) {
-    constexpr int U = 4;      // steps of 32 k in flight
-    Q36_GDS();
-    __shared__ float red[LS_WARPS][8 * NT][LS_COLS + 1];
+    constexpr int U = 8;      // steps of 32 k in flight
+    cudaTriggerProgrammaticLaunchCompletion();
+    __shared__ float red[LS_WARPS][8][LS_COLS + 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
-    const int n0 = blockIdx.x * LS_COLS, rows = rows_used ? min(T, *rows_used) : T;
+    const int n0 = blockIdx.x * LS_COLS;
     const int steps = (K + 31) / 32;
     const uint16_t *wp[2] = {w + (size_t)min(n0 + g, N - 1) * K + 8 * j, w + (size_t)min(n0 + g + 8, N - 1) * K + 8 * j};
-    const uint16_t *xp[NT];
+    // the first round of W on its way to L2 while the launch before this one runs (a hint: nothing is read yet)
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++) xp[nt] = x + (size_t)min(nt * 8 + g, T - 1) * xs + 8 * j;
-    float c[NT][4];
-#pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) c[nt][i] = 0.f;
+    for (int u = 0; u < U; u++) {
+        const int k = (warp + u * LS_WARPS) * 32;
+        if (k + 8 * j < K) { prefetch_l2(wp[0] + k); prefetch_l2(wp[1] + k); }
+    }
+    cudaGridDependencySynchronize();
+    const int rows = rows_used ? min(T, *rows_used) : T;
+    const uint16_t *xp = x + (size_t)min(g, T - 1) * xs + 8 * j;
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
     const uint4 zero = make_uint4(0, 0, 0, 0);
     for (int s0 = warp; s0 < steps; s0 += LS_WARPS * U) {
-        uint4 a[U][2], b[U][NT];
+        uint4 a[U][2], b[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int k = (s0 + u * LS_WARPS) * 32;
             const bool in = k + 8 * j < K;     // K is a multiple of 8
 #pragma unroll
             for (int h = 0; h < 2; h++) a[u][h] = in ? __ldcs(reinterpret_cast<const uint4 *>(wp[h] + k)) : zero;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) b[u][nt] = in ? *reinterpret_cast<const uint4 *>(xp[nt] + k) : zero;
+            b[u] = in ? *reinterpret_cast<const uint4 *>(xp + k) : zero;
         }
 #pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                mma_bf16(c[nt], a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u][nt].x, b[u][nt].y);
-                mma_bf16(c[nt], a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u][nt].z, b[u][nt].w);
-            }
+        for (int u = 0; u < U; u++) {
+            mma_bf16(c, a[u][0].x, a[u][1].x, a[u][0].y, a[u][1].y, b[u].x, b[u].y);
+            mma_bf16(c, a[u][0].z, a[u][1].z, a[u][0].w, a[u][1].w, b[u].z, b[u].w);
+        }
     }
 #pragma unroll
-    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) red[warp][nt * 8 + 2 * j + (i & 1)][g + 8 * (i >> 1)] = c[nt][i];
+    for (int i = 0; i < 4; i++) red[warp][2 * j + (i & 1)][g + 8 * (i >> 1)] = c[i];
     __syncthreads();
-    if (tid < 8 * NT * LS_COLS) {
+    if (tid < 8 * LS_COLS) {
         const int t = tid / LS_COLS, n = tid % LS_COLS;
         float v[1] = {0.f};
 #pragma unroll
@@ -138,11 +135,12 @@ k_linear_few(const uint16_t *__restrict__ x, long long xs, const uint16_t *__res
 // one column of y, so that bias is a register and a warp's accesses to residual and y are 32 neighbours.
 // SPLIT > 1: a cluster shares a tile, each CTA a part of K; the parts are added in rank order over distributed shared memory.
 constexpr int LT_M = 128, LT_K = 64, LT_EPI_WARPS = 8, LT_THREADS = 32 * (2 + LT_EPI_WARPS);
-template <int BN>
+template <int BN, int SPLIT>
 struct LtCfg {
     static constexpr int STAGE = LT_M * LT_K * 2 + BN * LT_K * 2;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int SMEM = STAGE * STAGES + 1024;
+    static constexpr int STAGES = SPLIT > 1 ? (BN == 64 ? 3 : 4) : BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int PARTS = SPLIT > 1 ? BN * LT_M * 4 : 0;      // what the cluster's CTAs send: [rank][row of mine][column]
+    static constexpr int SMEM = STAGE * STAGES + PARTS + 1024;
 };
 struct LtMaps { CUtensorMap w, x; };
 __device__ int g_linear_status;      // where a wait gave up (0: nowhere)
@@ -151,27 +149,29 @@ __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, u
     asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
                  ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
 }
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ uint32_t map_cluster(uint32_t addr, int rank) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(rank));
+    return a;
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, int rank) {
-    float v;
-    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
-    return v;
-}
+__device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
 template <int BN, int SPLIT>
 __global__ void __launch_bounds__(LT_THREADS, 1)
 k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K, const int *rows_used, int t_tiles, int n_tiles) {
-    using C = LtCfg<BN>;
+    using C = LtCfg<BN, SPLIT>;
     constexpr int TM_COLS = SPLIT == 1 ? 2 * BN : BN;
     constexpr uint32_t IDESC = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(LT_M >> 4) << 24);
-    Q36_GDS();
+    cudaTriggerProgrammaticLaunchCompletion();
     extern __shared__ uint8_t raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ uint64_t full_b[C::STAGES], empty_b[C::STAGES], acc_full_b[2], acc_empty_b[2];
     __shared__ uint32_t tmem_s;
     __shared__ volatile int abort_flag;
+    constexpr int PER = BN / SPLIT;       // rows of a tile that one CTA of a cluster finishes
+    const uint32_t parts = smem_u32(smem + C::STAGE * C::STAGES);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const uint32_t full0 = smem_u32(full_b), empty0 = smem_u32(empty_b), accf0 = smem_u32(acc_full_b), acce0 = smem_u32(acc_empty_b);
     if (tid == 0) {
@@ -187,6 +187,8 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (SPLIT > 1) cluster_arrive();       // "I run": awaited before anything is sent to another CTA
+    cudaGridDependencySynchronize();
     const uint32_t tmem = tmem_s;
     const int rows = rows_used ? min(T, *rows_used) : T;
     const int tiles = t_tiles * n_tiles, all_steps = (K + LT_K - 1) / LT_K;
@@ -250,6 +252,7 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
     } else {
         const int q = warp & 3, half = (warp - 2) >> 2;
         uint32_t tc = 0;
+        if (SPLIT > 1) cluster_wait();
         for (int i = first; i < tiles; i += step) {
             int n0, t0;
             place(i, n0, t0);
@@ -272,10 +275,12 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
                 if constexpr (SPLIT == 1) {
                     if (n < N) finish(e, n, bias, t0 + c, rows, v);
                 } else {
-                    // every MMA of this CTA is over: the stages are free to hold its sums, [row][column]
-                    float *p = reinterpret_cast<float *>(smem) + c * LT_M + 32 * q + lane;
+                    // to the CTA of the cluster that finishes these rows, [my rank][row][column]
 #pragma unroll
-                    for (int x = 0; x < 16; x++) p[x * LT_M] = v[x];
+                    for (int x = 0; x < 16; x++) {
+                        const int to = (c + x) / PER, row = (c + x) % PER;
+                        st_cluster(map_cluster(parts + ((rank * PER + row) * LT_M + 32 * q + lane) * 4, to), v[x]);
+                    }
                 }
             }
             tc_fence_before();
@@ -285,30 +290,30 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
         }
     }
     if constexpr (SPLIT > 1) {
-        cluster_sync();
+        __syncwarp();
+        if (warp < 2) cluster_wait();
+        cluster_arrive();
+        cluster_wait();
         int n0, t0;
         place(first, n0, t0);
         if (warp >= 2 && t0 < rows && !abort_flag) {
             const int f = (tid - 64) % LT_M, half = (tid - 64) / LT_M, n = n0 + f;
-            constexpr int PER = BN / SPLIT;       // rows of the tile this CTA finishes, by two groups of threads
-            constexpr int CH = PER >= 16 ? 8 : PER / 2;
+            constexpr int CH = PER >= 16 ? 8 : PER / 2;      // two groups of threads
             const float bias = e.bias && n < N ? e.bias[n] : 0.f;
-            for (int c = rank * PER + half * (PER / 2); c < rank * PER + (half + 1) * (PER / 2); c += CH) {
-                if (t0 + c >= rows) break;
+            const float *p = reinterpret_cast<const float *>(smem + C::STAGE * C::STAGES) + f;
+            for (int c = half * (PER / 2); c < (half + 1) * (PER / 2); c += CH) {
+                const int t = t0 + rank * PER + c;
+                if (t >= rows) break;
                 float v[CH];
 #pragma unroll
                 for (int x = 0; x < CH; x++) {
-                    float part[SPLIT];
+                    v[x] = p[(c + x) * LT_M];
 #pragma unroll
-                    for (int r = 0; r < SPLIT; r++) part[r] = ld_cluster(smem_u32(smem) + ((c + x) * LT_M + f) * 4, r);
-                    v[x] = part[0];
-#pragma unroll
-                    for (int r = 1; r < SPLIT; r++) v[x] += part[r];
+                    for (int r = 1; r < SPLIT; r++) v[x] += p[(r * PER + c + x) * LT_M];
                 }
-                if (n < N) finish(e, n, bias, t0 + c, rows, v);
+                if (n < N) finish(e, n, bias, t, rows, v);
             }
         }
-        cluster_sync();      // nobody leaves while its sums are read
     }
     tc_fence_before();
     __syncthreads();
@@ -335,7 +340,7 @@ static int make_map_bf16(CUtensorMap *m, const void *base, long rows, long cols,
 
 template <int BN, int SPLIT>
 static int run_tc(const LtMaps &maps, const Epilogue &e, int T, int N, int K, const int *rows_used, cudaStream_t st) {
-    using C = LtCfg<BN>;
+    using C = LtCfg<BN, SPLIT>;
     static bool attr_done[MAX_DEVICES] = {false};
     int rc;
     if ((rc = ensure_smem_attr((const void *)k_linear_tc<BN, SPLIT>, C::SMEM, attr_done))) return rc;
@@ -372,24 +377,33 @@ static int run_split(int split, const LtMaps &maps, const Epilogue &e, int T, in
 int launch_linear(const void *x, long long xs, const void *w, const float *bias, int act, const void *res, int res_bf16, long long rs,
                   void *y, int y_bf16, long long ys, int T, int N, int K, const int *rows_used, cudaStream_t st) {
     const Epilogue e{bias, res, y, rs, ys, act, res_bf16, y_bf16};
-    if (T <= 16) {
-        const dim3 grid((N + LS_COLS - 1) / LS_COLS), block(LS_THREADS);
-        if (T <= 8) launch_k(k_linear_few<1>, grid, block, 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
-        else launch_k(k_linear_few<2>, grid, block, 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
+    // The stream up to 8 rows while its warps have all of W in flight at once; us at 2048 columns against the split tiles: K 2048 5.8 /
+    // 6.0, K 4096 11.4 / 7.5.
+    if (T <= 8 && K <= 2048) {
+        launch_k(k_linear_few, dim3((N + LS_COLS - 1) / LS_COLS), dim3(LS_THREADS), 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
         return check_launch();
     }
-    const int bn = T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
-    // K is split while a cluster's CTAs still find an SM each and have two steps of 64 at least
-    const long tiles = (long)((T + bn - 1) / bn) * ((N + LT_M - 1) / LT_M);
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= sm_count() && (K + LT_K - 1) / LT_K >= split * 4) split *= 2;
+    // Tile height and split of K by what an SM has to load (150 KB per us, two CTAs of 32 or 64 rows at a time), what the exchange
+    // of a cluster costs (2.3 us at 128 rows) and what a second round of CTAs costs.  Measured us at 2048 columns, K 2048, for
+    // (rows, split): 64 tokens (32, 4) 6.9, (64, 8) 7.5, (64, 1) 13.5; 200 tokens (64, 4) 9.3, (128, 4) 9.2, (32, 8) 23; 300
+    // tokens (64, 2) 10.9, (128, 4) 17.3; 1000 tokens (128, 1) 15.8, (256, 1) 17.0, (128, 4) 36.
+    int bn = 0, split = 1;
+    float best = 0.f;
+    const int steps = (K + LT_K - 1) / LT_K, sms = sm_count();
+    for (int cb = 32; cb <= 256; cb *= 2)
+        for (int cs = 1; cs <= (cb == 256 ? 1 : 8) && (cs == 1 || steps >= 2 * cs); cs *= 2) {
+            const long ctas = (long)((T + cb - 1) / cb) * ((N + LT_M - 1) / LT_M) * cs, per_sm = (ctas + sms - 1) / sms;
+            const long rounds = cs == 1 ? 1 : (per_sm + (cb <= 64 ? 1 : 0)) / (cb <= 64 ? 2 : 1);
+            const float us = per_sm * ((steps + cs - 1) / cs) * (LT_M + cb) * (LT_K * 2 / 1024.f) / 150.f + (cs > 1 ? 0.018f * cb : 0.f) + 3.f * (rounds - 1);
+            if (!bn || us < best) { best = us; bn = cb; split = cs; }
+        }
     LtMaps maps;
     int rc;
     if ((rc = make_map_bf16(&maps.w, w, N, K, K, LT_M)) || (rc = make_map_bf16(&maps.x, x, T, K, xs, bn))) return rc;
     if (bn == 32) return run_split<32>(split, maps, e, T, N, K, rows_used, st);
     if (bn == 64) return run_split<64>(split, maps, e, T, N, K, rows_used, st);
     if (bn == 128) return run_split<128>(split, maps, e, T, N, K, rows_used, st);
-    return run_split<256>(split, maps, e, T, N, K, rows_used, st);
+    return run_tc<256, 1>(maps, e, T, N, K, rows_used, st);
 }
 
 // Where a bounded wait of the tile kernel gave up since the process began (0: nowhere).

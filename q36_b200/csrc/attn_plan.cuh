@@ -5,9 +5,8 @@
 
 namespace q36 {
 
-// rows: rows of a tile; unit: tokens of a unit; a request takes part when min_rows <= its rows <= max_rows.
-// causal_tiles: every row tile ends at its own last position (tiles of long prompts) instead of the request's.
-struct SpanRule { int rows, unit, min_rows, max_rows, causal_tiles; };
+// rows: rows of a tile; unit: tokens of a unit; a request takes part when it has max_rows rows at most.
+struct SpanRule { int rows, unit, max_rows; };
 
 struct SeqSpans { int t0, n, len, tiles, u_lo, u_hi; };   // units [u_lo, u_hi) of the cached tokens that any row sees
 
@@ -15,23 +14,12 @@ __device__ __forceinline__ SeqSpans seq_spans(const AttnArgs &a, const SpanRule 
     SeqSpans s;
     seq_span(a, b, s.t0, s.n, s.len);
     const int rows = s.n * a.G;
-    s.tiles = rows > 0 && rows >= r.min_rows && rows <= r.max_rows ? (rows + r.rows - 1) / r.rows : 0;
+    s.tiles = rows > 0 && rows <= r.max_rows ? (rows + r.rows - 1) / r.rows : 0;
     const int lo = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
     s.u_lo = lo / r.unit;
     s.u_hi = max((s.len + r.unit - 1) / r.unit, s.u_lo + 1);     // (at least one: rows that see nothing are written too)
     return s;
 }
-// units of row tile rt
-__device__ __forceinline__ void tile_units(const AttnArgs &a, const SpanRule &r, const SeqSpans &s, int rt, int &u0, int &u1) {
-    u0 = s.u_lo;
-    u1 = s.u_hi;
-    if (r.causal_tiles) {
-        const int i0 = rt * r.rows / a.G, i1 = min(rt * r.rows + r.rows, s.n * a.G) - 1, p0 = s.len - s.n + i0, p1 = s.len - s.n + i1 / a.G;
-        u0 = a.window > 0 ? max(0, p0 - a.window + 1) / r.unit : 0;
-        u1 = max(u0 + 1, (max(p1 + 1, 0) + r.unit - 1) / r.unit);
-    }
-}
-
 template <int THREADS>
 struct PlanSmem { long long sum[THREADS / 32]; long long base; int b; };
 
@@ -44,47 +32,24 @@ struct PlanPos {
     long long span_base;
 };
 
-__device__ __forceinline__ long long seq_units(const AttnArgs &a, const SpanRule &r, const SeqSpans &s) {
-    if (!r.causal_tiles) return (long long)s.tiles * a.kv.Hkv * (s.u_hi - s.u_lo);
-    long long n = 0;
-    for (int rt = 0; rt < s.tiles; rt++) {
-        int u0, u1;
-        tile_units(a, r, s, rt, u0, u1);
-        n += u1 - u0;
-    }
-    return n * a.kv.Hkv;
+__device__ __forceinline__ long long seq_units(const AttnArgs &a, const SeqSpans &s) {
+    return (long long)s.tiles * a.kv.Hkv * (s.u_hi - s.u_lo);
 }
 
 // Moves pos to the span that holds pos.at, from request pos.b (whose first unit is pos.seq_base) on.
 __device__ __forceinline__ void plan_locate(const AttnArgs &a, const SpanRule &r, PlanPos &pos) {
     for (;;) {
         pos.s = seq_spans(a, r, pos.b);
-        const long long n = seq_units(a, r, pos.s);
+        const long long n = seq_units(a, pos.s);
         if (pos.at < pos.seq_base + n) break;
         pos.seq_base += n;
         pos.b++;
     }
     const long long off = pos.at - pos.seq_base;
-    if (!r.causal_tiles) {
-        const int u = pos.s.u_hi - pos.s.u_lo;
-        const int span = (int)(off / u);
-        pos.hk = span / pos.s.tiles;
-        pos.rt = span - pos.hk * pos.s.tiles;
-        pos.span_base = pos.seq_base + (long long)span * u;
-    } else {
-        pos.span_base = pos.seq_base;
-        for (pos.rt = 0;; pos.rt++) {
-            int u0, u1;
-            tile_units(a, r, pos.s, pos.rt, u0, u1);
-            const long long all = (long long)(u1 - u0) * a.kv.Hkv;
-            if (pos.at < pos.span_base + all) {
-                pos.hk = (int)((pos.at - pos.span_base) / (u1 - u0));
-                pos.span_base += (long long)pos.hk * (u1 - u0);
-                break;
-            }
-            pos.span_base += all;
-        }
-    }
+    const int u = pos.s.u_hi - pos.s.u_lo, span = (int)(off / u);
+    pos.hk = span / pos.s.tiles;
+    pos.rt = span - pos.hk * pos.s.tiles;
+    pos.span_base = pos.seq_base + (long long)span * u;
 }
 
 // This CTA's range; false when it is empty.  All threads take part.
@@ -93,7 +58,7 @@ __device__ __forceinline__ bool plan_start(const AttnArgs &a, const SpanRule &r,
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int per = (a.B + THREADS - 1) / THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
     long long mine = 0;
-    for (int b = b0; b < b1; b++) mine += seq_units(a, r, seq_spans(a, r, b));
+    for (int b = b0; b < b1; b++) mine += seq_units(a, seq_spans(a, r, b));
     long long inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -124,14 +89,12 @@ __device__ __forceinline__ bool plan_start(const AttnArgs &a, const SpanRule &r,
 // A piece of one span: units [u0, u1) of [0, units), the first of which holds token u_first * unit.
 struct PlanSeg { int b, hk, rt, t0, n, len, u0, u1, units, u_first; long long span_base; };
 
-__device__ __forceinline__ PlanSeg plan_segment(const AttnArgs &a, const SpanRule &r, const PlanPos &pos) {
+__device__ __forceinline__ PlanSeg plan_segment(const PlanPos &pos) {
     PlanSeg g;
-    int lo, hi;
-    tile_units(a, r, pos.s, pos.rt, lo, hi);
     g.b = pos.b; g.hk = pos.hk; g.rt = pos.rt;
     g.t0 = pos.s.t0; g.n = pos.s.n; g.len = pos.s.len;
-    g.units = hi - lo;
-    g.u_first = lo;
+    g.units = pos.s.u_hi - pos.s.u_lo;
+    g.u_first = pos.s.u_lo;
     g.u0 = (int)(pos.at - pos.span_base);
     g.u1 = (int)min((long long)g.units, pos.end - pos.span_base);
     g.span_base = pos.span_base;
@@ -145,17 +108,18 @@ __device__ __forceinline__ void plan_next(const AttnArgs &a, const SpanRule &r, 
 
 // A span that was cut: its first piece's slot and the number of pieces.  The next pieces are the first pieces of the CTAs
 // that follow: slot 2 * CTA.
-struct AttnPart { int parts, slot, b_t0, n, hk, rt, pad[2]; };
+struct AttnPart { int parts, slot, t0, n, hk, row0, rows, pad; };
 
-__device__ __forceinline__ AttnPart plan_parts(const PlanSeg &g, const PlanPos &pos, int slot) {
+__device__ __forceinline__ AttnPart plan_parts(const AttnArgs &a, const SpanRule &r, const PlanSeg &g, const PlanPos &pos, int slot) {
     AttnPart p;
     p.parts = (int)((g.span_base + g.units - 1) / pos.per - blockIdx.x) + 1;
     p.slot = slot;
-    p.b_t0 = g.t0;
+    p.t0 = g.t0;
     p.n = g.n;
     p.hk = g.hk;
-    p.rt = g.rt;
-    p.pad[0] = p.pad[1] = 0;
+    p.row0 = g.rt * r.rows;
+    p.rows = min(r.rows, g.n * a.G - p.row0);
+    p.pad = 0;
     return p;
 }
 
@@ -184,6 +148,10 @@ __device__ __forceinline__ void attn_store_lse(const AttnArgs &a, int t0, int n,
 constexpr int DEC_MAX_OCC = 4;
 int launch_decode(const AttnArgs &a, int rows, int max_rows, void *ws, cudaStream_t st);
 uint64_t decode_ws_bytes(int Dh, int rows);
+int launch_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t st);
+uint64_t prefill_ws_bytes(int Dh);
+int prefill_wait_status(int *out, cudaStream_t st);
+int linear_wait_status(int *out, cudaStream_t st);
 int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st);
 
 }  // namespace q36

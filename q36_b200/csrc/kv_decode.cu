@@ -139,7 +139,7 @@ k_attn_decode(AttnArgs a, int max_rows, AttnPart *__restrict__ desc, float *__re
     extern __shared__ __align__(16) uint8_t smem_raw[];
     DecSmem<DH, NT> &sm = *reinterpret_cast<DecSmem<DH, NT> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
-    const SpanRule rule{R, DEC_UNIT, 0, max_rows, 0};
+    const SpanRule rule{R, DEC_UNIT, max_rows};
     PlanPos pos;
     if (!plan_start<DEC_THREADS>(a, rule, DEC_WARPS, sm.plan, pos)) {
         if (tid == 0) desc[blockIdx.x].parts = 0;
@@ -148,7 +148,7 @@ k_attn_decode(AttnArgs a, int max_rows, AttnPart *__restrict__ desc, float *__re
     if (tid == 0) desc[blockIdx.x].parts = 0;
     bool first = true;
     while (pos.at < pos.end) {
-        const PlanSeg sg = plan_segment(a, rule, pos);
+        const PlanSeg sg = plan_segment(pos);
         // ---- q: operand fragments of the row tile, lane = (row g, quarter j): dims 32b + 8j + 4s + 0..3
         uint32_t qf[TERMS][NT][NB][4];
         float fac[NT][2];       // scale * log2(e) / 2^(power of two of the row), of columns 2j, 2j + 1
@@ -474,7 +474,7 @@ k_attn_decode(AttnArgs a, int max_rows, AttnPart *__restrict__ desc, float *__re
             else attn_store_lse(a, sg.t0, sg.n, sg.hk, sg.rt * R + tid, ma, la);
         }
         // the CTA that has a cut span's first piece says what belongs together
-        if (tid == 0 && !whole && sg.u0 == 0) desc[blockIdx.x] = plan_parts(sg, pos, slot);
+        if (tid == 0 && !whole && sg.u0 == 0) desc[blockIdx.x] = plan_parts(a, rule, sg, pos, slot);
         __syncthreads();
         first = false;
         plan_next(a, rule, sg, pos);

@@ -1,0 +1,601 @@
+// Attention of many rows per request over the paged 4-bit cache, bf16: prompts and prompt chunks.
+//
+// Rows are (new token, query head of the kv head's group): a tile of 256 rows (128 at 256-wide heads) shares K and V, so that the
+// cache is read and widened to bf16 once for all of them.  E2M1 times a power of two is exact in bf16.
+// One CTA, tiles of KT cached tokens:
+//   warps 8-11, 12-15   K, V of the next tile: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
+//   warp 16             S = Q K^T and O += P V on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's place)
+//   warps 0-3, 4-7      softmax of 128 rows each, a row per thread: maximum, 2^(S - m) rounded to bf16 once (half a step 2^-8, as
+//                       the output's), the sum of the unrounded weights in f32
+// m is a lagging maximum: O is rescaled (in TMEM) only when a row would pass 2^8.
+// With two row tiles the tensor cores work on one while the other's softmax runs; 256-wide heads have one tile and two S.
+//
+// Work: the spans (kv head, row tile) of all long requests, measured in the tokens they see, are cut into equal ranges, one per CTA;
+// cuts are moved down to tile boundaries.  Cut spans are joined as in the decode kernel.
+#include <math.h>
+
+#include "attn_plan.cuh"
+#include "tc_ptx.cuh"
+
+namespace q36 {
+
+template <int DH>
+struct PfCfg {
+    static constexpr int NQ = DH == 256 ? 1 : 2, R = 128 * NQ, KT = DH == 256 ? 64 : 128;
+    static constexpr int NB = DH / 32, BPT = NB < 4 ? NB : 4;          // scale blocks, and those a widening thread has
+    static constexpr int Q_BYTES = 128 * DH * 2, T_BYTES = KT * DH * 2;
+    static constexpr int SMEM = NQ * Q_BYTES + 4 * T_BYTES + 1024;
+    static constexpr int TM_S = KT, TM_O0 = 2 * KT;                    // columns: S0 | S1 | O0 (| O1)
+    static constexpr int TMEM = 512;
+};
+constexpr int PF_THREADS = 17 * 32;
+constexpr float PF_NONE = -1.0e30f;      // "no token yet": finite, so that differences stay defined
+constexpr float PF_GROW = 8.f;
+__device__ int g_prefill_status;         // where a wait gave up (0: nowhere)
+
+// ---------------------------------------------------------------- plan
+// Span rt of a request: tokens c rt .. of the new ones (c whole tokens of G rows); it sees cached tokens [lo, hi).  Its size is
+// hi - lo + 1, which is piecewise linear in rt: prefix sums have a closed form.
+struct PfSeq { int t0, n, len, c, tiles; };
+__device__ __forceinline__ long long sum_pos(long long a, long long c, long long n) {      // sum over x < n of max(0, a + c x)
+    long long x0 = a < 0 ? (-a + c - 1) / c : 0;
+    if (x0 >= n) return 0;
+    const long long k = n - x0, f = a + c * x0;
+    return k * f + c * (k * (k - 1) / 2);
+}
+__device__ __forceinline__ PfSeq pf_seq(const AttnArgs &a, int R, int min_rows, int b) {
+    PfSeq s;
+    seq_span(a, b, s.t0, s.n, s.len);
+    s.c = R / a.G;
+    s.tiles = s.n * a.G >= min_rows ? (s.n + s.c - 1) / s.c : 0;
+    return s;
+}
+__device__ __forceinline__ void pf_range(const AttnArgs &a, const PfSeq &s, int rt, int &lo, int &hi) {
+    const int base = s.len - s.n;
+    hi = max(0, base + min((rt + 1) * s.c, s.n));
+    lo = a.window > 0 ? min(max(0, base + rt * s.c - a.window + 1), hi) : 0;
+}
+// units of the row tiles before rt
+__device__ __forceinline__ long long pf_prefix(const AttnArgs &a, const PfSeq &s, int rt) {
+    const long long base = s.len - s.n;
+    long long u = sum_pos(base + s.c, s.c, rt) + rt;
+    if (rt > 0 && (long long)rt * s.c > s.n) u += max(0ll, base + s.n) - max(0ll, base + (long long)rt * s.c);     // the last tile is shorter
+    if (a.window > 0) u -= sum_pos(base - a.window + 1, s.c, rt);
+    return u;
+}
+struct PfPos { long long at, end, per, seq_base, span_base; int b, hk, rt; PfSeq s; };
+__device__ __forceinline__ void pf_locate(const AttnArgs &a, int R, int min_rows, PfPos &p) {
+    long long one;
+    for (;;) {
+        p.s = pf_seq(a, R, min_rows, p.b);
+        one = pf_prefix(a, p.s, p.s.tiles);
+        if (p.at < p.seq_base + one * a.kv.Hkv) break;
+        p.seq_base += one * a.kv.Hkv;
+        p.b++;
+    }
+    const long long off = p.at - p.seq_base;
+    p.hk = (int)(off / one);
+    const long long in = off - p.hk * one;
+    int lo = 0, hi = p.s.tiles;
+    while (hi - lo > 1) {
+        const int m = (lo + hi) >> 1;
+        if (pf_prefix(a, p.s, m) <= in) lo = m; else hi = m;
+    }
+    p.rt = lo;
+    p.span_base = p.seq_base + p.hk * one + pf_prefix(a, p.s, lo);
+}
+struct PfSeg { int lo, hi, j0, j1, whole, head; long long units; };     // key tiles [j0, j1); head: this is the span's first piece
+__device__ __forceinline__ PfSeg pf_segment(const AttnArgs &a, int KT, const PfPos &p) {
+    PfSeg g;
+    pf_range(a, p.s, p.rt, g.lo, g.hi);
+    g.units = (long long)(g.hi - g.lo) + 1;
+    const long long y0 = p.at - p.span_base, y1 = min(g.units, p.end - p.span_base);
+    g.head = y0 == 0;
+    g.whole = g.head && y1 == g.units;
+    const int first = g.lo / KT, last = max((g.hi + KT - 1) / KT, first + 1);
+    g.j0 = y0 == 0 ? first : min((int)((g.lo + y0) / KT), last);
+    g.j1 = y1 == g.units ? last : min((int)((g.lo + y1) / KT), last);
+    return g;
+}
+__device__ __forceinline__ bool pf_next(const AttnArgs &a, int R, int min_rows, const PfSeg &g, PfPos &p) {
+    p.at = min(p.span_base + g.units, p.end);
+    if (p.at >= p.end) return false;
+    pf_locate(a, R, min_rows, p);
+    return true;
+}
+
+// ---------------------------------------------------------------- 4 bits -> bf16
+// The eight magnitudes of a block as bf16, high and low bytes apart: eight bytes each, picked by the three magnitude bits of a code.
+struct Lut { uint32_t ha, hb, la, lb; };
+__device__ __forceinline__ Lut make_lut(uint32_t s) {
+    const uint32_t p23 = s * 0x00800080u + 0x00400000u, p45 = p23 + 0x00800080u, p67 = p45 + 0x00800080u, p01 = ((s - 1) << 23);
+    return Lut{__byte_perm(p01, p23, 0x7531), __byte_perm(p45, p67, 0x7531), __byte_perm(p01, p23, 0x6420), __byte_perm(p45, p67, 0x6420)};
+}
+__device__ __forceinline__ void widen4(const Lut &t, uint32_t sel, uint32_t sign, uint32_t &x, uint32_t &y) {
+    const uint32_t h = __byte_perm(t.ha, t.hb, sel) | (sign & 0x80808080u), l = __byte_perm(t.la, t.lb, sel);
+    x = __byte_perm(l, h, 0x5140);
+    y = __byte_perm(l, h, 0x7362);
+}
+__device__ __forceinline__ uint32_t prmt_sign(uint32_t a, uint32_t b, uint32_t sel) {      // bytes of 0xff / 0x00 by sign bits
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+// eight codes (low nibble first) -> eight bf16
+__device__ __forceinline__ uint4 widen8(const Lut &t, uint32_t w) {
+    uint4 o;
+    const uint32_t m = w & 0x77777777u, w4 = w << 4;
+    widen4(t, m, prmt_sign(w4, w, 0xd9c8), o.x, o.y);
+    widen4(t, m >> 16, prmt_sign(w4, w, 0xfbea), o.z, o.w);
+    return o;
+}
+
+// ---------------------------------------------------------------- tcgen05
+__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void tc_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                 ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+                 "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// operand whose contiguous direction is N (the dims): 64 of them per 128-byte row, rows (tokens) in groups of 8, panels of 64 dims
+// `panel` bytes apart
+__device__ __forceinline__ uint64_t desc_n_major(uint32_t saddr, uint32_t panel) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ float pf_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+struct PfBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], q_full; };
+
+template <int DH>
+__global__ void __launch_bounds__(PF_THREADS, 1)
+k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__restrict__ part) {
+    using C = PfCfg<DH>;
+    constexpr int NQ = C::NQ, R = C::R, KT = C::KT, NB = C::NB, BPT = C::BPT;
+    constexpr uint32_t ID_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
+    constexpr uint32_t ID_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | (8u << 24);
+    Q36_GDS();
+    extern __shared__ uint8_t raw[];
+    uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    __shared__ PfBars bars;
+    __shared__ uint32_t tmem_s, bad_s[4][4];      // bad_s: tokens of a tile whose page is bad; a ring of 4, since K runs ahead of the softmax
+    __shared__ volatile int abort_flag;
+    __shared__ long long plan_sum[PF_THREADS / 32], plan_base;
+    __shared__ int plan_b;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const uint32_t q_s = smem_u32(smem), k_s = q_s + NQ * C::Q_BYTES, v_s = k_s + 2 * C::T_BYTES;
+    auto bar = [&](uint64_t &b) { return smem_u32(&b); };
+    if (tid == 0) {
+        abort_flag = 0;
+        for (int i = 0; i < 2; i++) {
+            mbar_init(bar(bars.k_full[i]), 4);
+            mbar_init(bar(bars.v_full[i]), 4);
+            mbar_init(bar(bars.k_empty[i]), 1);
+            mbar_init(bar(bars.v_empty[i]), 1);
+            mbar_init(bar(bars.s_full[i]), 1);
+            mbar_init(bar(bars.p_full[i]), 4);
+            mbar_init(bar(bars.o_done[i]), 1);
+        }
+        mbar_init(bar(bars.q_full), 4 * NQ);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        desc[blockIdx.x].parts = 0;
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(C::TMEM) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    // ---- this CTA's range of the work
+    PfPos pos;
+    {
+        const int per = (a.B + PF_THREADS - 1) / PF_THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+        long long mine = 0;
+        for (int b = b0; b < b1; b++) {
+            const PfSeq s = pf_seq(a, R, min_rows, b);
+            if (s.tiles) mine += pf_prefix(a, s, s.tiles) * a.kv.Hkv;
+        }
+        long long inc = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) plan_sum[warp] = inc;
+        __syncthreads();
+        long long total = 0, before = 0;
+        for (int w = 0; w < PF_THREADS / 32; w++) {
+            if (w == warp) before = total;
+            total += plan_sum[w];
+        }
+        const long long excl = before + inc - mine;
+        pos.per = max((total + gridDim.x - 1) / gridDim.x, (long long)(2 * KT));
+        pos.at = min(pos.per * blockIdx.x, total);
+        pos.end = min(pos.at + pos.per, total);
+        if (pos.at < pos.end && pos.at >= excl && pos.at < excl + mine) { plan_base = excl; plan_b = b0; }
+        __syncthreads();
+        if (pos.at < pos.end) {
+            pos.seq_base = plan_base;
+            pos.b = plan_b;
+            pf_locate(a, R, min_rows, pos);
+        }
+    }
+    tc_fence_after();
+    const uint32_t tmem = tmem_s;
+    bool more = pos.at < pos.end;
+
+    if (warp < 8) {
+        // ------------------------------------------------------------ softmax: a row per thread
+        const int i = warp >> 2, row = tid & 127;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        uint32_t sc = 0, oc = 0, kt = 0;       // tiles of this row tile, O's awaited, K tiles before this piece
+        // a negative scale goes to the signs of q: m follows the largest score
+        const float scale2 = fabsf(a.scale2);
+        const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
+        bool first = true, ok = true;
+        while (more && ok && i < NQ) {
+            const PfSeg g = pf_segment(a, KT, pos);
+            const int r_tile = i * 128 + row, rows = min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G), r = pos.rt * pos.s.c * a.G + r_tile;
+            const bool mine = r_tile < rows, active = i * 128 < rows && g.j0 < g.j1;
+            const int tok_i = mine ? r / a.G : 0, hq = pos.hk * a.G + (mine ? r - tok_i * a.G : 0);
+            if (g.j0 < g.j1) {
+                // Q: this thread's row (the MMAs that read the last one are over: its results were awaited)
+                const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (size_t)(pos.s.t0 + tok_i) * a.q_stride + (size_t)hq * DH);
+#pragma unroll 8
+                for (int c = 0; c < DH / 8; c++) {
+                    uint4 v = mine ? src[c] : make_uint4(0, 0, 0, 0);
+                    v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
+                    *reinterpret_cast<uint4 *>(smem + i * C::Q_BYTES + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(bars.q_full));
+            }
+            const int p = pos.s.len - pos.s.n + tok_i;              // position; the row sees [lo_r, p]
+            const int hi_r = mine ? p : -1, lo_r = a.window > 0 ? p - a.window + 1 : 0;
+            float m = PF_NONE, l = 0.f;
+            if (active) {
+                const int t_first = min((pos.rt * pos.s.c * a.G + i * 128) / a.G, pos.s.n - 1), t_last = min((pos.rt * pos.s.c * a.G + min(i * 128 + 127, rows - 1)) / a.G, pos.s.n - 1);
+                const int all_hi = pos.s.len - pos.s.n + t_first, all_lo = a.window > 0 ? pos.s.len - pos.s.n + t_last - a.window + 1 : 0;
+                for (int j = g.j0; j < g.j1; j++, sc++) {
+                    const uint32_t x = NQ == 2 ? i : sc & 1, ph = NQ == 2 ? sc & 1 : (sc >> 1) & 1;
+                    if (!(ok = mbar_wait(bar(bars.s_full[x]), ph, &abort_flag, &g_prefill_status, 0x500 + x, TC_SPIN_LIMIT, 0))) break;
+                    __syncwarp();
+                    tc_fence_after();
+                    const uint32_t s_col = tmem + lanes + x * C::TM_S;
+                    const uint32_t st = (kt + (j - g.j0)) & 3;       // its place in bad_s
+                    uint32_t bad = 0;
+#pragma unroll
+                    for (int w = 0; w < KT / 32; w++) bad |= bad_s[st][w];
+                    const bool edge = bad || j * KT < all_lo || j * KT + KT - 1 > all_hi;
+                    auto masked = [&](uint32_t (&v)[32], int c) {
+                        const uint32_t b = bad_s[st][c >> 5];
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const int t = j * KT + c + e;
+                            if (t > hi_r || t < lo_r || (b >> e & 1)) v[e] = 0xff800000u;
+                        }
+                    };
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < KT; c += 32) {
+                        uint32_t v[32];
+                        tc_ld32(s_col + c, v);
+                        tc_ld_wait();
+                        if (edge) masked(v, c);
+#pragma unroll
+                        for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(v[e]));
+                    }
+                    const float top = mx == -INFINITY ? mx : mx * scale2;
+                    const bool grow = top > m + PF_GROW;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float mn = grow ? top : m, f = pf_ex2(m - mn);
+                        l *= f;
+                        m = mn;
+                        if (j > g.j0) {
+                            // O holds the tiles before this one
+                            if (NQ == 1 && !(ok = mbar_wait(bar(bars.o_done[0]), (oc + (j - g.j0) - 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
+                            __syncwarp();
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < DH; c += 16) {
+                                uint32_t v[16];
+                                const uint32_t o_col = tmem + lanes + C::TM_O0 + i * DH + c;
+                                tc_ld16(o_col, v);
+                                tc_ld_wait();
+#pragma unroll
+                                for (int e = 0; e < 16; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                                tc_st16(o_col, v);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int c = 0; c < KT; c += 32) {
+                        uint32_t v[32], w[16];
+                        tc_ld32(s_col + c, v);
+                        tc_ld_wait();
+                        if (edge) masked(v, c);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            float p0 = pf_ex2(fmaf(__uint_as_float(v[e]), scale2, -m)), p1 = pf_ex2(fmaf(__uint_as_float(v[e + 1]), scale2, -m));
+                            if (edge) {      // (a scale of 0 makes no -inf of a masked score)
+                                if (v[e] == 0xff800000u) p0 = 0.f;
+                                if (v[e + 1] == 0xff800000u) p1 = 0.f;
+                            }
+                            l += p0;
+                            l += p1;
+                            w[e / 2] = pack_bf16(p0, p1);
+                        }
+                        tc_st16(s_col + c / 2, w);
+                    }
+                    tc_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(bars.p_full[x]));
+                }
+                if (!ok) break;
+                // ---- the piece's result
+                const uint32_t n_o = NQ == 2 ? 1 : (uint32_t)(g.j1 - g.j0);
+                oc += n_o;
+                // (two S: the product before the last may be under way too, and a parity names one phase of two)
+                if (NQ == 1 && n_o > 1 && !(ok = mbar_wait(bar(bars.o_done[0]), oc & 1, &abort_flag, &g_prefill_status, 0x710, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                if (!(ok = mbar_wait(bar(bars.o_done[NQ == 2 ? i : 0]), (oc - 1) & 1, &abort_flag, &g_prefill_status, 0x700 + i, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                __syncwarp();
+                tc_fence_after();
+            }
+            float *dst = part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * attn_part_floats(R, DH);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (active) {
+#pragma unroll 1
+                for (int c = 0; c < DH; c += 16) {
+                    uint32_t v[16];
+                    tc_ld16(tmem + lanes + C::TM_O0 + i * DH + c, v);
+                    tc_ld_wait();
+                    float4 o[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        o[e] = make_float4(__uint_as_float(v[4 * e]) * inv, __uint_as_float(v[4 * e + 1]) * inv, __uint_as_float(v[4 * e + 2]) * inv,
+                                           __uint_as_float(v[4 * e + 3]) * inv);
+                    if (!mine) continue;
+                    if (g.whole) {
+                        __nv_bfloat16 *d = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)(pos.s.t0 + tok_i) * a.o_stride + (size_t)hq * DH + c;
+#pragma unroll
+                        for (int e = 0; e < 2; e++)
+                            reinterpret_cast<uint4 *>(d)[e] = make_uint4(pack_bf16(o[2 * e].x, o[2 * e].y), pack_bf16(o[2 * e].z, o[2 * e].w),
+                                                                         pack_bf16(o[2 * e + 1].x, o[2 * e + 1].y), pack_bf16(o[2 * e + 1].z, o[2 * e + 1].w));
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) *reinterpret_cast<float4 *>(dst + 2 * R + r_tile * DH + c + 4 * e) = o[e];
+                    }
+                }
+                tc_fence_before();
+            }
+            if (mine) {
+                if (g.whole) { if (a.lse) a.lse[(size_t)(pos.s.t0 + tok_i) * a.Hq + hq] = l > 0.f || l != l ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY; }
+                else { dst[2 * r_tile] = m; dst[2 * r_tile + 1] = l; }
+            }
+            if (tid == 0 && !g.whole && g.head) {
+                AttnPart d;
+                d.parts = (int)((pos.span_base + g.units - 1) / pos.per - blockIdx.x) + 1;
+                d.slot = 2 * blockIdx.x + (first ? 0 : 1);
+                d.t0 = pos.s.t0;
+                d.n = pos.s.n;
+                d.hk = pos.hk;
+                d.row0 = pos.rt * pos.s.c * a.G;
+                d.rows = rows;
+                d.pad = 0;
+                desc[blockIdx.x] = d;
+            }
+            first = false;
+            kt += max(g.j1 - g.j0, 0);
+            more = pf_next(a, R, min_rows, g, pos);
+        }
+    } else if (warp < 16) {
+        // ------------------------------------------------------------ widening: warps 8-11 K, 12-15 V
+        const bool is_v = warp >= 12;
+        const int th = tid & 127, tl = th % KT, half = th / KT;     // token of the tile; which four scale blocks (256-wide heads)
+        const uint32_t dst0 = is_v ? v_s : k_s;
+        uint32_t kc = 0;
+        bool ok = true;
+        while (more && ok) {
+            const PfSeg g = pf_segment(a, KT, pos);
+            const int *row = a.table + (size_t)pos.b * a.max_blocks;
+            auto page = [&](int j) {
+                const int t = j * KT + tl, col = t >> a.kv.log_bs;
+                return j < g.j1 && t < pos.s.len && col < a.max_blocks ? __ldg(row + col) : -1;
+            };
+            uint32_t raw_w[4 * BPT], scale = 0;
+            bool has = false;
+            auto fetch = [&](int j, int id) {
+                has = id >= 0 && id < a.kv.n_blocks;
+                if (!has) return;
+                const int t = (j * KT + tl) & (a.kv.bs - 1);
+                const uint8_t *reg = a.kv.at(id, pos.hk);
+                const uint8_t *sp = reg + a.kv.bs * DH + (is_v ? a.kv.bs * NB : 0) + t * NB + half * 4;
+                if constexpr (NB == 2) scale = __ldg(reinterpret_cast<const uint16_t *>(sp));
+                else scale = __ldg(reinterpret_cast<const uint32_t *>(sp));
+                if (!is_v) {
+                    const uint8_t *src = reg + kv_k_off(t, 0, half * 4, DH);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {       // word q of every block
+                        if constexpr (BPT == 4) {
+                            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src + q * (DH / 8)));
+                            raw_w[4 * q] = u.x; raw_w[4 * q + 1] = u.y; raw_w[4 * q + 2] = u.z; raw_w[4 * q + 3] = u.w;
+                        } else {
+                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
+                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                        }
+                    }
+                } else {
+                    const uint8_t *src = reg + a.kv.bs * (DH / 2) + kv_v_off(t, 0, half * 4, DH);
+#pragma unroll
+                    for (int q = 0; q < 8; q++) {       // four dims of every block
+                        if constexpr (BPT == 4) {
+                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
+                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                        } else {
+                            raw_w[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
+                        }
+                    }
+                }
+            };
+            int id_next = page(g.j0 + 1);
+            fetch(g.j0, page(g.j0));
+            for (int j = g.j0; j < g.j1; j++, kc++) {
+                const uint32_t st = kc & 1, ph = (kc >> 1) & 1;
+                if (!(ok = mbar_wait(bar(is_v ? bars.v_empty[st] : bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, 0))) break;
+                __syncwarp();
+                uint8_t *dst = smem + (dst0 - q_s) + st * C::T_BYTES + tl * 128;
+#pragma unroll
+                for (int b = 0; b < BPT; b++) {
+                    const Lut t = make_lut((scale >> (8 * b)) & 0xff);
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t w;
+                        if (!is_v) w = raw_w[BPT * q + b];
+                        else w = __byte_perm(raw_w[(BPT / 2) * (2 * q) + b / 2], raw_w[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
+                        const uint4 v = has ? widen8(t, w) : make_uint4(0, 0, 0, 0);
+                        const int c = (half * 4 + b) * 4 + q;          // 16-byte chunk of the row
+                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * (KT * 128) + (((c & 7) ^ (tl & 7)) << 4)) = v;
+                    }
+                }
+                if (!is_v && half == 0) {
+                    // tokens of the request whose page is bad
+                    const uint32_t bad = __ballot_sync(0xffffffffu, !has && j * KT + tl < pos.s.len);
+                    if (lane == 0) bad_s[kc & 3][tl >> 5] = bad;
+                }
+                const int id = id_next;
+                if (j + 1 < g.j1) {
+                    id_next = page(j + 2);
+                    fetch(j + 1, id);
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(is_v ? bars.v_full[st] : bars.k_full[st]));
+            }
+            if (ok) more = pf_next(a, R, min_rows, g, pos);
+        }
+    } else if (lane == 0) {
+        // ------------------------------------------------------------ MMA
+        uint32_t kq = 0, vq = 0, pq[2] = {0, 0}, qn = 0;
+        bool ok = true;
+        auto wait = [&](uint64_t &b, uint32_t ph, int where) { ok = ok && mbar_wait(bar(b), ph, &abort_flag, &g_prefill_status, where); };
+        auto qk = [&](int i, uint32_t x, uint32_t st) {
+            const uint32_t qa = q_s + i * C::Q_BYTES, kb = k_s + st * C::T_BYTES;
+#pragma unroll
+            for (int kk = 0; kk < DH / 16; kk++)
+                pf_mma_ss(tmem + x * C::TM_S, desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32), desc_sw128(kb + (kk >> 2) * (KT * 128) + (kk & 3) * 32), ID_QK, kk ? 1u : 0u);
+        };
+        auto pv = [&](int i, uint32_t x, uint32_t st, bool more_than_first) {
+            const uint32_t vb = v_s + st * C::T_BYTES;
+#pragma unroll
+            for (int kk = 0; kk < KT / 16; kk++)
+                pf_mma_ts(tmem + C::TM_O0 + i * DH, tmem + x * C::TM_S + kk * 8, desc_n_major(vb + kk * 2048, KT * 128), ID_PV, (more_than_first || kk) ? 1u : 0u);
+        };
+        while (more && ok) {
+            const PfSeg g = pf_segment(a, KT, pos);
+            const int rows = min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G), nq = NQ == 2 && rows > 128 ? 2 : 1, n = g.j1 - g.j0;
+            if (n > 0) {
+                wait(bars.q_full, qn & 1, 0x100);
+                qn++;
+                if (NQ == 2) {
+                    for (int j = -1; j < n && ok; j++) {
+                        if (j >= 0) wait(bars.v_full[vq & 1], (vq >> 1) & 1, 0x200);
+                        if (j + 1 < n) wait(bars.k_full[kq & 1], (kq >> 1) & 1, 0x210);
+                        for (int i = 0; i < nq && ok; i++) {
+                            if (j >= 0) {
+                                wait(bars.p_full[i], pq[i] & 1, 0x300 + i);
+                                pq[i]++;
+                                if (!ok) break;
+                                tc_fence_after();
+                                pv(i, i, vq & 1, j > 0);
+                                if (i == nq - 1) tc_commit(bar(bars.v_empty[vq & 1]));
+                                if (j == n - 1) tc_commit(bar(bars.o_done[i]));
+                            }
+                            if (j + 1 < n && ok) {
+                                tc_fence_after();
+                                qk(i, i, kq & 1);
+                                tc_commit(bar(bars.s_full[i]));
+                            }
+                        }
+                        if (j >= 0) vq++;
+                        if (j + 1 < n) { if (ok) tc_commit(bar(bars.k_empty[kq & 1])); kq++; }
+                    }
+                } else {
+                    auto one_qk = [&]() {
+                        wait(bars.k_full[kq & 1], (kq >> 1) & 1, 0x210);
+                        if (!ok) return;
+                        tc_fence_after();
+                        qk(0, kq & 1, kq & 1);
+                        tc_commit(bar(bars.s_full[kq & 1]));
+                        tc_commit(bar(bars.k_empty[kq & 1]));
+                        kq++;
+                    };
+                    one_qk();
+                    if (n > 1 && ok) one_qk();
+                    for (int j = 0; j < n && ok; j++) {
+                        wait(bars.v_full[vq & 1], (vq >> 1) & 1, 0x200);
+                        wait(bars.p_full[vq & 1], (vq >> 1) & 1, 0x300);
+                        if (!ok) break;
+                        tc_fence_after();
+                        pv(0, vq & 1, vq & 1, j > 0);
+                        tc_commit(bar(bars.v_empty[vq & 1]));
+                        tc_commit(bar(bars.o_done[0]));
+                        vq++;
+                        if (j + 2 < n) one_qk();
+                    }
+                }
+            }
+            if (ok) more = pf_next(a, R, min_rows, g, pos);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+}
+
+template <int DH>
+static int run_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t st) {
+    using C = PfCfg<DH>;
+    static bool attr_done[MAX_DEVICES] = {false};
+    int rc;
+    if ((rc = ensure_smem_attr((const void *)k_attn_prefill<DH>, C::SMEM, attr_done))) return rc;
+    const int grid = sm_count();
+    AttnPart *desc = (AttnPart *)ws;
+    float *part = (float *)((uint8_t *)ws + attn_desc_bytes(grid));
+    launch_k(k_attn_prefill<DH>, dim3(grid), dim3(PF_THREADS), C::SMEM, st, a, min_rows, desc, part);
+    if ((rc = check_launch())) return rc;
+    return launch_attn_join(a, C::R, grid, desc, part, st);
+}
+
+uint64_t prefill_ws_bytes(int Dh) {
+    const int grid = sm_count(), rows = Dh == 256 ? 128 : 256;
+    return attn_desc_bytes(grid) + 2ull * grid * attn_part_floats(rows, Dh) * 4;
+}
+int launch_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t st) {
+    if (a.kv.Dh == 64) return run_prefill<64>(a, min_rows, ws, st);
+    return a.kv.Dh == 128 ? run_prefill<128>(a, min_rows, ws, st) : run_prefill<256>(a, min_rows, ws, st);
+}
+
+// Where a bounded wait gave up since the process began (0: nowhere).
+int prefill_wait_status(int *out, cudaStream_t st) {
+    if (cudaMemcpyFromSymbolAsync(out, g_prefill_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess) return check_launch();
+    return cudaStreamSynchronize(st) == cudaSuccess ? Q36_MOE_OK : check_launch();
+}
+
+}  // namespace q36

@@ -3,10 +3,11 @@
 // Rows are (new token, query head of the kv head's group): a tile of 256 rows (128 at 256-wide heads) shares K and V, so that the
 // cache is read and widened to bf16 once for all of them.  E2M1 times a power of two is exact in bf16.
 // One CTA, tiles of KT cached tokens:
-//   warps 8-11, 12-15   K, V of the next tile: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
-//   warp 16             S = Q K^T and O += P V on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's place)
-//   warps 0-3, 4-7      softmax of 128 rows each, a row per thread: maximum, 2^(S - m) rounded to bf16 once (half a step 2^-8, as
-//                       the output's), the sum of the unrounded weights in f32
+//   warps 0-3, 4-7   softmax of 128 rows each, a row per thread with all its scores in registers: maximum, 2^(S - m) rounded to
+//                    bf16 once (half a step 2^-8, as the output's), the sum of the unrounded weights in f32
+//   warps 8-11       K and V of the next tile: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
+//   warp 12          S = Q K^T and O += P V on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's place)
+// 256-wide heads have one row tile: there warps 8-11 widen K, 12-15 V, and warp 4 issues the products.
 // m is a lagging maximum: O is rescaled (in TMEM) only when a row would pass 2^8.
 // With two row tiles the tensor cores work on one while the other's softmax runs; 256-wide heads have one tile and two S.
 //
@@ -19,6 +20,10 @@
 
 namespace q36 {
 
+constexpr int PF_THREADS = 16 * 32;
+// registers after the roles part: softmax, widening, and whoever has least to do; 512 threads start with 128 each
+constexpr int PF_REGS_SOFTMAX = 184;
+
 template <int DH>
 struct PfCfg {
     static constexpr int NQ = DH == 256 ? 1 : 2, R = 128 * NQ, KT = DH == 256 ? 64 : 128;
@@ -27,10 +32,17 @@ struct PfCfg {
     static constexpr int SMEM = NQ * Q_BYTES + 4 * T_BYTES + 1024;
     static constexpr int TM_S = KT, TM_O0 = 2 * KT;                    // columns: S0 | S1 | O0 (| O1)
     static constexpr int TMEM = 512;
+    static constexpr int MMA_WARP = NQ == 2 ? 12 : 4;
+    static constexpr int REGS_W = NQ == 2 ? 80 : 96;                   // widening warps: one group (K and V) or two
+    static constexpr int REGS_X = 64;                   // warps 12-15 (NQ 2), 4-7 (NQ 1)
+    static_assert(NQ == 2 ? 2 * PF_REGS_SOFTMAX + REGS_W + REGS_X <= 512 : PF_REGS_SOFTMAX + 2 * REGS_W + REGS_X <= 512, "the block's registers");
 };
-constexpr int PF_THREADS = 17 * 32;
 constexpr float PF_NONE = -1.0e30f;      // "no token yet": finite, so that differences stay defined
 constexpr float PF_GROW = 8.f;
+#ifndef XSPAN
+#define XSPAN 192
+#endif
+constexpr int PF_SPAN = XSPAN;
 __device__ int g_prefill_status;         // where a wait gave up (0: nowhere)
 
 // ---------------------------------------------------------------- plan
@@ -58,7 +70,7 @@ __device__ __forceinline__ void pf_range(const AttnArgs &a, const PfSeq &s, int 
 // units of the row tiles before rt
 __device__ __forceinline__ long long pf_prefix(const AttnArgs &a, const PfSeq &s, int rt) {
     const long long base = s.len - s.n;
-    long long u = sum_pos(base + s.c, s.c, rt) + rt;
+    long long u = sum_pos(base + s.c, s.c, rt) + (long long)rt * PF_SPAN;
     if (rt > 0 && (long long)rt * s.c > s.n) u += max(0ll, base + s.n) - max(0ll, base + (long long)rt * s.c);     // the last tile is shorter
     if (a.window > 0) u -= sum_pos(base - a.window + 1, s.c, rt);
     return u;
@@ -88,7 +100,7 @@ struct PfSeg { int lo, hi, j0, j1, whole, head; long long units; };     // key t
 __device__ __forceinline__ PfSeg pf_segment(const AttnArgs &a, int KT, const PfPos &p) {
     PfSeg g;
     pf_range(a, p.s, p.rt, g.lo, g.hi);
-    g.units = (long long)(g.hi - g.lo) + 1;
+    g.units = (long long)(g.hi - g.lo) + PF_SPAN;
     const long long y0 = p.at - p.span_base, y1 = min(g.units, p.end - p.span_base);
     g.head = y0 == 0;
     g.whole = g.head && y1 == g.units;
@@ -97,10 +109,16 @@ __device__ __forceinline__ PfSeg pf_segment(const AttnArgs &a, int KT, const PfP
     g.j1 = y1 == g.units ? last : min((int)((g.lo + y1) / KT), last);
     return g;
 }
+// The span behind this one (spans of a request: row tiles of one kv head after the other); false behind the range.
 __device__ __forceinline__ bool pf_next(const AttnArgs &a, int R, int min_rows, const PfSeg &g, PfPos &p) {
     p.at = min(p.span_base + g.units, p.end);
     if (p.at >= p.end) return false;
-    pf_locate(a, R, min_rows, p);
+    p.span_base = p.at;
+    if (++p.rt < p.s.tiles) return true;
+    p.rt = 0;
+    if (++p.hk < a.kv.Hkv) return true;
+    p.hk = 0;
+    do p.s = pf_seq(a, R, min_rows, ++p.b); while (p.s.tiles == 0);
     return true;
 }
 
@@ -160,7 +178,29 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)), "l"(*reinterpret_cast<uint64_t *>(&c)));
+    return *reinterpret_cast<float2 *>(&r);
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(*reinterpret_cast<uint64_t *>(&a)), "l"(*reinterpret_cast<uint64_t *>(&b)));
+    return *reinterpret_cast<float2 *>(&r);
+}
+
 struct PfBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], q_full; };
+
+template <bool FIRST, typename A, typename B>
+__device__ __forceinline__ auto &pick(A &x, B &y) {
+    if constexpr (FIRST) return x;
+    else return y;
+}
+template <int NB>
+__device__ __forceinline__ uint32_t ld_scales(const uint8_t *p) {
+    if constexpr (NB == 2) return __ldg(reinterpret_cast<const uint16_t *>(p));
+    else return __ldg(reinterpret_cast<const uint32_t *>(p));
+}
 
 template <int DH>
 __global__ void __launch_bounds__(PF_THREADS, 1)
@@ -178,7 +218,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
     __shared__ long long plan_sum[PF_THREADS / 32], plan_base;
     __shared__ int plan_b;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t q_s = smem_u32(smem), k_s = q_s + NQ * C::Q_BYTES, v_s = k_s + 2 * C::T_BYTES;
+    const uint32_t q_s = smem_u32(smem), k_s = q_s + NQ * C::Q_BYTES, v_s = k_s + 2 * C::T_BYTES;      // K and V: two stages each
     auto bar = [&](uint64_t &b) { return smem_u32(&b); };
     if (tid == 0) {
         abort_flag = 0;
@@ -195,7 +235,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         desc[blockIdx.x].parts = 0;
     }
-    if (warp == 16) {
+    if (warp == C::MMA_WARP) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(C::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -238,16 +278,17 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
     const uint32_t tmem = tmem_s;
     bool more = pos.at < pos.end;
 
-    if (warp < 8) {
+    if (warp < 4 * NQ) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REGS_SOFTMAX));
         // ------------------------------------------------------------ softmax: a row per thread
         const int i = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         uint32_t sc = 0, oc = 0, kt = 0;       // tiles of this row tile, O's awaited, K tiles before this piece
         // a negative scale goes to the signs of q: m follows the largest score
-        const float scale2 = fabsf(a.scale2);
+        const float scale2 = fmaxf(fabsf(a.scale2), 1e-37f);      // (not 0: a hidden score stays -infinity)
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
         bool first = true, ok = true;
-        while (more && ok && i < NQ) {
+        while (more && ok) {
             const PfSeg g = pf_segment(a, KT, pos);
             const int r_tile = i * 128 + row, rows = min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G), r = pos.rt * pos.s.c * a.G + r_tile;
             const bool mine = r_tile < rows, active = i * 128 < rows && g.j0 < g.j1;
@@ -255,7 +296,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             if (g.j0 < g.j1) {
                 // Q: this thread's row (the MMAs that read the last one are over: its results were awaited)
                 const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (size_t)(pos.s.t0 + tok_i) * a.q_stride + (size_t)hq * DH);
-#pragma unroll 8
+#pragma unroll 16
                 for (int c = 0; c < DH / 8; c++) {
                     uint4 v = mine ? src[c] : make_uint4(0, 0, 0, 0);
                     v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
@@ -282,24 +323,33 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
 #pragma unroll
                     for (int w = 0; w < KT / 32; w++) bad |= bad_s[st][w];
                     const bool edge = bad || j * KT < all_lo || j * KT + KT - 1 > all_hi;
-                    auto masked = [&](uint32_t (&v)[32], int c) {
-                        const uint32_t b = bad_s[st][c >> 5];
+                    uint32_t v[KT / 32][32];
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            const int t = j * KT + c + e;
-                            if (t > hi_r || t < lo_r || (b >> e & 1)) v[e] = 0xff800000u;
+                    for (int c = 0; c < KT / 32; c++) tc_ld32(s_col + 32 * c, v[c]);
+                    tc_ld_wait();
+                    if (edge) {
+#pragma unroll
+                        for (int c = 0; c < KT / 32; c++) {
+                            // bits of the tokens that the row does not see
+                            const int t = j * KT + 32 * c, from = lo_r - t, to = hi_r - t;
+                            uint32_t hide = bad_s[st][c];
+                            hide |= from >= 32 ? 0xffffffffu : from > 0 ? (1u << from) - 1u : 0u;
+                            hide |= to < 0 ? 0xffffffffu : to < 31 ? 0xfffffffeu << to : 0u;
+#pragma unroll
+                            for (int e = 0; e < 32; e++)
+                                if (hide >> e & 1) v[c][e] = 0xff800000u;
                         }
-                    };
-                    float mx = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < KT; c += 32) {
-                        uint32_t v[32];
-                        tc_ld32(s_col + c, v);
-                        tc_ld_wait();
-                        if (edge) masked(v, c);
-#pragma unroll
-                        for (int e = 0; e < 32; e++) mx = fmaxf(mx, __uint_as_float(v[e]));
                     }
+                    float mc[KT / 32];
+#pragma unroll
+                    for (int c = 0; c < KT / 32; c++) {
+                        mc[c] = __uint_as_float(v[c][0]);
+#pragma unroll
+                        for (int e = 1; e < 32; e++) mc[c] = fmaxf(mc[c], __uint_as_float(v[c][e]));
+                    }
+                    float mx = mc[0];
+#pragma unroll
+                    for (int c = 1; c < KT / 32; c++) mx = fmaxf(mx, mc[c]);
                     const float top = mx == -INFINITY ? mx : mx * scale2;
                     const bool grow = top > m + PF_GROW;
                     if (__any_sync(0xffffffffu, grow)) {
@@ -323,25 +373,23 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                             }
                         }
                     }
+                    float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
+                    const float2 k2 = {scale2, scale2}, m2 = {-m, -m};
 #pragma unroll
-                    for (int c = 0; c < KT; c += 32) {
-                        uint32_t v[32], w[16];
-                        tc_ld32(s_col + c, v);
-                        tc_ld_wait();
-                        if (edge) masked(v, c);
+                    for (int c = 0; c < KT / 32; c++) {
+                        uint32_t w[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            float p0 = pf_ex2(fmaf(__uint_as_float(v[e]), scale2, -m)), p1 = pf_ex2(fmaf(__uint_as_float(v[e + 1]), scale2, -m));
-                            if (edge) {      // (a scale of 0 makes no -inf of a masked score)
-                                if (v[e] == 0xff800000u) p0 = 0.f;
-                                if (v[e + 1] == 0xff800000u) p1 = 0.f;
-                            }
-                            l += p0;
-                            l += p1;
-                            w[e / 2] = pack_bf16(p0, p1);
+                            float2 x = fma2(make_float2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), k2, m2);
+                            x.x = pf_ex2(x.x);
+                            x.y = pf_ex2(x.y);
+                            sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], x);
+                            w[e / 2] = pack_bf16(x.x, x.y);
                         }
-                        tc_st16(s_col + c / 2, w);
+                        tc_st16(s_col + 16 * c, w);
                     }
+                    sum[0] = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+                    l += sum[0].x + sum[0].y;
                     tc_st_wait();
                     tc_fence_before();
                     __syncwarp();
@@ -404,11 +452,11 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             kt += max(g.j1 - g.j0, 0);
             more = pf_next(a, R, min_rows, g, pos);
         }
-    } else if (warp < 16) {
-        // ------------------------------------------------------------ widening: warps 8-11 K, 12-15 V
-        const bool is_v = warp >= 12;
-        const int th = tid & 127, tl = th % KT, half = th / KT;     // token of the tile; which four scale blocks (256-wide heads)
-        const uint32_t dst0 = is_v ? v_s : k_s;
+    } else if (warp >= 8 && (NQ == 1 || warp < 12)) {
+        // ------------------------------------------------------------ widening: a token per thread (256-wide heads: half of one, K or V)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_W));
+        const int th = tid & 127, tl = th % KT, half = th / KT;
+        const bool do_k = NQ == 2 || warp < 12, do_v = NQ == 2 || warp >= 12;
         uint32_t kc = 0;
         bool ok = true;
         while (more && ok) {
@@ -418,78 +466,102 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 const int t = j * KT + tl, col = t >> a.kv.log_bs;
                 return j < g.j1 && t < pos.s.len && col < a.max_blocks ? __ldg(row + col) : -1;
             };
-            uint32_t raw_w[4 * BPT], scale = 0;
+            uint32_t kw[NQ == 2 ? 4 * BPT : 1], vw[NQ == 2 ? 4 * BPT : 1], kw1[NQ == 2 ? 1 : 4 * BPT], k_scale = 0, v_scale = 0;
+            auto &k_raw = pick<NQ == 2>(kw, kw1);
+            auto &v_raw = pick<NQ == 2>(vw, kw1);
             bool has = false;
             auto fetch = [&](int j, int id) {
                 has = id >= 0 && id < a.kv.n_blocks;
                 if (!has) return;
                 const int t = (j * KT + tl) & (a.kv.bs - 1);
                 const uint8_t *reg = a.kv.at(id, pos.hk);
-                const uint8_t *sp = reg + a.kv.bs * DH + (is_v ? a.kv.bs * NB : 0) + t * NB + half * 4;
-                if constexpr (NB == 2) scale = __ldg(reinterpret_cast<const uint16_t *>(sp));
-                else scale = __ldg(reinterpret_cast<const uint32_t *>(sp));
-                if (!is_v) {
+                const uint8_t *sp = reg + a.kv.bs * DH + t * NB + half * 4;
+                if (do_k) {
+                    k_scale = ld_scales<NB>(sp);
                     const uint8_t *src = reg + kv_k_off(t, 0, half * 4, DH);
 #pragma unroll
                     for (int q = 0; q < 4; q++) {       // word q of every block
                         if constexpr (BPT == 4) {
                             const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src + q * (DH / 8)));
-                            raw_w[4 * q] = u.x; raw_w[4 * q + 1] = u.y; raw_w[4 * q + 2] = u.z; raw_w[4 * q + 3] = u.w;
+                            k_raw[4 * q] = u.x; k_raw[4 * q + 1] = u.y; k_raw[4 * q + 2] = u.z; k_raw[4 * q + 3] = u.w;
                         } else {
                             const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
-                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                            k_raw[2 * q] = u.x; k_raw[2 * q + 1] = u.y;
                         }
                     }
-                } else {
+                }
+                if (do_v) {
+                    v_scale = ld_scales<NB>(sp + a.kv.bs * NB);
                     const uint8_t *src = reg + a.kv.bs * (DH / 2) + kv_v_off(t, 0, half * 4, DH);
 #pragma unroll
                     for (int q = 0; q < 8; q++) {       // four dims of every block
                         if constexpr (BPT == 4) {
                             const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
-                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                            v_raw[2 * q] = u.x; v_raw[2 * q + 1] = u.y;
                         } else {
-                            raw_w[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
+                            v_raw[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
                         }
                     }
                 }
+            };
+            // 16-byte chunk 4 b + q of the token's row: dims 32 b + 8 q ..
+            auto put = [&](uint8_t *dst, int b, int q, uint4 v) {
+                const int c = (half * 4 + b) * 4 + q;
+                *reinterpret_cast<uint4 *>(dst + (c >> 3) * (KT * 128) + (((c & 7) ^ (tl & 7)) << 4)) = v;
+            };
+            auto give = [&](uint64_t &b) {
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(b));
             };
             int id_next = page(g.j0 + 1);
             fetch(g.j0, page(g.j0));
             for (int j = g.j0; j < g.j1; j++, kc++) {
                 const uint32_t st = kc & 1, ph = (kc >> 1) & 1;
-                if (!(ok = mbar_wait(bar(is_v ? bars.v_empty[st] : bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, 0))) break;
-                __syncwarp();
-                uint8_t *dst = smem + (dst0 - q_s) + st * C::T_BYTES + tl * 128;
+                const uint4 none = make_uint4(0, 0, 0, 0);
+                if (do_k) {
+                    if (!(ok = mbar_wait(bar(bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                    __syncwarp();
+                    uint8_t *dst = smem + NQ * C::Q_BYTES + st * C::T_BYTES + tl * 128;
 #pragma unroll
-                for (int b = 0; b < BPT; b++) {
-                    const Lut t = make_lut((scale >> (8 * b)) & 0xff);
+                    for (int b = 0; b < BPT; b++) {
+                        const Lut t = make_lut((k_scale >> (8 * b)) & 0xff);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        uint32_t w;
-                        if (!is_v) w = raw_w[BPT * q + b];
-                        else w = __byte_perm(raw_w[(BPT / 2) * (2 * q) + b / 2], raw_w[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
-                        const uint4 v = has ? widen8(t, w) : make_uint4(0, 0, 0, 0);
-                        const int c = (half * 4 + b) * 4 + q;          // 16-byte chunk of the row
-                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * (KT * 128) + (((c & 7) ^ (tl & 7)) << 4)) = v;
+                        for (int q = 0; q < 4; q++) put(dst, b, q, has ? widen8(t, k_raw[BPT * q + b]) : none);
                     }
+                    if (half == 0) {
+                        // tokens of the request whose page is bad
+                        const uint32_t bad = __ballot_sync(0xffffffffu, !has && j * KT + tl < pos.s.len);
+                        if (lane == 0) bad_s[kc & 3][tl >> 5] = bad;
+                    }
+                    give(bars.k_full[st]);
                 }
-                if (!is_v && half == 0) {
-                    // tokens of the request whose page is bad
-                    const uint32_t bad = __ballot_sync(0xffffffffu, !has && j * KT + tl < pos.s.len);
-                    if (lane == 0) bad_s[kc & 3][tl >> 5] = bad;
+                if (do_v) {
+                    if (!(ok = mbar_wait(bar(bars.v_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x810 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                    __syncwarp();
+                    uint8_t *dst = smem + NQ * C::Q_BYTES + (2 + st) * C::T_BYTES + tl * 128;
+#pragma unroll
+                    for (int b = 0; b < BPT; b++) {
+                        const Lut t = make_lut((v_scale >> (8 * b)) & 0xff);
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const uint32_t w = __byte_perm(v_raw[(BPT / 2) * (2 * q) + b / 2], v_raw[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
+                            put(dst, b, q, has ? widen8(t, w) : none);
+                        }
+                    }
                 }
                 const int id = id_next;
                 if (j + 1 < g.j1) {
                     id_next = page(j + 2);
                     fetch(j + 1, id);
                 }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(is_v ? bars.v_full[st] : bars.k_full[st]));
+                if (do_v) give(bars.v_full[st]);
             }
             if (ok) more = pf_next(a, R, min_rows, g, pos);
         }
-    } else if (lane == 0) {
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_X));
+        if (warp == C::MMA_WARP && lane == 0) {
         // ------------------------------------------------------------ MMA
         uint32_t kq = 0, vq = 0, pq[2] = {0, 0}, qn = 0;
         bool ok = true;
@@ -562,11 +634,12 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             }
             if (ok) more = pf_next(a, R, min_rows, g, pos);
         }
+        }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    if (warp == C::MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
 }
 
 template <int DH>

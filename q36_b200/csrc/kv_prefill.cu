@@ -22,7 +22,7 @@ namespace q36 {
 
 constexpr int PF_THREADS = 16 * 32;
 // registers after the roles part: softmax, widening, and whoever has least to do; 512 threads start with 128 each
-constexpr int PF_REGS_SOFTMAX = 184;
+constexpr int PF_REGS_SOFTMAX = 168;
 
 template <int DH>
 struct PfCfg {
@@ -33,7 +33,7 @@ struct PfCfg {
     static constexpr int TM_S = KT, TM_O0 = 2 * KT;                    // columns: S0 | S1 | O0 (| O1)
     static constexpr int TMEM = 512;
     static constexpr int MMA_WARP = NQ == 2 ? 12 : 4;
-    static constexpr int REGS_W = NQ == 2 ? 80 : 96;                   // widening warps: one group (K and V) or two
+    static constexpr int REGS_W = 112;                                 // widening warps: one group (K and V) or two
     static constexpr int REGS_X = 64;                   // warps 12-15 (NQ 2), 4-7 (NQ 1)
     static_assert(NQ == 2 ? 2 * PF_REGS_SOFTMAX + REGS_W + REGS_X <= 512 : PF_REGS_SOFTMAX + 2 * REGS_W + REGS_X <= 512, "the block's registers");
 };
@@ -125,8 +125,10 @@ __device__ __forceinline__ bool pf_next(const AttnArgs &a, int R, int min_rows, 
 // ---------------------------------------------------------------- 4 bits -> bf16
 // The eight magnitudes of a block as bf16, high and low bytes apart: eight bytes each, picked by the three magnitude bits of a code.
 struct Lut { uint32_t ha, hb, la, lb; };
-__device__ __forceinline__ Lut make_lut(uint32_t s) {
-    const uint32_t p23 = s * 0x00800080u + 0x00400000u, p45 = p23 + 0x00800080u, p67 = p45 + 0x00800080u, p01 = ((s - 1) << 23);
+// `has` false: a token that is not there, all zeros.
+__device__ __forceinline__ Lut make_lut(uint32_t s, bool has) {
+    const uint32_t one = has ? 0x00800080u : 0u;
+    const uint32_t p23 = s * one + (has ? 0x00400000u : 0u), p45 = p23 + one, p67 = p45 + one, p01 = has ? (s - 1) << 23 : 0u;
     return Lut{__byte_perm(p01, p23, 0x7531), __byte_perm(p45, p67, 0x7531), __byte_perm(p01, p23, 0x6420), __byte_perm(p45, p67, 0x6420)};
 }
 __device__ __forceinline__ void widen4(const Lut &t, uint32_t sel, uint32_t sign, uint32_t &x, uint32_t &y) {
@@ -466,7 +468,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 const int t = j * KT + tl, col = t >> a.kv.log_bs;
                 return j < g.j1 && t < pos.s.len && col < a.max_blocks ? __ldg(row + col) : -1;
             };
-            uint32_t kw[NQ == 2 ? 4 * BPT : 1], vw[NQ == 2 ? 4 * BPT : 1], kw1[NQ == 2 ? 1 : 4 * BPT], k_scale = 0, v_scale = 0;
+            uint32_t kw[NQ == 2 ? 4 * BPT : 1] = {}, vw[NQ == 2 ? 4 * BPT : 1] = {}, kw1[NQ == 2 ? 1 : 4 * BPT] = {}, k_scale = 0, v_scale = 0;
             auto &k_raw = pick<NQ == 2>(kw, kw1);
             auto &v_raw = pick<NQ == 2>(vw, kw1);
             bool has = false;
@@ -518,16 +520,15 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             fetch(g.j0, page(g.j0));
             for (int j = g.j0; j < g.j1; j++, kc++) {
                 const uint32_t st = kc & 1, ph = (kc >> 1) & 1;
-                const uint4 none = make_uint4(0, 0, 0, 0);
                 if (do_k) {
                     if (!(ok = mbar_wait(bar(bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
                     __syncwarp();
                     uint8_t *dst = smem + NQ * C::Q_BYTES + st * C::T_BYTES + tl * 128;
 #pragma unroll
                     for (int b = 0; b < BPT; b++) {
-                        const Lut t = make_lut((k_scale >> (8 * b)) & 0xff);
+                        const Lut t = make_lut((k_scale >> (8 * b)) & 0xff, has);
 #pragma unroll
-                        for (int q = 0; q < 4; q++) put(dst, b, q, has ? widen8(t, k_raw[BPT * q + b]) : none);
+                        for (int q = 0; q < 4; q++) put(dst, b, q, widen8(t, k_raw[BPT * q + b]));
                     }
                     if (half == 0) {
                         // tokens of the request whose page is bad
@@ -542,11 +543,11 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                     uint8_t *dst = smem + NQ * C::Q_BYTES + (2 + st) * C::T_BYTES + tl * 128;
 #pragma unroll
                     for (int b = 0; b < BPT; b++) {
-                        const Lut t = make_lut((v_scale >> (8 * b)) & 0xff);
+                        const Lut t = make_lut((v_scale >> (8 * b)) & 0xff, has);
 #pragma unroll
                         for (int q = 0; q < 4; q++) {
                             const uint32_t w = __byte_perm(v_raw[(BPT / 2) * (2 * q) + b / 2], v_raw[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
-                            put(dst, b, q, has ? widen8(t, w) : none);
+                            put(dst, b, q, widen8(t, w));
                         }
                     }
                 }

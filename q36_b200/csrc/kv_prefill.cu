@@ -2,14 +2,14 @@
 //
 // Rows are (new token, query head of the kv head's group): a tile of 256 rows (128 at 256-wide heads) shares K and V, so that the
 // cache is read and widened to bf16 once for all of them.  E2M1 times a power of two is exact in bf16.
-// One CTA, tiles of KT cached tokens:
-//   warps 0-3, 4-7   softmax of 128 rows each, a row per thread with all its scores in registers: maximum, 2^(S - m) rounded to
-//                    bf16 once (half a step 2^-8, as the output's), the sum of the unrounded weights in f32
-//   warps 8-11       K and V of the next tile: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
-//   warp 12          S = Q K^T and O += P V on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's place)
-// 256-wide heads have one row tile: there warps 8-11 widen K, 12-15 V, and warp 4 issues the products.
+// One CTA, tiles of 64 cached tokens:
+//   warps 0-3, 4-7     softmax of 128 rows each, a row per thread with its scores in registers: maximum, 2^(S - m) rounded to bf16
+//                      once (half a step 2^-8, as the output's), the sum of the unrounded weights in f32
+//   warps 8-11, 12-15  K, V: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
+//   warps 16, 17       S = Q K^T and O += P V on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's place), a row tile each:
+//                      one thread issues an MMA per 90 cycles at most, which the pipe needs 32 to 64 for
+// Every row tile has two S, so that the products of a tile run while the softmax is at the one before.
 // m is a lagging maximum: O is rescaled (in TMEM) only when a row would pass 2^8.
-// With two row tiles the tensor cores work on one while the other's softmax runs; 256-wide heads have one tile and two S.
 //
 // Work: the spans (kv head, row tile) of all long requests, measured in the tokens they see, are cut into equal ranges, one per CTA;
 // cuts are moved down to tile boundaries.  Cut spans are joined as in the decode kernel.
@@ -20,22 +20,19 @@
 
 namespace q36 {
 
-constexpr int PF_THREADS = 16 * 32;
-// registers after the roles part: softmax, widening, and whoever has least to do; 512 threads start with 128 each
-constexpr int PF_REGS_SOFTMAX = 168;
+constexpr int PF_THREADS = 20 * 32;
+// registers after the roles part: softmax, widening, issuers; 640 threads start with 96 each
+constexpr int PF_REGS_SOFTMAX = 120, PF_REGS_WIDEN = 88, PF_REGS_ISSUE = 64;
+static_assert(2 * PF_REGS_SOFTMAX + 2 * PF_REGS_WIDEN + PF_REGS_ISSUE <= 5 * 96, "the block's registers");
 
 template <int DH>
 struct PfCfg {
-    static constexpr int NQ = DH == 256 ? 1 : 2, R = 128 * NQ, KT = DH == 256 ? 64 : 128;
-    static constexpr int NB = DH / 32, BPT = NB < 4 ? NB : 4;          // scale blocks, and those a widening thread has
+    static constexpr int NQ = DH == 256 ? 1 : 2, R = 128 * NQ, KT = 64, STAGES = DH == 256 ? 2 : 4;
+    static constexpr int NB = DH / 32, BPT = NB / 2;                   // scale blocks, and those a widening thread has
     static constexpr int Q_BYTES = 128 * DH * 2, T_BYTES = KT * DH * 2;
-    static constexpr int SMEM = NQ * Q_BYTES + 4 * T_BYTES + 1024;
-    static constexpr int TM_S = KT, TM_O0 = 2 * KT;                    // columns: S0 | S1 | O0 (| O1)
+    static constexpr int SMEM = NQ * Q_BYTES + 2 * STAGES * T_BYTES + 1024;
+    static constexpr int TM_S = KT, TM_O0 = 2 * NQ * KT;               // columns: two S of each row tile, then O of each
     static constexpr int TMEM = 512;
-    static constexpr int MMA_WARP = NQ == 2 ? 12 : 4;
-    static constexpr int REGS_W = 112;                                 // widening warps: one group (K and V) or two
-    static constexpr int REGS_X = 64;                   // warps 12-15 (NQ 2), 4-7 (NQ 1)
-    static_assert(NQ == 2 ? 2 * PF_REGS_SOFTMAX + REGS_W + REGS_X <= 512 : PF_REGS_SOFTMAX + 2 * REGS_W + REGS_X <= 512, "the block's registers");
 };
 constexpr float PF_NONE = -1.0e30f;      // "no token yet": finite, so that differences stay defined
 constexpr float PF_GROW = 8.f;
@@ -191,16 +188,13 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return *reinterpret_cast<float2 *>(&r);
 }
 
-struct PfBars { uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2], q_full; };
+struct PfBars { uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], q_full[2]; };
 
-template <bool FIRST, typename A, typename B>
-__device__ __forceinline__ auto &pick(A &x, B &y) {
-    if constexpr (FIRST) return x;
-    else return y;
-}
-template <int NB>
-__device__ __forceinline__ uint32_t ld_scales(const uint8_t *p) {
-    if constexpr (NB == 2) return __ldg(reinterpret_cast<const uint16_t *>(p));
+// 1, 2 or 4 bytes
+template <int BYTES>
+__device__ __forceinline__ uint32_t ld_part(const uint8_t *p) {
+    if constexpr (BYTES == 1) return __ldg(p);
+    else if constexpr (BYTES == 2) return __ldg(reinterpret_cast<const uint16_t *>(p));
     else return __ldg(reinterpret_cast<const uint32_t *>(p));
 }
 
@@ -208,36 +202,37 @@ template <int DH>
 __global__ void __launch_bounds__(PF_THREADS, 1)
 k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__restrict__ part) {
     using C = PfCfg<DH>;
-    constexpr int NQ = C::NQ, R = C::R, KT = C::KT, NB = C::NB, BPT = C::BPT;
+    constexpr int NQ = C::NQ, R = C::R, KT = C::KT, NB = C::NB, BPT = C::BPT, ST = C::STAGES;
     constexpr uint32_t ID_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
     constexpr uint32_t ID_PV = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | ((uint32_t)(DH >> 3) << 17) | (8u << 24);
     Q36_GDS();
     extern __shared__ uint8_t raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ PfBars bars;
-    __shared__ uint32_t tmem_s, bad_s[4][4];      // bad_s: tokens of a tile whose page is bad; a ring of 4, since K runs ahead of the softmax
+    __shared__ uint32_t tmem_s, bad_s[8][2];      // bad_s: tokens of a tile whose page is bad; a ring of 8: K runs up to 5 tiles ahead of the softmax
     __shared__ volatile int abort_flag;
     __shared__ long long plan_sum[PF_THREADS / 32], plan_base;
     __shared__ int plan_b;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t q_s = smem_u32(smem), k_s = q_s + NQ * C::Q_BYTES, v_s = k_s + 2 * C::T_BYTES;      // K and V: two stages each
+    const uint32_t q_s = smem_u32(smem), k_s = q_s + NQ * C::Q_BYTES, v_s = k_s + ST * C::T_BYTES;
     auto bar = [&](uint64_t &b) { return smem_u32(&b); };
     if (tid == 0) {
         abort_flag = 0;
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < ST; i++) {
             mbar_init(bar(bars.k_full[i]), 4);
             mbar_init(bar(bars.v_full[i]), 4);
-            mbar_init(bar(bars.k_empty[i]), 1);
-            mbar_init(bar(bars.v_empty[i]), 1);
-            mbar_init(bar(bars.s_full[i]), 1);
-            mbar_init(bar(bars.p_full[i]), 4);
-            mbar_init(bar(bars.o_done[i]), 1);
+            mbar_init(bar(bars.k_empty[i]), NQ);
+            mbar_init(bar(bars.v_empty[i]), NQ);
         }
-        mbar_init(bar(bars.q_full), 4 * NQ);
+        for (int i = 0; i < 2; i++) {
+            for (int x = 0; x < 2; x++) { mbar_init(bar(bars.s_full[i][x]), 1); mbar_init(bar(bars.p_full[i][x]), 4); }
+            mbar_init(bar(bars.o_done[i]), 1);
+            mbar_init(bar(bars.q_full[i]), 4);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         desc[blockIdx.x].parts = 0;
     }
-    if (warp == C::MMA_WARP) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_s)), "r"(C::TMEM) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -280,7 +275,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
     const uint32_t tmem = tmem_s;
     bool more = pos.at < pos.end;
 
-    if (warp < 4 * NQ) {
+    if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REGS_SOFTMAX));
         // ------------------------------------------------------------ softmax: a row per thread
         const int i = warp >> 2, row = tid & 127;
@@ -290,12 +285,12 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         const float scale2 = fmaxf(fabsf(a.scale2), 1e-37f);      // (not 0: a hidden score stays -infinity)
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
         bool first = true, ok = true;
-        while (more && ok) {
+        while (more && ok && i < NQ) {
             const PfSeg g = pf_segment(a, KT, pos);
             const int r_tile = i * 128 + row, rows = min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G), r = pos.rt * pos.s.c * a.G + r_tile;
             const bool mine = r_tile < rows, active = i * 128 < rows && g.j0 < g.j1;
             const int tok_i = mine ? r / a.G : 0, hq = pos.hk * a.G + (mine ? r - tok_i * a.G : 0);
-            if (g.j0 < g.j1) {
+            if (active) {
                 // Q: this thread's row (the MMAs that read the last one are over: its results were awaited)
                 const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (size_t)(pos.s.t0 + tok_i) * a.q_stride + (size_t)hq * DH);
 #pragma unroll 16
@@ -306,7 +301,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar(bars.q_full));
+                if (lane == 0) mbar_arrive(bar(bars.q_full[i]));
             }
             const int p = pos.s.len - pos.s.n + tok_i;              // position; the row sees [lo_r, p]
             const int hi_r = mine ? p : -1, lo_r = a.window > 0 ? p - a.window + 1 : 0;
@@ -315,12 +310,12 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 const int t_first = min((pos.rt * pos.s.c * a.G + i * 128) / a.G, pos.s.n - 1), t_last = min((pos.rt * pos.s.c * a.G + min(i * 128 + 127, rows - 1)) / a.G, pos.s.n - 1);
                 const int all_hi = pos.s.len - pos.s.n + t_first, all_lo = a.window > 0 ? pos.s.len - pos.s.n + t_last - a.window + 1 : 0;
                 for (int j = g.j0; j < g.j1; j++, sc++) {
-                    const uint32_t x = NQ == 2 ? i : sc & 1, ph = NQ == 2 ? sc & 1 : (sc >> 1) & 1;
-                    if (!(ok = mbar_wait(bar(bars.s_full[x]), ph, &abort_flag, &g_prefill_status, 0x500 + x, TC_SPIN_LIMIT, 0))) break;
+                    const uint32_t x = sc & 1, ph = (sc >> 1) & 1;
+                    if (!(ok = mbar_wait(bar(bars.s_full[i][x]), ph, &abort_flag, &g_prefill_status, 0x500 + x, TC_SPIN_LIMIT, 0))) break;
                     __syncwarp();
                     tc_fence_after();
-                    const uint32_t s_col = tmem + lanes + x * C::TM_S;
-                    const uint32_t st = (kt + (j - g.j0)) & 3;       // its place in bad_s
+                    const uint32_t s_col = tmem + lanes + (2 * i + x) * C::TM_S;
+                    const uint32_t st = (kt + (j - g.j0)) & 7;       // its place in bad_s
                     uint32_t bad = 0;
 #pragma unroll
                     for (int w = 0; w < KT / 32; w++) bad |= bad_s[st][w];
@@ -360,7 +355,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                         m = mn;
                         if (j > g.j0) {
                             // O holds the tiles before this one
-                            if (NQ == 1 && !(ok = mbar_wait(bar(bars.o_done[0]), (oc + (j - g.j0) - 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
+                            if (!(ok = mbar_wait(bar(bars.o_done[i]), (oc + (j - g.j0) - 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
                             __syncwarp();
                             tc_fence_after();
 #pragma unroll 1
@@ -395,15 +390,15 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                     tc_st_wait();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(bar(bars.p_full[x]));
+                    if (lane == 0) mbar_arrive(bar(bars.p_full[i][x]));
                 }
                 if (!ok) break;
                 // ---- the piece's result
-                const uint32_t n_o = NQ == 2 ? 1 : (uint32_t)(g.j1 - g.j0);
+                const uint32_t n_o = (uint32_t)(g.j1 - g.j0);
                 oc += n_o;
-                // (two S: the product before the last may be under way too, and a parity names one phase of two)
-                if (NQ == 1 && n_o > 1 && !(ok = mbar_wait(bar(bars.o_done[0]), oc & 1, &abort_flag, &g_prefill_status, 0x710, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
-                if (!(ok = mbar_wait(bar(bars.o_done[NQ == 2 ? i : 0]), (oc - 1) & 1, &abort_flag, &g_prefill_status, 0x700 + i, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                // (the product before the last may be under way too, and a parity names one phase of two)
+                if (n_o > 1 && !(ok = mbar_wait(bar(bars.o_done[i]), oc & 1, &abort_flag, &g_prefill_status, 0x710, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                if (!(ok = mbar_wait(bar(bars.o_done[i]), (oc - 1) & 1, &abort_flag, &g_prefill_status, 0x700 + i, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
                 __syncwarp();
                 tc_fence_after();
             }
@@ -454,11 +449,11 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             kt += max(g.j1 - g.j0, 0);
             more = pf_next(a, R, min_rows, g, pos);
         }
-    } else if (warp >= 8 && (NQ == 1 || warp < 12)) {
-        // ------------------------------------------------------------ widening: a token per thread (256-wide heads: half of one, K or V)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_W));
+    } else if (warp < 16) {
+        // ------------------------------------------------------------ widening: half a token of K or V per thread
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_WIDEN));
         const int th = tid & 127, tl = th % KT, half = th / KT;
-        const bool do_k = NQ == 2 || warp < 12, do_v = NQ == 2 || warp >= 12;
+        const bool is_v = warp >= 12;
         uint32_t kc = 0;
         bool ok = true;
         while (more && ok) {
@@ -468,179 +463,140 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 const int t = j * KT + tl, col = t >> a.kv.log_bs;
                 return j < g.j1 && t < pos.s.len && col < a.max_blocks ? __ldg(row + col) : -1;
             };
-            uint32_t kw[NQ == 2 ? 4 * BPT : 1] = {}, vw[NQ == 2 ? 4 * BPT : 1] = {}, kw1[NQ == 2 ? 1 : 4 * BPT] = {}, k_scale = 0, v_scale = 0;
-            auto &k_raw = pick<NQ == 2>(kw, kw1);
-            auto &v_raw = pick<NQ == 2>(vw, kw1);
+            uint32_t raw_w[BPT == 1 ? 8 : 4 * BPT] = {}, scale = 0;
             bool has = false;
             auto fetch = [&](int j, int id) {
                 has = id >= 0 && id < a.kv.n_blocks;
                 if (!has) return;
                 const int t = (j * KT + tl) & (a.kv.bs - 1);
                 const uint8_t *reg = a.kv.at(id, pos.hk);
-                const uint8_t *sp = reg + a.kv.bs * DH + t * NB + half * 4;
-                if (do_k) {
-                    k_scale = ld_scales<NB>(sp);
-                    const uint8_t *src = reg + kv_k_off(t, 0, half * 4, DH);
+                scale = ld_part<BPT>(reg + a.kv.bs * DH + (is_v ? a.kv.bs * NB : 0) + t * NB + half * BPT);
+                if (!is_v) {
+                    const uint8_t *src = reg + kv_k_off(t, 0, half * BPT, DH);
 #pragma unroll
                     for (int q = 0; q < 4; q++) {       // word q of every block
                         if constexpr (BPT == 4) {
                             const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src + q * (DH / 8)));
-                            k_raw[4 * q] = u.x; k_raw[4 * q + 1] = u.y; k_raw[4 * q + 2] = u.z; k_raw[4 * q + 3] = u.w;
-                        } else {
+                            raw_w[4 * q] = u.x; raw_w[4 * q + 1] = u.y; raw_w[4 * q + 2] = u.z; raw_w[4 * q + 3] = u.w;
+                        } else if constexpr (BPT == 2) {
                             const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
-                            k_raw[2 * q] = u.x; k_raw[2 * q + 1] = u.y;
+                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                        } else {
+                            raw_w[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
                         }
                     }
-                }
-                if (do_v) {
-                    v_scale = ld_scales<NB>(sp + a.kv.bs * NB);
-                    const uint8_t *src = reg + a.kv.bs * (DH / 2) + kv_v_off(t, 0, half * 4, DH);
+                } else {
+                    const uint8_t *src = reg + a.kv.bs * (DH / 2) + kv_v_off(t, 0, half * BPT, DH);
 #pragma unroll
                     for (int q = 0; q < 8; q++) {       // four dims of every block
                         if constexpr (BPT == 4) {
                             const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
-                            v_raw[2 * q] = u.x; v_raw[2 * q + 1] = u.y;
+                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
                         } else {
-                            v_raw[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
+                            raw_w[q] = ld_part<2 * BPT>(src + q * (DH / 8));
                         }
                     }
                 }
-            };
-            // 16-byte chunk 4 b + q of the token's row: dims 32 b + 8 q ..
-            auto put = [&](uint8_t *dst, int b, int q, uint4 v) {
-                const int c = (half * 4 + b) * 4 + q;
-                *reinterpret_cast<uint4 *>(dst + (c >> 3) * (KT * 128) + (((c & 7) ^ (tl & 7)) << 4)) = v;
-            };
-            auto give = [&](uint64_t &b) {
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(b));
             };
             int id_next = page(g.j0 + 1);
             fetch(g.j0, page(g.j0));
             for (int j = g.j0; j < g.j1; j++, kc++) {
-                const uint32_t st = kc & 1, ph = (kc >> 1) & 1;
-                if (do_k) {
-                    if (!(ok = mbar_wait(bar(bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
-                    __syncwarp();
-                    uint8_t *dst = smem + NQ * C::Q_BYTES + st * C::T_BYTES + tl * 128;
+                const uint32_t st = kc % ST, ph = (kc / ST) & 1;
+                if (!(ok = mbar_wait(bar(is_v ? bars.v_empty[st] : bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                __syncwarp();
+                uint8_t *dst = smem + NQ * C::Q_BYTES + ((is_v ? ST : 0) + st) * C::T_BYTES + tl * 128;
 #pragma unroll
-                    for (int b = 0; b < BPT; b++) {
-                        const Lut t = make_lut((k_scale >> (8 * b)) & 0xff, has);
+                for (int b = 0; b < BPT; b++) {
+                    const Lut t = make_lut((scale >> (8 * b)) & 0xff, has);
 #pragma unroll
-                        for (int q = 0; q < 4; q++) put(dst, b, q, widen8(t, k_raw[BPT * q + b]));
+                    for (int q = 0; q < 4; q++) {
+                        uint32_t w;
+                        if (!is_v) w = raw_w[BPT * q + b];
+                        else if constexpr (BPT == 1) w = raw_w[2 * q] | raw_w[2 * q + 1] << 16;
+                        else w = __byte_perm(raw_w[(BPT / 2) * (2 * q) + b / 2], raw_w[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
+                        const int c = (half * BPT + b) * 4 + q;      // 16-byte chunk of the token's row: dims 8 c ..
+                        *reinterpret_cast<uint4 *>(dst + (c >> 3) * (KT * 128) + (((c & 7) ^ (tl & 7)) << 4)) = widen8(t, w);
                     }
-                    if (half == 0) {
-                        // tokens of the request whose page is bad
-                        const uint32_t bad = __ballot_sync(0xffffffffu, !has && j * KT + tl < pos.s.len);
-                        if (lane == 0) bad_s[kc & 3][tl >> 5] = bad;
-                    }
-                    give(bars.k_full[st]);
                 }
-                if (do_v) {
-                    if (!(ok = mbar_wait(bar(bars.v_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x810 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
-                    __syncwarp();
-                    uint8_t *dst = smem + NQ * C::Q_BYTES + (2 + st) * C::T_BYTES + tl * 128;
-#pragma unroll
-                    for (int b = 0; b < BPT; b++) {
-                        const Lut t = make_lut((v_scale >> (8 * b)) & 0xff, has);
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {
-                            const uint32_t w = __byte_perm(v_raw[(BPT / 2) * (2 * q) + b / 2], v_raw[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
-                            put(dst, b, q, widen8(t, w));
-                        }
-                    }
+                if (!is_v && half == 0) {
+                    // tokens of the request whose page is bad
+                    const uint32_t bad = __ballot_sync(0xffffffffu, !has && j * KT + tl < pos.s.len);
+                    if (lane == 0) bad_s[kc & 7][tl >> 5] = bad;
                 }
                 const int id = id_next;
                 if (j + 1 < g.j1) {
                     id_next = page(j + 2);
                     fetch(j + 1, id);
                 }
-                if (do_v) give(bars.v_full[st]);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(is_v ? bars.v_full[st] : bars.k_full[st]));
             }
             if (ok) more = pf_next(a, R, min_rows, g, pos);
         }
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REGS_X));
-        if (warp == C::MMA_WARP && lane == 0) {
-        // ------------------------------------------------------------ MMA
-        uint32_t kq = 0, vq = 0, pq[2] = {0, 0}, qn = 0;
-        bool ok = true;
-        auto wait = [&](uint64_t &b, uint32_t ph, int where) { ok = ok && mbar_wait(bar(b), ph, &abort_flag, &g_prefill_status, where); };
-        auto qk = [&](int i, uint32_t x, uint32_t st) {
-            const uint32_t qa = q_s + i * C::Q_BYTES, kb = k_s + st * C::T_BYTES;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_ISSUE));
+        if (warp < 16 + NQ && lane == 0) {
+            // ------------------------------------------------------------ products of row tile i
+            const int i = warp - 16;
+            uint32_t kq = 0, vq = 0, sq = 0, pq = 0, qn = 0;       // K and V tiles passed, S issued, P awaited, Q awaited
+            bool ok = true;
+            auto wait = [&](uint64_t &b, uint32_t ph, int where) { ok = ok && mbar_wait(bar(b), ph, &abort_flag, &g_prefill_status, where); };
+            const uint32_t qa = q_s + i * C::Q_BYTES;
+            while (more && ok) {
+                const PfSeg g = pf_segment(a, KT, pos);
+                const int n = g.j1 - g.j0;
+                // a tile without rows only passes the stages on
+                const bool active = i * 128 < min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G);
+                auto next_s = [&]() {
+                    const uint32_t st = kq % ST;
+                    wait(bars.k_full[st], (kq / ST) & 1, 0x210);
+                    kq++;
+                    if (!ok) return;
+                    if (!active) { mbar_arrive(bar(bars.k_empty[st])); return; }
+                    tc_fence_after();
+                    const uint32_t kb = k_s + st * C::T_BYTES, d = tmem + (2 * i + (sq & 1)) * C::TM_S;
 #pragma unroll
-            for (int kk = 0; kk < DH / 16; kk++)
-                pf_mma_ss(tmem + x * C::TM_S, desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32), desc_sw128(kb + (kk >> 2) * (KT * 128) + (kk & 3) * 32), ID_QK, kk ? 1u : 0u);
-        };
-        auto pv = [&](int i, uint32_t x, uint32_t st, bool more_than_first) {
-            const uint32_t vb = v_s + st * C::T_BYTES;
-#pragma unroll
-            for (int kk = 0; kk < KT / 16; kk++)
-                pf_mma_ts(tmem + C::TM_O0 + i * DH, tmem + x * C::TM_S + kk * 8, desc_n_major(vb + kk * 2048, KT * 128), ID_PV, (more_than_first || kk) ? 1u : 0u);
-        };
-        while (more && ok) {
-            const PfSeg g = pf_segment(a, KT, pos);
-            const int rows = min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G), nq = NQ == 2 && rows > 128 ? 2 : 1, n = g.j1 - g.j0;
-            if (n > 0) {
-                wait(bars.q_full, qn & 1, 0x100);
-                qn++;
-                if (NQ == 2) {
-                    for (int j = -1; j < n && ok; j++) {
-                        if (j >= 0) wait(bars.v_full[vq & 1], (vq >> 1) & 1, 0x200);
-                        if (j + 1 < n) wait(bars.k_full[kq & 1], (kq >> 1) & 1, 0x210);
-                        for (int i = 0; i < nq && ok; i++) {
-                            if (j >= 0) {
-                                wait(bars.p_full[i], pq[i] & 1, 0x300 + i);
-                                pq[i]++;
-                                if (!ok) break;
-                                tc_fence_after();
-                                pv(i, i, vq & 1, j > 0);
-                                if (i == nq - 1) tc_commit(bar(bars.v_empty[vq & 1]));
-                                if (j == n - 1) tc_commit(bar(bars.o_done[i]));
-                            }
-                            if (j + 1 < n && ok) {
-                                tc_fence_after();
-                                qk(i, i, kq & 1);
-                                tc_commit(bar(bars.s_full[i]));
-                            }
-                        }
-                        if (j >= 0) vq++;
-                        if (j + 1 < n) { if (ok) tc_commit(bar(bars.k_empty[kq & 1])); kq++; }
-                    }
-                } else {
-                    auto one_qk = [&]() {
-                        wait(bars.k_full[kq & 1], (kq >> 1) & 1, 0x210);
-                        if (!ok) return;
-                        tc_fence_after();
-                        qk(0, kq & 1, kq & 1);
-                        tc_commit(bar(bars.s_full[kq & 1]));
-                        tc_commit(bar(bars.k_empty[kq & 1]));
-                        kq++;
-                    };
-                    one_qk();
-                    if (n > 1 && ok) one_qk();
+                    for (int kk = 0; kk < DH / 16; kk++)
+                        pf_mma_ss(d, desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32), desc_sw128(kb + (kk >> 2) * (KT * 128) + (kk & 3) * 32), ID_QK, kk ? 1u : 0u);
+                    tc_commit(bar(bars.s_full[i][sq & 1]));
+                    tc_commit(bar(bars.k_empty[st]));
+                    sq++;
+                };
+                if (n > 0) {
+                    if (active) wait(bars.q_full[i], qn++ & 1, 0x100);
+                    if (ok) next_s();
+                    if (n > 1 && ok) next_s();
                     for (int j = 0; j < n && ok; j++) {
-                        wait(bars.v_full[vq & 1], (vq >> 1) & 1, 0x200);
-                        wait(bars.p_full[vq & 1], (vq >> 1) & 1, 0x300);
-                        if (!ok) break;
-                        tc_fence_after();
-                        pv(0, vq & 1, vq & 1, j > 0);
-                        tc_commit(bar(bars.v_empty[vq & 1]));
-                        tc_commit(bar(bars.o_done[0]));
+                        const uint32_t st = vq % ST;
+                        wait(bars.v_full[st], (vq / ST) & 1, 0x200);
                         vq++;
-                        if (j + 2 < n) one_qk();
+                        if (!ok) break;
+                        if (active) {
+                            wait(bars.p_full[i][pq & 1], (pq >> 1) & 1, 0x300);
+                            if (!ok) break;
+                            tc_fence_after();
+                            const uint32_t vb = v_s + st * C::T_BYTES, pa = tmem + (2 * i + (pq & 1)) * C::TM_S;
+#pragma unroll
+                            for (int kk = 0; kk < KT / 16; kk++)
+                                pf_mma_ts(tmem + C::TM_O0 + i * DH, pa + kk * 8, desc_n_major(vb + kk * 2048, KT * 128), ID_PV, (j > 0 || kk) ? 1u : 0u);
+                            tc_commit(bar(bars.v_empty[st]));
+                            tc_commit(bar(bars.o_done[i]));
+                            pq++;
+                        } else {
+                            mbar_arrive(bar(bars.v_empty[st]));
+                        }
+                        if (j + 2 < n) next_s();
                     }
                 }
+                if (ok) more = pf_next(a, R, min_rows, g, pos);
             }
-            if (ok) more = pf_next(a, R, min_rows, g, pos);
-        }
         }
     }
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == C::MMA_WARP) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
 }
 
 template <int DH>

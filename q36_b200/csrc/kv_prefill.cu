@@ -188,7 +188,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return *reinterpret_cast<float2 *>(&r);
 }
 
-struct PfBars { uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], q_full[2]; };
+struct PfBars { uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], o_last[2], q_full[2]; };      // o_done: every product with V, o_last: a piece's last
 
 // 1, 2 or 4 bytes
 template <int BYTES>
@@ -227,6 +227,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         for (int i = 0; i < 2; i++) {
             for (int x = 0; x < 2; x++) { mbar_init(bar(bars.s_full[i][x]), 1); mbar_init(bar(bars.p_full[i][x]), 4); }
             mbar_init(bar(bars.o_done[i]), 1);
+            mbar_init(bar(bars.o_last[i]), 1);
             mbar_init(bar(bars.q_full[i]), 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -280,7 +281,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         // ------------------------------------------------------------ softmax: a row per thread
         const int i = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        uint32_t sc = 0, oc = 0, kt = 0;       // tiles of this row tile, O's awaited, K tiles before this piece
+        uint32_t sc = 0, oc = 0, kt = 0, pieces = 0;       // tiles of this row tile, its products with V and K tiles before this piece, pieces
         // a negative scale goes to the signs of q: m follows the largest score
         const float scale2 = fmaxf(fabsf(a.scale2), 1e-37f);      // (not 0: a hidden score stays -infinity)
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
@@ -354,7 +355,8 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                         l *= f;
                         m = mn;
                         if (j > g.j0) {
-                            // O holds the tiles before this one
+                            // O holds the tiles before this one.  (S(j) being there says that PV(j - 2) is over: of the two phases
+                            // that a parity tells apart, the one awaited is the latest that can be open.)
                             if (!(ok = mbar_wait(bar(bars.o_done[i]), (oc + (j - g.j0) - 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
                             __syncwarp();
                             tc_fence_after();
@@ -394,11 +396,8 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 }
                 if (!ok) break;
                 // ---- the piece's result
-                const uint32_t n_o = (uint32_t)(g.j1 - g.j0);
-                oc += n_o;
-                // (the product before the last may be under way too, and a parity names one phase of two)
-                if (n_o > 1 && !(ok = mbar_wait(bar(bars.o_done[i]), oc & 1, &abort_flag, &g_prefill_status, 0x710, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
-                if (!(ok = mbar_wait(bar(bars.o_done[i]), (oc - 1) & 1, &abort_flag, &g_prefill_status, 0x700 + i, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
+                oc += (uint32_t)(g.j1 - g.j0);
+                if (!(ok = mbar_wait(bar(bars.o_last[i]), pieces++ & 1, &abort_flag, &g_prefill_status, 0x700 + i, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
                 __syncwarp();
                 tc_fence_after();
             }
@@ -582,6 +581,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                                 pf_mma_ts(tmem + C::TM_O0 + i * DH, pa + kk * 8, desc_n_major(vb + kk * 2048, KT * 128), ID_PV, (j > 0 || kk) ? 1u : 0u);
                             tc_commit(bar(bars.v_empty[st]));
                             tc_commit(bar(bars.o_done[i]));
+                            if (j == n - 1) tc_commit(bar(bars.o_last[i]));
                             pq++;
                         } else {
                             mbar_arrive(bar(bars.v_empty[st]));

@@ -6,8 +6,8 @@
 //   warps 0-3, 4-7     softmax of 128 rows each, a row per thread with its scores in registers: maximum, 2^(S - m) rounded to bf16
 //                      once (half a step 2^-8, as the output's), the sum of the unrounded weights in f32
 //   warps 8-11, 12-15  K, V: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
-//   warps 16, 17       S = Q K^T and O += P V on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's place), a row tile each:
-//                      one thread issues an MMA per 90 cycles at most, which the pipe needs 32 to 64 for
+//   warps 16 - 19      S = Q K^T and O += P V of each row tile on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's
+//                      place): one thread issues an MMA per 90 cycles at most, which the pipe needs 32 to 64 for
 // Every row tile has two S, so that the products of a tile run while the softmax is at the one before.
 // m is a lagging maximum: O is rescaled (in TMEM) only when a row would pass 2^8.
 //
@@ -188,7 +188,9 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return *reinterpret_cast<float2 *>(&r);
 }
 
-struct PfBars { uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2], o_last[2], q_full[2]; };      // o_done: every product with V, o_last: a piece's last
+// Every wait names a phase by its parity, so no barrier may be two phases on from one that is still to be awaited: the P / O barriers
+// are one per place, whose next phase needs what follows the wait.
+struct PfBars { uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2][2], p_full[2][2], o_done[2][2], o_last[2], q_full[2]; };      // o_done: product with the P in one of two places, o_last: a piece's last
 
 // 1, 2 or 4 bytes
 template <int BYTES>
@@ -225,8 +227,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             mbar_init(bar(bars.v_empty[i]), NQ);
         }
         for (int i = 0; i < 2; i++) {
-            for (int x = 0; x < 2; x++) { mbar_init(bar(bars.s_full[i][x]), 1); mbar_init(bar(bars.p_full[i][x]), 4); }
-            mbar_init(bar(bars.o_done[i]), 1);
+            for (int x = 0; x < 2; x++) { mbar_init(bar(bars.s_full[i][x]), 1); mbar_init(bar(bars.p_full[i][x]), 4); mbar_init(bar(bars.o_done[i][x]), 1); }
             mbar_init(bar(bars.o_last[i]), 1);
             mbar_init(bar(bars.q_full[i]), 4);
         }
@@ -281,7 +282,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         // ------------------------------------------------------------ softmax: a row per thread
         const int i = warp >> 2, row = tid & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        uint32_t sc = 0, oc = 0, kt = 0, pieces = 0;       // tiles of this row tile, its products with V and K tiles before this piece, pieces
+        uint32_t sc = 0, kt = 0, pieces = 0;       // tiles of this row tile, K tiles before this piece, pieces
         // a negative scale goes to the signs of q: m follows the largest score
         const float scale2 = fmaxf(fabsf(a.scale2), 1e-37f);      // (not 0: a hidden score stays -infinity)
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
@@ -355,9 +356,8 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                         l *= f;
                         m = mn;
                         if (j > g.j0) {
-                            // O holds the tiles before this one.  (S(j) being there says that PV(j - 2) is over: of the two phases
-                            // that a parity tells apart, the one awaited is the latest that can be open.)
-                            if (!(ok = mbar_wait(bar(bars.o_done[i]), (oc + (j - g.j0) - 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
+                            // O holds the tiles before this one
+                            if (!(ok = mbar_wait(bar(bars.o_done[i][x ^ 1]), ((sc - 1) >> 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
                             __syncwarp();
                             tc_fence_after();
 #pragma unroll 1
@@ -396,7 +396,6 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 }
                 if (!ok) break;
                 // ---- the piece's result
-                oc += (uint32_t)(g.j1 - g.j0);
                 if (!(ok = mbar_wait(bar(bars.o_last[i]), pieces++ & 1, &abort_flag, &g_prefill_status, 0x700 + i, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
                 __syncwarp();
                 tc_fence_after();
@@ -535,10 +534,11 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_ISSUE));
-        if (warp < 16 + NQ && lane == 0) {
-            // ------------------------------------------------------------ products of row tile i
-            const int i = warp - 16;
-            uint32_t kq = 0, vq = 0, sq = 0, pq = 0, qn = 0;       // K and V tiles passed, S issued, P awaited, Q awaited
+        const int i = (warp - 16) >> 1;
+        if (i < NQ && lane == 0) {
+            // ------------------------------------------------------------ products of row tile i: S (even warps) or P V (odd)
+            const bool do_s = (warp & 1) == 0;
+            uint32_t kv = 0, n_mine = 0, qn = 0;       // tiles passed, products of this issuer, pieces
             bool ok = true;
             auto wait = [&](uint64_t &b, uint32_t ph, int where) { ok = ok && mbar_wait(bar(b), ph, &abort_flag, &g_prefill_status, where); };
             const uint32_t qa = q_s + i * C::Q_BYTES;
@@ -547,47 +547,41 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 const int n = g.j1 - g.j0;
                 // a tile without rows only passes the stages on
                 const bool active = i * 128 < min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G);
-                auto next_s = [&]() {
-                    const uint32_t st = kq % ST;
-                    wait(bars.k_full[st], (kq / ST) & 1, 0x210);
-                    kq++;
-                    if (!ok) return;
-                    if (!active) { mbar_arrive(bar(bars.k_empty[st])); return; }
-                    tc_fence_after();
-                    const uint32_t kb = k_s + st * C::T_BYTES, d = tmem + (2 * i + (sq & 1)) * C::TM_S;
-#pragma unroll
-                    for (int kk = 0; kk < DH / 16; kk++)
-                        pf_mma_ss(d, desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32), desc_sw128(kb + (kk >> 2) * (KT * 128) + (kk & 3) * 32), ID_QK, kk ? 1u : 0u);
-                    tc_commit(bar(bars.s_full[i][sq & 1]));
-                    tc_commit(bar(bars.k_empty[st]));
-                    sq++;
-                };
-                if (n > 0) {
-                    if (active) wait(bars.q_full[i], qn++ & 1, 0x100);
-                    if (ok) next_s();
-                    if (n > 1 && ok) next_s();
-                    for (int j = 0; j < n && ok; j++) {
-                        const uint32_t st = vq % ST;
-                        wait(bars.v_full[st], (vq / ST) & 1, 0x200);
-                        vq++;
-                        if (!ok) break;
-                        if (active) {
-                            wait(bars.p_full[i][pq & 1], (pq >> 1) & 1, 0x300);
-                            if (!ok) break;
-                            tc_fence_after();
-                            const uint32_t vb = v_s + st * C::T_BYTES, pa = tmem + (2 * i + (pq & 1)) * C::TM_S;
-#pragma unroll
-                            for (int kk = 0; kk < KT / 16; kk++)
-                                pf_mma_ts(tmem + C::TM_O0 + i * DH, pa + kk * 8, desc_n_major(vb + kk * 2048, KT * 128), ID_PV, (j > 0 || kk) ? 1u : 0u);
-                            tc_commit(bar(bars.v_empty[st]));
-                            tc_commit(bar(bars.o_done[i]));
-                            if (j == n - 1) tc_commit(bar(bars.o_last[i]));
-                            pq++;
-                        } else {
-                            mbar_arrive(bar(bars.v_empty[st]));
-                        }
-                        if (j + 2 < n) next_s();
+                if (n > 0 && active && do_s) wait(bars.q_full[i], qn++ & 1, 0x100);
+                for (int j = 0; j < n && ok; j++, kv++) {
+                    const uint32_t st = kv % ST, x = n_mine & 1;
+                    uint64_t &full = do_s ? bars.k_full[st] : bars.v_full[st], &empty = do_s ? bars.k_empty[st] : bars.v_empty[st];
+                    wait(full, (kv / ST) & 1, do_s ? 0x210 : 0x200);
+                    if (!ok) break;
+                    if (!active) {
+                        mbar_arrive(bar(empty));
+                        continue;
                     }
+                    const uint32_t s_col = tmem + (2 * i + x) * C::TM_S;
+                    if (do_s) {
+                        // the place was P's of two tiles ago
+                        if (n_mine >= 2) wait(bars.o_done[i][x], ((n_mine >> 1) & 1) ^ 1, 0x220);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t kb = k_s + st * C::T_BYTES;
+#pragma unroll
+                        for (int kk = 0; kk < DH / 16; kk++)
+                            pf_mma_ss(s_col, desc_sw128(qa + (kk >> 2) * 16384 + (kk & 3) * 32), desc_sw128(kb + (kk >> 2) * (KT * 128) + (kk & 3) * 32), ID_QK, kk ? 1u : 0u);
+                        tc_commit(bar(bars.s_full[i][x]));
+                        tc_commit(bar(empty));
+                    } else {
+                        wait(bars.p_full[i][x], (n_mine >> 1) & 1, 0x300);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t vb = v_s + st * C::T_BYTES;
+#pragma unroll
+                        for (int kk = 0; kk < KT / 16; kk++)
+                            pf_mma_ts(tmem + C::TM_O0 + i * DH, s_col + kk * 8, desc_n_major(vb + kk * 2048, KT * 128), ID_PV, (j > 0 || kk) ? 1u : 0u);
+                        tc_commit(bar(bars.o_done[i][x]));
+                        tc_commit(bar(empty));
+                        if (j == n - 1) tc_commit(bar(bars.o_last[i]));
+                    }
+                    n_mine++;
                 }
                 if (ok) more = pf_next(a, R, min_rows, g, pos);
             }

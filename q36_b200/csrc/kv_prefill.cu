@@ -295,11 +295,15 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             if (active) {
                 // Q: this thread's row (the MMAs that read the last one are over: its results were awaited)
                 const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (size_t)(pos.s.t0 + tok_i) * a.q_stride + (size_t)hq * DH);
-#pragma unroll 16
-                for (int c = 0; c < DH / 8; c++) {
-                    uint4 v = mine ? src[c] : make_uint4(0, 0, 0, 0);
-                    v.x ^= flip; v.y ^= flip; v.z ^= flip; v.w ^= flip;
-                    *reinterpret_cast<uint4 *>(smem + i * C::Q_BYTES + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = v;
+#pragma unroll
+                for (int c0 = 0; c0 < DH / 8; c0 += 8) {
+                    uint4 v[8];       // (all on their way before the first is stored)
+#pragma unroll
+                    for (int c = 0; c < 8; c++) v[c] = mine ? __ldg(src + c0 + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                    for (int c = 0; c < 8; c++)
+                        *reinterpret_cast<uint4 *>(smem + i * C::Q_BYTES + (c0 >> 3) * 16384 + row * 128 + ((c ^ (row & 7)) << 4)) =
+                            make_uint4(v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -404,25 +408,26 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (active) {
 #pragma unroll 1
-                for (int c = 0; c < DH; c += 16) {
-                    uint32_t v[16];
-                    tc_ld16(tmem + lanes + C::TM_O0 + i * DH + c, v);
+                for (int c = 0; c < DH; c += 32) {
+                    uint32_t v[32];
+                    tc_ld32(tmem + lanes + C::TM_O0 + i * DH + c, v);
                     tc_ld_wait();
-                    float4 o[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        o[e] = make_float4(__uint_as_float(v[4 * e]) * inv, __uint_as_float(v[4 * e + 1]) * inv, __uint_as_float(v[4 * e + 2]) * inv,
-                                           __uint_as_float(v[4 * e + 3]) * inv);
                     if (!mine) continue;
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * inv);
                     if (g.whole) {
-                        __nv_bfloat16 *d = reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)(pos.s.t0 + tok_i) * a.o_stride + (size_t)hq * DH + c;
+                        uint4 *d = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)(pos.s.t0 + tok_i) * a.o_stride + (size_t)hq * DH + c);
 #pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            reinterpret_cast<uint4 *>(d)[e] = make_uint4(pack_bf16(o[2 * e].x, o[2 * e].y), pack_bf16(o[2 * e].z, o[2 * e].w),
-                                                                         pack_bf16(o[2 * e + 1].x, o[2 * e + 1].y), pack_bf16(o[2 * e + 1].z, o[2 * e + 1].w));
+                        for (int e = 0; e < 4; e++) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int x = 0; x < 4; x++) w[x] = pack_bf16(__uint_as_float(v[8 * e + 2 * x]), __uint_as_float(v[8 * e + 2 * x + 1]));
+                            d[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     } else {
+                        uint4 *d = reinterpret_cast<uint4 *>(dst + 2 * R + r_tile * DH + c);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) *reinterpret_cast<float4 *>(dst + 2 * R + r_tile * DH + c + 4 * e) = o[e];
+                        for (int e = 0; e < 8; e++) d[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     }
                 }
                 tc_fence_before();
@@ -461,26 +466,26 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 const int t = j * KT + tl, col = t >> a.kv.log_bs;
                 return j < g.j1 && t < pos.s.len && col < a.max_blocks ? __ldg(row + col) : -1;
             };
-            uint32_t raw_w[BPT == 1 ? 8 : 4 * BPT] = {}, scale = 0;
-            bool has = false;
-            auto fetch = [&](int j, int id) {
-                has = id >= 0 && id < a.kv.n_blocks;
-                if (!has) return;
+            constexpr int RAW = BPT == 1 ? 8 : 4 * BPT;
+            struct Half { uint32_t w[RAW], scale; bool has; };
+            auto fetch = [&](int j, int id, Half &f) {
+                f.has = id >= 0 && id < a.kv.n_blocks;
+                if (!f.has) return;
                 const int t = (j * KT + tl) & (a.kv.bs - 1);
                 const uint8_t *reg = a.kv.at(id, pos.hk);
-                scale = ld_part<BPT>(reg + a.kv.bs * DH + (is_v ? a.kv.bs * NB : 0) + t * NB + half * BPT);
+                f.scale = ld_part<BPT>(reg + a.kv.bs * DH + (is_v ? a.kv.bs * NB : 0) + t * NB + half * BPT);
                 if (!is_v) {
                     const uint8_t *src = reg + kv_k_off(t, 0, half * BPT, DH);
 #pragma unroll
                     for (int q = 0; q < 4; q++) {       // word q of every block
                         if constexpr (BPT == 4) {
                             const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src + q * (DH / 8)));
-                            raw_w[4 * q] = u.x; raw_w[4 * q + 1] = u.y; raw_w[4 * q + 2] = u.z; raw_w[4 * q + 3] = u.w;
+                            f.w[4 * q] = u.x; f.w[4 * q + 1] = u.y; f.w[4 * q + 2] = u.z; f.w[4 * q + 3] = u.w;
                         } else if constexpr (BPT == 2) {
                             const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
-                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                            f.w[2 * q] = u.x; f.w[2 * q + 1] = u.y;
                         } else {
-                            raw_w[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
+                            f.w[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
                         }
                     }
                 } else {
@@ -489,43 +494,46 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                     for (int q = 0; q < 8; q++) {       // four dims of every block
                         if constexpr (BPT == 4) {
                             const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
-                            raw_w[2 * q] = u.x; raw_w[2 * q + 1] = u.y;
+                            f.w[2 * q] = u.x; f.w[2 * q + 1] = u.y;
                         } else {
-                            raw_w[q] = ld_part<2 * BPT>(src + q * (DH / 8));
+                            f.w[q] = ld_part<2 * BPT>(src + q * (DH / 8));
                         }
                     }
                 }
             };
-            int id_next = page(g.j0 + 1);
-            fetch(g.j0, page(g.j0));
+            // data two tiles ahead, page ids three
+            Half cur = {}, nxt = {}, far = {};
+            int id_next = page(g.j0 + 2);
+            fetch(g.j0, page(g.j0), cur);
+            fetch(g.j0 + 1, page(g.j0 + 1), nxt);
             for (int j = g.j0; j < g.j1; j++, kc++) {
                 const uint32_t st = kc % ST, ph = (kc / ST) & 1;
+                const int id = id_next;
+                id_next = page(j + 3);
+                fetch(j + 2, id, far);
                 if (!(ok = mbar_wait(bar(is_v ? bars.v_empty[st] : bars.k_empty[st]), ph ^ 1, &abort_flag, &g_prefill_status, 0x800 + st, TC_SPIN_LIMIT, TC_BACKOFF_NS))) break;
                 __syncwarp();
                 uint8_t *dst = smem + NQ * C::Q_BYTES + ((is_v ? ST : 0) + st) * C::T_BYTES + tl * 128;
 #pragma unroll
                 for (int b = 0; b < BPT; b++) {
-                    const Lut t = make_lut((scale >> (8 * b)) & 0xff, has);
+                    const Lut t = make_lut((cur.scale >> (8 * b)) & 0xff, cur.has);
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         uint32_t w;
-                        if (!is_v) w = raw_w[BPT * q + b];
-                        else if constexpr (BPT == 1) w = raw_w[2 * q] | raw_w[2 * q + 1] << 16;
-                        else w = __byte_perm(raw_w[(BPT / 2) * (2 * q) + b / 2], raw_w[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
+                        if (!is_v) w = cur.w[BPT * q + b];
+                        else if constexpr (BPT == 1) w = cur.w[2 * q] | cur.w[2 * q + 1] << 16;
+                        else w = __byte_perm(cur.w[(BPT / 2) * (2 * q) + b / 2], cur.w[(BPT / 2) * (2 * q + 1) + b / 2], (b & 1) ? 0x7632 : 0x5410);
                         const int c = (half * BPT + b) * 4 + q;      // 16-byte chunk of the token's row: dims 8 c ..
                         *reinterpret_cast<uint4 *>(dst + (c >> 3) * (KT * 128) + (((c & 7) ^ (tl & 7)) << 4)) = widen8(t, w);
                     }
                 }
                 if (!is_v && half == 0) {
                     // tokens of the request whose page is bad
-                    const uint32_t bad = __ballot_sync(0xffffffffu, !has && j * KT + tl < pos.s.len);
+                    const uint32_t bad = __ballot_sync(0xffffffffu, !cur.has && j * KT + tl < pos.s.len);
                     if (lane == 0) bad_s[kc & 7][tl >> 5] = bad;
                 }
-                const int id = id_next;
-                if (j + 1 < g.j1) {
-                    id_next = page(j + 2);
-                    fetch(j + 1, id);
-                }
+                cur = nxt;
+                nxt = far;
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(is_v ? bars.v_full[st] : bars.k_full[st]));

@@ -286,24 +286,37 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         // a negative scale goes to the signs of q: m follows the largest score
         const float scale2 = fmaxf(fabsf(a.scale2), 1e-37f);      // (not 0: a hidden score stays -infinity)
         const uint32_t flip = a.scale2 < 0.f ? 0x80008000u : 0u;
+        // rows of Q, and of results on their way out, in shared memory: 16-byte chunks swizzled as the MMA reads them.  A warp moves 32 rows,
+        // RPI of them at a time with CPR lanes on each.
+        constexpr int CPR = DH / 8, RPI = 32 / CPR;
+        auto chunk = [&](int rr, int c) { return smem + i * C::Q_BYTES + (c >> 3) * 16384 + ((warp & 3) * 32 + rr) * 128 + ((c ^ (rr & 7)) & 7) * 16; };
         bool first = true, ok = true;
         while (more && ok && i < NQ) {
             const PfSeg g = pf_segment(a, KT, pos);
             const int r_tile = i * 128 + row, rows = min(pos.s.c * a.G, pos.s.n * a.G - pos.rt * pos.s.c * a.G), r = pos.rt * pos.s.c * a.G + r_tile;
             const bool mine = r_tile < rows, active = i * 128 < rows && g.j0 < g.j1;
             const int tok_i = mine ? r / a.G : 0, hq = pos.hk * a.G + (mine ? r - tok_i * a.G : 0);
+            const long long q_off = mine ? (long long)(pos.s.t0 + tok_i) * a.q_stride + (long long)hq * DH : -1;
+            const long long q_first = (long long)pos.s.t0 * a.q_stride + (long long)pos.hk * a.G * DH;
             if (active) {
-                // Q: this thread's row (the MMAs that read the last one are over: its results were awaited)
-                const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(a.q) + (size_t)(pos.s.t0 + tok_i) * a.q_stride + (size_t)hq * DH);
+                // Q: this warp's 32 rows, neighbouring lanes on neighbouring 16 bytes (the MMAs that read the last rows are over:
+                // their results were awaited)
+                const uint16_t *q = reinterpret_cast<const uint16_t *>(a.q) + (lane % CPR) * 8;
 #pragma unroll
-                for (int c0 = 0; c0 < DH / 8; c0 += 8) {
-                    uint4 v[8];       // (all on their way before the first is stored)
+                for (int k0 = 0; k0 < CPR; k0 += 8) {
+                    // (all on their way before the first is stored; a row that is not there reads the tile's first)
+                    long long off[8];
+                    uint4 v[8];
 #pragma unroll
-                    for (int c = 0; c < 8; c++) v[c] = mine ? __ldg(src + c0 + c) : make_uint4(0, 0, 0, 0);
+                    for (int k = 0; k < 8; k++) off[k] = __shfl_sync(0xffffffffu, q_off, (k0 + k) * RPI + lane / CPR);
 #pragma unroll
-                    for (int c = 0; c < 8; c++)
-                        *reinterpret_cast<uint4 *>(smem + i * C::Q_BYTES + (c0 >> 3) * 16384 + row * 128 + ((c ^ (row & 7)) << 4)) =
-                            make_uint4(v[c].x ^ flip, v[c].y ^ flip, v[c].z ^ flip, v[c].w ^ flip);
+                    for (int k = 0; k < 8; k++) v[k] = __ldg(reinterpret_cast<const uint4 *>(q + (off[k] < 0 ? q_first : off[k])));
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const uint32_t keep = off[k] < 0 ? 0u : ~0u;
+                        *reinterpret_cast<uint4 *>(chunk((k0 + k) * RPI + lane / CPR, lane % CPR)) =
+                            make_uint4((v[k].x ^ flip) & keep, (v[k].y ^ flip) & keep, (v[k].z ^ flip) & keep, (v[k].w ^ flip) & keep);
+                    }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
@@ -407,28 +420,40 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             float *dst = part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * attn_part_floats(R, DH);
             const float inv = l == 0.f ? 0.f : 1.f / l;
             if (active) {
+                // through Q's place, so that a row leaves as a whole: bf16 at once, f32 in halves
+                const int n_pass = g.whole ? 1 : 2, dims = DH / n_pass;
+                for (int pass = 0; pass < n_pass; pass++) {
 #pragma unroll 1
-                for (int c = 0; c < DH; c += 32) {
-                    uint32_t v[32];
-                    tc_ld32(tmem + lanes + C::TM_O0 + i * DH + c, v);
-                    tc_ld_wait();
-                    if (!mine) continue;
+                    for (int c = 0; c < dims; c += 32) {
+                        uint32_t v[32];
+                        tc_ld32(tmem + lanes + C::TM_O0 + i * DH + pass * dims + c, v);
+                        tc_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * inv);
-                    if (g.whole) {
-                        uint4 *d = reinterpret_cast<uint4 *>(reinterpret_cast<__nv_bfloat16 *>(a.out) + (size_t)(pos.s.t0 + tok_i) * a.o_stride + (size_t)hq * DH + c);
+                        for (int e = 0; e < 32; e++) v[e] = __float_as_uint(__uint_as_float(v[e]) * inv);
+                        if (g.whole) {
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            uint32_t w[4];
+                            for (int e = 0; e < 4; e++) {
+                                uint32_t w[4];
 #pragma unroll
-                            for (int x = 0; x < 4; x++) w[x] = pack_bf16(__uint_as_float(v[8 * e + 2 * x]), __uint_as_float(v[8 * e + 2 * x + 1]));
-                            d[e] = make_uint4(w[0], w[1], w[2], w[3]);
+                                for (int x = 0; x < 4; x++) w[x] = pack_bf16(__uint_as_float(v[8 * e + 2 * x]), __uint_as_float(v[8 * e + 2 * x + 1]));
+                                *reinterpret_cast<uint4 *>(chunk(lane, c / 8 + e)) = make_uint4(w[0], w[1], w[2], w[3]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) *reinterpret_cast<uint4 *>(chunk(lane, c / 4 + e)) = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                         }
-                    } else {
-                        uint4 *d = reinterpret_cast<uint4 *>(dst + 2 * R + r_tile * DH + c);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) d[e] = make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     }
+                    __syncwarp();
+#pragma unroll 4
+                    for (int k = 0; k < CPR; k++) {
+                        const int rr = k * RPI + lane / CPR, c = lane % CPR;
+                        const long long off = __shfl_sync(0xffffffffu, mine ? (long long)(pos.s.t0 + tok_i) * a.o_stride + (long long)hq * DH : -1ll, rr);
+                        const uint4 v = *reinterpret_cast<const uint4 *>(chunk(rr, c));
+                        if (off < 0) continue;
+                        if (g.whole) *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(a.out) + off + c * 8) = v;
+                        else *reinterpret_cast<uint4 *>(dst + 2 * R + (size_t)(i * 128 + (warp & 3) * 32 + rr) * DH + pass * dims + c * 4) = v;
+                    }
+                    __syncwarp();
                 }
                 tc_fence_before();
             }

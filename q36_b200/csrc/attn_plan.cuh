@@ -5,8 +5,14 @@
 
 namespace q36 {
 
-// rows: rows of a tile; unit: tokens of a unit; a request takes part when it has max_rows rows at most.
-struct SpanRule { int rows, unit, max_rows; };
+// rows: rows of a tile; unit: tokens of a unit; all: every request takes part, not only those that is_long leaves.
+struct SpanRule { int rows, unit, all; };
+
+// Which requests go to the tile kernel (bf16, when the host says that there may be any).  It does 128 or 256 rows at ten times the
+// rate of the other one, but a piece of work costs it 10 us to begin and end.  us of the few-row kernel / of this one, 16 heads of
+// 128 on 2: 16 new tokens (128 rows) CROSS
+constexpr int LONG_ROWS = 65, LONG_WORK = 1 << 20;
+__device__ __forceinline__ bool is_long(int rows, int len) { return rows >= LONG_ROWS && (long long)rows * len >= LONG_WORK; }
 
 struct SeqSpans { int t0, n, len, tiles, u_lo, u_hi; };   // units [u_lo, u_hi) of the cached tokens that any row sees
 
@@ -14,7 +20,7 @@ __device__ __forceinline__ SeqSpans seq_spans(const AttnArgs &a, const SpanRule 
     SeqSpans s;
     seq_span(a, b, s.t0, s.n, s.len);
     const int rows = s.n * a.G;
-    s.tiles = rows > 0 && rows <= r.max_rows ? (rows + r.rows - 1) / r.rows : 0;
+    s.tiles = rows > 0 && (r.all || !is_long(rows, s.len)) ? (rows + r.rows - 1) / r.rows : 0;
     const int lo = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
     s.u_lo = lo / r.unit;
     s.u_hi = max((s.len + r.unit - 1) / r.unit, s.u_lo + 1);     // (at least one: rows that see nothing are written too)
@@ -146,9 +152,9 @@ __device__ __forceinline__ void attn_store_lse(const AttnArgs &a, int t0, int n,
 }
 
 constexpr int DEC_MAX_OCC = 4;
-int launch_decode(const AttnArgs &a, int rows, int max_rows, void *ws, cudaStream_t st);
+int launch_decode(const AttnArgs &a, int rows, int all, void *ws, cudaStream_t st);
 uint64_t decode_ws_bytes(int Dh, int rows);
-int launch_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t st);
+int launch_prefill(const AttnArgs &a, void *ws, cudaStream_t st);
 uint64_t prefill_ws_bytes(int Dh);
 int prefill_wait_status(int *out, cudaStream_t st);
 int linear_wait_status(int *out, cudaStream_t st);

@@ -7,74 +7,123 @@ namespace q36 {
 
 constexpr int JOIN_THREADS = 128;
 
-// Block (i, y): rows y * per .. of the span whose first piece CTA i had, if it had one of a cut span.  Piece p counts
-// l_p 2^(m_p - m); a piece that saw nothing has no row to read.
+// The join.  Row r of the span whose first piece CTA i had, if it had one of a cut span: piece p counts l_p 2^(m_p - m); a piece that
+// saw nothing has no row to read.
+__device__ __forceinline__ const float *join_slot(const float *part, const AttnPart &d, int cta, int p, int stride) {
+    return part + (size_t)(p == 0 ? d.slot : 2 * (cta + p)) * stride;
+}
+
+// Spans in up to hundreds of pieces (few rows): block (i, r), the pieces over its threads.
 template <int DH>
 __global__ void __launch_bounds__(JOIN_THREADS)
-k_attn_join(AttnArgs a, int tile_rows, int per, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
+k_attn_join(AttnArgs a, int tile_rows, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
     Q36_GDS();
     constexpr int C4 = DH / 4, LANES = JOIN_THREADS / C4;      // threads over the dims, and pieces in parallel
     extern __shared__ float w[];                               // one weight per piece
-    __shared__ float red[JOIN_THREADS / 32];
+    __shared__ float red[2][JOIN_THREADS / 32];
     __shared__ float4 acc[LANES][C4];
     const AttnPart d = desc[blockIdx.x];
-    const int tid = threadIdx.x, r0 = blockIdx.y * per;
-    if (d.parts == 0) return;
+    const int r = blockIdx.y, tid = threadIdx.x, cta = blockIdx.x;
+    if (d.parts == 0 || r >= d.rows) return;
     const int stride = attn_part_floats(tile_rows, DH);
-    auto slot = [&](int p) { return part + (size_t)(p == 0 ? d.slot : 2 * ((int)blockIdx.x + p)) * stride; };
-    for (int r = r0; r < min(r0 + per, d.rows); r++) {
-        float m = -3.0e38f;
-        for (int p = tid; p < d.parts; p += JOIN_THREADS) m = fmaxf(m, slot(p)[2 * r]);
-        m = warp_max(m);
-        __syncthreads();
-        if ((tid & 31) == 0) red[tid >> 5] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-        __syncthreads();
-        float l = 0.f;
-        for (int p = tid; p < d.parts; p += JOIN_THREADS) {
-            const float *s = slot(p);
-            l += w[p] = s[2 * r + 1] * exp2f(s[2 * r] - m);
-        }
-        l = warp_sum(l);
-        if ((tid & 31) == 0) red[tid >> 5] = l;
-        __syncthreads();
-        l = red[0] + red[1] + red[2] + red[3];
-        const int c = tid % C4, lane = tid / C4;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float m = -3.0e38f;
+    for (int p = tid; p < d.parts; p += JOIN_THREADS) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
+    m = warp_max(m);
+    if ((tid & 31) == 0) red[0][tid >> 5] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float l = 0.f;
+    for (int p = tid; p < d.parts; p += JOIN_THREADS) {
+        const float *s = join_slot(part, d, cta, p, stride);
+        l += w[p] = s[2 * r + 1] * exp2f(s[2 * r] - m);
+    }
+    l = warp_sum(l);
+    if ((tid & 31) == 0) red[1][tid >> 5] = l;
+    __syncthreads();
+    l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+    const int c = tid % C4, lane = tid / C4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-        for (int p = lane; p < d.parts; p += LANES) {
-            const float f = w[p];
-            if (f == 0.f) continue;
-            const float4 v = *reinterpret_cast<const float4 *>(slot(p) + 2 * tile_rows + r * DH + 4 * c);
-            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-        }
-        acc[lane][c] = o;
-        __syncthreads();
-        if (lane == 0) {
+    for (int p = lane; p < d.parts; p += LANES) {
+        const float f = w[p];
+        if (f == 0.f) continue;
+        const float4 v = *reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * tile_rows + r * DH + 4 * c);
+        o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+    }
+    acc[lane][c] = o;
+    __syncthreads();
+    if (lane == 0) {
 #pragma unroll
-            for (int i = 1; i < LANES; i++) { const float4 v = acc[i][c]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
-            const float f = l == 0.f ? 0.f : 1.f / l;
-            attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-            if (c == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
-        }
+        for (int i = 1; i < LANES; i++) { const float4 v = acc[i][c]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+        if (c == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
     }
 }
 
+// Many rows, few pieces: a warp per row.
+template <int DH>
+__global__ void __launch_bounds__(JOIN_THREADS)
+k_attn_join_rows(AttnArgs a, int tile_rows, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
+    Q36_GDS();
+    constexpr int N4 = (DH + 127) / 128;      // 16-byte pieces of a row per lane
+    const AttnPart d = desc[blockIdx.x];
+    const int r = blockIdx.y * (JOIN_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, cta = blockIdx.x;
+    if (d.parts == 0 || r >= d.rows) return;
+    const int stride = attn_part_floats(tile_rows, DH);
+    float m = -3.0e38f;
+    for (int p = lane; p < d.parts; p += 32) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
+    m = warp_max(m);
+    float l = 0.f;
+    float4 o[N4];
+#pragma unroll
+    for (int k = 0; k < N4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < d.parts; p0 += 32) {
+        float mine = 0.f;
+        if (p0 + lane < d.parts) {
+            const float *s = join_slot(part, d, cta, p0 + lane, stride);
+            mine = s[2 * r + 1] * exp2f(s[2 * r] - m);
+        }
+        l += warp_sum(mine);
+#pragma unroll 4
+        for (int p = 0; p < min(32, d.parts - p0); p++) {
+            const float f = __shfl_sync(0xffffffffu, mine, p);
+            if (f == 0.f) continue;
+            const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p0 + p, stride) + 2 * tile_rows + r * DH);
+#pragma unroll
+            for (int k = 0; k < N4; k++) {
+                if (DH < 128 && lane >= DH / 4) continue;
+                const float4 v = s[32 * k + lane];
+                o[k].x = fmaf(f, v.x, o[k].x); o[k].y = fmaf(f, v.y, o[k].y); o[k].z = fmaf(f, v.z, o[k].z); o[k].w = fmaf(f, v.w, o[k].w);
+            }
+        }
+    }
+    const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int k = 0; k < N4; k++) {
+        if (DH < 128 && lane >= DH / 4) continue;
+        attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), make_float4(o[k].x * f, o[k].y * f, o[k].z * f, o[k].w * f));
+    }
+    if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+}
+
 int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st) {
-    // a row per block where a span may be in hundreds of pieces, several where it is in two or three
-    const int per = tile_rows > 16 ? 8 : 1;
-    const dim3 blocks(grid, tile_rows / per), threads(JOIN_THREADS);
-    if (a.kv.Dh == 64) launch_k(k_attn_join<64>, blocks, threads, grid * 4, st, a, tile_rows, per, desc, part);
-    else if (a.kv.Dh == 128) launch_k(k_attn_join<128>, blocks, threads, grid * 4, st, a, tile_rows, per, desc, part);
-    else launch_k(k_attn_join<256>, blocks, threads, grid * 4, st, a, tile_rows, per, desc, part);
+    const dim3 threads(JOIN_THREADS);
+    if (tile_rows > 16) {
+        const dim3 blocks(grid, tile_rows / (JOIN_THREADS / 32));
+        if (a.kv.Dh == 64) launch_k(k_attn_join_rows<64>, blocks, threads, 0, st, a, tile_rows, desc, part);
+        else if (a.kv.Dh == 128) launch_k(k_attn_join_rows<128>, blocks, threads, 0, st, a, tile_rows, desc, part);
+        else launch_k(k_attn_join_rows<256>, blocks, threads, 0, st, a, tile_rows, desc, part);
+        return check_launch();
+    }
+    const dim3 blocks(grid, tile_rows);
+    if (a.kv.Dh == 64) launch_k(k_attn_join<64>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
+    else if (a.kv.Dh == 128) launch_k(k_attn_join<128>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
+    else launch_k(k_attn_join<256>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
     return check_launch();
 }
 
 static int rows_of(int Hq, int Hkv, int max_q) { return (int)min((long)(Hq / Hkv) * max_q, (long)INT32_MAX); }
-
-// From this many rows per kv head on a bf16 request goes to the tile kernel.
-constexpr int LONG_ROWS = 65;
 
 uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) {
     const int rows = rows_of(Hq, Hkv, max_q);
@@ -85,10 +134,10 @@ uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) {
 int launch_attention(const AttnArgs &a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st) {
     (void)ws_bytes;
     const int rows = rows_of(a.Hq, a.kv.Hkv, max_q);
-    if (!a.q_bf16 || rows < LONG_ROWS) return launch_decode(a, rows, INT32_MAX, ws, st);
+    if (!a.q_bf16 || rows < LONG_ROWS) return launch_decode(a, rows, 1, ws, st);
     int rc;
-    if ((rc = launch_decode(a, rows, LONG_ROWS - 1, ws, st))) return rc;
-    return launch_prefill(a, LONG_ROWS, ws, st);
+    if ((rc = launch_decode(a, rows, 0, ws, st))) return rc;
+    return launch_prefill(a, ws, st);
 }
 
 }  // namespace q36

@@ -132,14 +132,14 @@ struct DecSmem {
 
 template <int DH, int NT, bool F32>
 __global__ void __launch_bounds__(DEC_THREADS)
-k_attn_decode(AttnArgs a, int max_rows, AttnPart *__restrict__ desc, float *__restrict__ part) {
+k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restrict__ part) {
     constexpr int NB = DH / 32, R = 8 * NT, TERMS = F32 ? 2 : 1;
     using Frag = DecFrag<DH>;
     Q36_GDS();
     extern __shared__ __align__(16) uint8_t smem_raw[];
     DecSmem<DH, NT> &sm = *reinterpret_cast<DecSmem<DH, NT> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
-    const SpanRule rule{R, DEC_UNIT, max_rows};
+    const SpanRule rule{R, DEC_UNIT, all};
     PlanPos pos;
     if (!plan_start<DEC_THREADS>(a, rule, DEC_WARPS, sm.plan, pos)) {
         if (tid == 0) desc[blockIdx.x].parts = 0;
@@ -482,7 +482,7 @@ k_attn_decode(AttnArgs a, int max_rows, AttnPart *__restrict__ desc, float *__re
 }
 
 template <int DH, int NT, bool F32>
-static int run(const AttnArgs &a, int max_rows, void *ws, cudaStream_t st) {
+static int run(const AttnArgs &a, int all, void *ws, cudaStream_t st) {
     static bool attr_done[MAX_DEVICES] = {false};
     static int occ[MAX_DEVICES] = {0};
     const int smem = sizeof(DecSmem<DH, NT>), dev = current_device();
@@ -497,7 +497,7 @@ static int run(const AttnArgs &a, int max_rows, void *ws, cudaStream_t st) {
     const int grid = sm_count() * occ[dev];
     AttnPart *desc = (AttnPart *)ws;
     float *part = (float *)((uint8_t *)ws + attn_desc_bytes(grid));
-    launch_k(k_attn_decode<DH, NT, F32>, dim3(grid), dim3(DEC_THREADS), smem, st, a, max_rows, desc, part);
+    launch_k(k_attn_decode<DH, NT, F32>, dim3(grid), dim3(DEC_THREADS), smem, st, a, all, desc, part);
     if ((rc = check_launch())) return rc;
     return launch_attn_join(a, 8 * NT, grid, desc, part, st);
 }
@@ -511,18 +511,18 @@ uint64_t decode_ws_bytes(int Dh, int rows) {
     return attn_desc_bytes(grid) + 2ull * grid * attn_part_floats(8 * decode_nt(Dh, rows), Dh) * 4;
 }
 
-int launch_decode(const AttnArgs &a, int rows, int max_rows, void *ws, cudaStream_t st) {
+int launch_decode(const AttnArgs &a, int rows, int all, void *ws, cudaStream_t st) {
     const bool f32 = !a.q_bf16;
     const int nt = decode_nt(a.kv.Dh, rows);
     if (a.kv.Dh == 64) {
-        if (nt == 1) return f32 ? run<64, 1, true>(a, max_rows, ws, st) : run<64, 1, false>(a, max_rows, ws, st);
-        return f32 ? run<64, 2, true>(a, max_rows, ws, st) : run<64, 2, false>(a, max_rows, ws, st);
+        if (nt == 1) return f32 ? run<64, 1, true>(a, all, ws, st) : run<64, 1, false>(a, all, ws, st);
+        return f32 ? run<64, 2, true>(a, all, ws, st) : run<64, 2, false>(a, all, ws, st);
     }
     if (a.kv.Dh == 128) {
-        if (nt == 1) return f32 ? run<128, 1, true>(a, max_rows, ws, st) : run<128, 1, false>(a, max_rows, ws, st);
-        return f32 ? run<128, 2, true>(a, max_rows, ws, st) : run<128, 2, false>(a, max_rows, ws, st);
+        if (nt == 1) return f32 ? run<128, 1, true>(a, all, ws, st) : run<128, 1, false>(a, all, ws, st);
+        return f32 ? run<128, 2, true>(a, all, ws, st) : run<128, 2, false>(a, all, ws, st);
     }
-    return f32 ? run<256, 1, true>(a, max_rows, ws, st) : run<256, 1, false>(a, max_rows, ws, st);
+    return f32 ? run<256, 1, true>(a, all, ws, st) : run<256, 1, false>(a, all, ws, st);
 }
 
 }  // namespace q36

@@ -36,15 +36,15 @@ struct PfCfg {
 };
 constexpr float PF_NONE = -1.0e30f;      // "no token yet": finite, so that differences stay defined
 constexpr float PF_GROW = 8.f;
-#ifndef XSPAN
-#define XSPAN 192
-#endif
-constexpr int PF_SPAN = XSPAN;
+// What a span costs beside its tokens (Q in, results out, the pipeline's start), in tokens.  Prompt of 8192, 2 x 256 spans: us at 1
+// 577, 192 450, 384 373, 512 374, 768 379.
+constexpr int PF_SPAN = 448;
+constexpr int PF_MIN = 1024;        // the smallest range of a CTA
 __device__ int g_prefill_status;         // where a wait gave up (0: nowhere)
 
 // ---------------------------------------------------------------- plan
 // Span rt of a request: tokens c rt .. of the new ones (c whole tokens of G rows); it sees cached tokens [lo, hi).  Its size is
-// hi - lo + 1, which is piecewise linear in rt: prefix sums have a closed form.
+// hi - lo + PF_SPAN, which is piecewise linear in rt: prefix sums have a closed form.
 struct PfSeq { int t0, n, len, c, tiles; };
 __device__ __forceinline__ long long sum_pos(long long a, long long c, long long n) {      // sum over x < n of max(0, a + c x)
     long long x0 = a < 0 ? (-a + c - 1) / c : 0;
@@ -52,11 +52,11 @@ __device__ __forceinline__ long long sum_pos(long long a, long long c, long long
     const long long k = n - x0, f = a + c * x0;
     return k * f + c * (k * (k - 1) / 2);
 }
-__device__ __forceinline__ PfSeq pf_seq(const AttnArgs &a, int R, int min_rows, int b) {
+__device__ __forceinline__ PfSeq pf_seq(const AttnArgs &a, int R, int b) {
     PfSeq s;
     seq_span(a, b, s.t0, s.n, s.len);
     s.c = R / a.G;
-    s.tiles = s.n * a.G >= min_rows ? (s.n + s.c - 1) / s.c : 0;
+    s.tiles = is_long(s.n * a.G, s.len) ? (s.n + s.c - 1) / s.c : 0;
     return s;
 }
 __device__ __forceinline__ void pf_range(const AttnArgs &a, const PfSeq &s, int rt, int &lo, int &hi) {
@@ -73,10 +73,10 @@ __device__ __forceinline__ long long pf_prefix(const AttnArgs &a, const PfSeq &s
     return u;
 }
 struct PfPos { long long at, end, per, seq_base, span_base; int b, hk, rt; PfSeq s; };
-__device__ __forceinline__ void pf_locate(const AttnArgs &a, int R, int min_rows, PfPos &p) {
+__device__ __forceinline__ void pf_locate(const AttnArgs &a, int R, PfPos &p) {
     long long one;
     for (;;) {
-        p.s = pf_seq(a, R, min_rows, p.b);
+        p.s = pf_seq(a, R, p.b);
         one = pf_prefix(a, p.s, p.s.tiles);
         if (p.at < p.seq_base + one * a.kv.Hkv) break;
         p.seq_base += one * a.kv.Hkv;
@@ -107,7 +107,7 @@ __device__ __forceinline__ PfSeg pf_segment(const AttnArgs &a, int KT, const PfP
     return g;
 }
 // The span behind this one (spans of a request: row tiles of one kv head after the other); false behind the range.
-__device__ __forceinline__ bool pf_next(const AttnArgs &a, int R, int min_rows, const PfSeg &g, PfPos &p) {
+__device__ __forceinline__ bool pf_next(const AttnArgs &a, int R, const PfSeg &g, PfPos &p) {
     p.at = min(p.span_base + g.units, p.end);
     if (p.at >= p.end) return false;
     p.span_base = p.at;
@@ -115,7 +115,7 @@ __device__ __forceinline__ bool pf_next(const AttnArgs &a, int R, int min_rows, 
     p.rt = 0;
     if (++p.hk < a.kv.Hkv) return true;
     p.hk = 0;
-    do p.s = pf_seq(a, R, min_rows, ++p.b); while (p.s.tiles == 0);
+    do p.s = pf_seq(a, R, ++p.b); while (p.s.tiles == 0);
     return true;
 }
 
@@ -202,7 +202,7 @@ __device__ __forceinline__ uint32_t ld_part(const uint8_t *p) {
 
 template <int DH>
 __global__ void __launch_bounds__(PF_THREADS, 1)
-k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__restrict__ part) {
+k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part) {
     using C = PfCfg<DH>;
     constexpr int NQ = C::NQ, R = C::R, KT = C::KT, NB = C::NB, BPT = C::BPT, ST = C::STAGES;
     constexpr uint32_t ID_QK = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(KT >> 3) << 17) | (8u << 24);
@@ -245,7 +245,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         const int per = (a.B + PF_THREADS - 1) / PF_THREADS, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
         long long mine = 0;
         for (int b = b0; b < b1; b++) {
-            const PfSeq s = pf_seq(a, R, min_rows, b);
+            const PfSeq s = pf_seq(a, R, b);
             if (s.tiles) mine += pf_prefix(a, s, s.tiles) * a.kv.Hkv;
         }
         long long inc = mine;
@@ -262,7 +262,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             total += plan_sum[w];
         }
         const long long excl = before + inc - mine;
-        pos.per = max((total + gridDim.x - 1) / gridDim.x, (long long)(2 * KT));
+        pos.per = max((total + gridDim.x - 1) / gridDim.x, (long long)PF_MIN);
         pos.at = min(pos.per * blockIdx.x, total);
         pos.end = min(pos.at + pos.per, total);
         if (pos.at < pos.end && pos.at >= excl && pos.at < excl + mine) { plan_base = excl; plan_b = b0; }
@@ -270,7 +270,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
         if (pos.at < pos.end) {
             pos.seq_base = plan_base;
             pos.b = plan_b;
-            pf_locate(a, R, min_rows, pos);
+            pf_locate(a, R, pos);
         }
     }
     tc_fence_after();
@@ -302,7 +302,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 // Q: this warp's 32 rows, neighbouring lanes on neighbouring 16 bytes (the MMAs that read the last rows are over:
                 // their results were awaited)
                 const uint16_t *q = reinterpret_cast<const uint16_t *>(a.q) + (lane % CPR) * 8;
-#pragma unroll
+#pragma unroll 1
                 for (int k0 = 0; k0 < CPR; k0 += 8) {
                     // (all on their way before the first is stored; a row that is not there reads the tile's first)
                     long long off[8];
@@ -422,6 +422,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             if (active) {
                 // through Q's place, so that a row leaves as a whole: bf16 at once, f32 in halves
                 const int n_pass = g.whole ? 1 : 2, dims = DH / n_pass;
+#pragma unroll 1
                 for (int pass = 0; pass < n_pass; pass++) {
 #pragma unroll 1
                     for (int c = 0; c < dims; c += 32) {
@@ -475,7 +476,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
             }
             first = false;
             kt += max(g.j1 - g.j0, 0);
-            more = pf_next(a, R, min_rows, g, pos);
+            more = pf_next(a, R, g, pos);
         }
     } else if (warp < 16) {
         // ------------------------------------------------------------ widening: half a token of K or V per thread
@@ -563,7 +564,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(is_v ? bars.v_full[st] : bars.k_full[st]));
             }
-            if (ok) more = pf_next(a, R, min_rows, g, pos);
+            if (ok) more = pf_next(a, R, g, pos);
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_ISSUE));
@@ -616,7 +617,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
                     }
                     n_mine++;
                 }
-                if (ok) more = pf_next(a, R, min_rows, g, pos);
+                if (ok) more = pf_next(a, R, g, pos);
             }
         }
     }
@@ -627,7 +628,7 @@ k_attn_prefill(AttnArgs a, int min_rows, AttnPart *__restrict__ desc, float *__r
 }
 
 template <int DH>
-static int run_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t st) {
+static int run_prefill(const AttnArgs &a, void *ws, cudaStream_t st) {
     using C = PfCfg<DH>;
     static bool attr_done[MAX_DEVICES] = {false};
     int rc;
@@ -635,7 +636,7 @@ static int run_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t s
     const int grid = sm_count();
     AttnPart *desc = (AttnPart *)ws;
     float *part = (float *)((uint8_t *)ws + attn_desc_bytes(grid));
-    launch_k(k_attn_prefill<DH>, dim3(grid), dim3(PF_THREADS), C::SMEM, st, a, min_rows, desc, part);
+    launch_k(k_attn_prefill<DH>, dim3(grid), dim3(PF_THREADS), C::SMEM, st, a, desc, part);
     if ((rc = check_launch())) return rc;
     return launch_attn_join(a, C::R, grid, desc, part, st);
 }
@@ -644,9 +645,9 @@ uint64_t prefill_ws_bytes(int Dh) {
     const int grid = sm_count(), rows = Dh == 256 ? 128 : 256;
     return attn_desc_bytes(grid) + 2ull * grid * attn_part_floats(rows, Dh) * 4;
 }
-int launch_prefill(const AttnArgs &a, int min_rows, void *ws, cudaStream_t st) {
-    if (a.kv.Dh == 64) return run_prefill<64>(a, min_rows, ws, st);
-    return a.kv.Dh == 128 ? run_prefill<128>(a, min_rows, ws, st) : run_prefill<256>(a, min_rows, ws, st);
+int launch_prefill(const AttnArgs &a, void *ws, cudaStream_t st) {
+    if (a.kv.Dh == 64) return run_prefill<64>(a, ws, st);
+    return a.kv.Dh == 128 ? run_prefill<128>(a, ws, st) : run_prefill<256>(a, ws, st);
 }
 
 // Where a bounded wait gave up since the process began (0: nowhere).

@@ -13,113 +13,145 @@ __device__ __forceinline__ const float *join_slot(const float *part, const AttnP
     return part + (size_t)(p == 0 ? d.slot : 2 * (cta + p)) * stride;
 }
 
+// Which CTAs had the first piece of a cut span (n of them), into list[].  Every block finds out for itself and takes its share of (span,
+// rows): a block per CTA and row, most of which leave at once, took 7 us at 296 x 16 and 12 at 148 x 64.
+__device__ __forceinline__ int join_list(const AttnPart *desc, int grid, int *list) {
+    __shared__ int cnt[JOIN_THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int n = 0;
+    for (int i0 = 0; i0 < grid; i0 += JOIN_THREADS) {
+        const int i = i0 + threadIdx.x;
+        const bool cut = i < grid && desc[i].parts > 0;
+        const unsigned in = __ballot_sync(0xffffffffu, cut);
+        if (lane == 0) cnt[warp] = __popc(in);
+        __syncthreads();
+        int at = n;
+#pragma unroll
+        for (int w = 0; w < JOIN_THREADS / 32; w++) {
+            if (w < warp) at += cnt[w];
+            n += cnt[w];
+        }
+        if (cut) list[at + __popc(in & ((1u << lane) - 1))] = i;      // in order: the blocks have to agree
+        __syncthreads();
+    }
+    return n;
+}
+
 // Spans in up to hundreds of pieces (few rows): block (i, r), the pieces over its threads.
 template <int DH>
 __global__ void __launch_bounds__(JOIN_THREADS)
-k_attn_join(AttnArgs a, int tile_rows, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
+k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
     Q36_GDS();
     constexpr int C4 = DH / 4, LANES = JOIN_THREADS / C4;      // threads over the dims, and pieces in parallel
-    extern __shared__ float w[];                               // one weight per piece
+    extern __shared__ float w[];                               // one weight per piece, then the list
     __shared__ float red[2][JOIN_THREADS / 32];
     __shared__ float4 acc[LANES][C4];
-    const AttnPart d = desc[blockIdx.x];
-    const int r = blockIdx.y, tid = threadIdx.x, cta = blockIdx.x;
-    if (d.parts == 0 || r >= d.rows) return;
-    const int stride = attn_part_floats(tile_rows, DH);
-    float m = -3.0e38f;
-    for (int p = tid; p < d.parts; p += JOIN_THREADS) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
-    m = warp_max(m);
-    if ((tid & 31) == 0) red[0][tid >> 5] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    float l = 0.f;
-    for (int p = tid; p < d.parts; p += JOIN_THREADS) {
-        const float *s = join_slot(part, d, cta, p, stride);
-        l += w[p] = s[2 * r + 1] * exp2f(s[2 * r] - m);
-    }
-    l = warp_sum(l);
-    if ((tid & 31) == 0) red[1][tid >> 5] = l;
-    __syncthreads();
-    l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-    const int c = tid % C4, lane = tid / C4;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    int *list = reinterpret_cast<int *>(w + grid);
+    const int n = join_list(desc, grid, list), tid = threadIdx.x;
+    for (int item = blockIdx.x; item < n * tile_rows; item += gridDim.x) {
+        const int cta = list[item / tile_rows], r = item % tile_rows;
+        const AttnPart d = desc[cta];
+        if (r >= d.rows) continue;
+        const int stride = attn_part_floats(tile_rows, DH);
+        float m = -3.0e38f;
+        for (int p = tid; p < d.parts; p += JOIN_THREADS) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
+        m = warp_max(m);
+        if ((tid & 31) == 0) red[0][tid >> 5] = m;
+        __syncthreads();
+        m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+        float l = 0.f;
+        for (int p = tid; p < d.parts; p += JOIN_THREADS) {
+            const float *s = join_slot(part, d, cta, p, stride);
+            l += w[p] = s[2 * r + 1] * exp2f(s[2 * r] - m);
+        }
+        l = warp_sum(l);
+        if ((tid & 31) == 0) red[1][tid >> 5] = l;
+        __syncthreads();
+        l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+        const int c = tid % C4, lane = tid / C4;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int p = lane; p < d.parts; p += LANES) {
-        const float f = w[p];
-        if (f == 0.f) continue;
-        const float4 v = *reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * tile_rows + r * DH + 4 * c);
-        o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-    }
-    acc[lane][c] = o;
-    __syncthreads();
-    if (lane == 0) {
+        for (int p = lane; p < d.parts; p += LANES) {
+            const float f = w[p];
+            if (f == 0.f) continue;
+            const float4 v = *reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * tile_rows + r * DH + 4 * c);
+            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
+        }
+        acc[lane][c] = o;
+        __syncthreads();
+        if (lane == 0) {
 #pragma unroll
-        for (int i = 1; i < LANES; i++) { const float4 v = acc[i][c]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
-        const float f = l == 0.f ? 0.f : 1.f / l;
-        attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-        if (c == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+            for (int i = 1; i < LANES; i++) { const float4 v = acc[i][c]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
+            const float f = l == 0.f ? 0.f : 1.f / l;
+            attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+            if (c == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+        }
+        __syncthreads();
     }
 }
 
 // Many rows, few pieces: a warp per row.
 template <int DH>
 __global__ void __launch_bounds__(JOIN_THREADS)
-k_attn_join_rows(AttnArgs a, int tile_rows, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
+k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
     Q36_GDS();
     constexpr int N4 = (DH + 127) / 128;      // 16-byte pieces of a row per lane
-    const AttnPart d = desc[blockIdx.x];
-    const int r = blockIdx.y * (JOIN_THREADS / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, cta = blockIdx.x;
-    if (d.parts == 0 || r >= d.rows) return;
-    const int stride = attn_part_floats(tile_rows, DH);
-    float m = -3.0e38f;
-    for (int p = lane; p < d.parts; p += 32) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
-    m = warp_max(m);
-    float l = 0.f;
-    float4 o[N4];
+    extern __shared__ int list[];
+    constexpr int WARPS = JOIN_THREADS / 32;
+    const int n = join_list(desc, grid, list), lane = threadIdx.x & 31, groups = tile_rows / WARPS;
+    for (int item = blockIdx.x; item < n * groups; item += gridDim.x) {
+        const int cta = list[item / groups], r = item % groups * WARPS + (threadIdx.x >> 5);
+        const AttnPart d = desc[cta];
+        if (r >= d.rows) continue;
+        const int stride = attn_part_floats(tile_rows, DH);
+        float m = -3.0e38f;
+        for (int p = lane; p < d.parts; p += 32) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
+        m = warp_max(m);
+        float l = 0.f;
+        float4 o[N4];
 #pragma unroll
-    for (int k = 0; k < N4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < d.parts; p0 += 32) {
-        float mine = 0.f;
-        if (p0 + lane < d.parts) {
-            const float *s = join_slot(part, d, cta, p0 + lane, stride);
-            mine = s[2 * r + 1] * exp2f(s[2 * r] - m);
-        }
-        l += warp_sum(mine);
+        for (int k = 0; k < N4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int p0 = 0; p0 < d.parts; p0 += 32) {
+            float mine = 0.f;
+            if (p0 + lane < d.parts) {
+                const float *s = join_slot(part, d, cta, p0 + lane, stride);
+                mine = s[2 * r + 1] * exp2f(s[2 * r] - m);
+            }
+            l += warp_sum(mine);
 #pragma unroll 4
-        for (int p = 0; p < min(32, d.parts - p0); p++) {
-            const float f = __shfl_sync(0xffffffffu, mine, p);
-            if (f == 0.f) continue;
-            const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p0 + p, stride) + 2 * tile_rows + r * DH);
+            for (int p = 0; p < min(32, d.parts - p0); p++) {
+                const float f = __shfl_sync(0xffffffffu, mine, p);
+                if (f == 0.f) continue;
+                const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p0 + p, stride) + 2 * tile_rows + r * DH);
 #pragma unroll
-            for (int k = 0; k < N4; k++) {
-                if (DH < 128 && lane >= DH / 4) continue;
-                const float4 v = s[32 * k + lane];
-                o[k].x = fmaf(f, v.x, o[k].x); o[k].y = fmaf(f, v.y, o[k].y); o[k].z = fmaf(f, v.z, o[k].z); o[k].w = fmaf(f, v.w, o[k].w);
+                for (int k = 0; k < N4; k++) {
+                    if (DH < 128 && lane >= DH / 4) continue;
+                    const float4 v = s[32 * k + lane];
+                    o[k].x = fmaf(f, v.x, o[k].x); o[k].y = fmaf(f, v.y, o[k].y); o[k].z = fmaf(f, v.z, o[k].z); o[k].w = fmaf(f, v.w, o[k].w);
+                }
             }
         }
-    }
-    const float f = l == 0.f ? 0.f : 1.f / l;
+        const float f = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int k = 0; k < N4; k++) {
-        if (DH < 128 && lane >= DH / 4) continue;
-        attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), make_float4(o[k].x * f, o[k].y * f, o[k].z * f, o[k].w * f));
+        for (int k = 0; k < N4; k++) {
+            if (DH < 128 && lane >= DH / 4) continue;
+            attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), make_float4(o[k].x * f, o[k].y * f, o[k].z * f, o[k].w * f));
+        }
+        if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
     }
-    if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
 }
 
 int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st) {
-    const dim3 threads(JOIN_THREADS);
+    const dim3 blocks((tile_rows > 16 ? 14 : 8) * sm_count()), threads(JOIN_THREADS);
     if (tile_rows > 16) {
-        const dim3 blocks(grid, tile_rows / (JOIN_THREADS / 32));
-        if (a.kv.Dh == 64) launch_k(k_attn_join_rows<64>, blocks, threads, 0, st, a, tile_rows, desc, part);
-        else if (a.kv.Dh == 128) launch_k(k_attn_join_rows<128>, blocks, threads, 0, st, a, tile_rows, desc, part);
-        else launch_k(k_attn_join_rows<256>, blocks, threads, 0, st, a, tile_rows, desc, part);
+        if (a.kv.Dh == 64) launch_k(k_attn_join_rows<64>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
+        else if (a.kv.Dh == 128) launch_k(k_attn_join_rows<128>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
+        else launch_k(k_attn_join_rows<256>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
         return check_launch();
     }
-    const dim3 blocks(grid, tile_rows);
-    if (a.kv.Dh == 64) launch_k(k_attn_join<64>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
-    else if (a.kv.Dh == 128) launch_k(k_attn_join<128>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
-    else launch_k(k_attn_join<256>, blocks, threads, grid * 4, st, a, tile_rows, desc, part);
+    if (a.kv.Dh == 64) launch_k(k_attn_join<64>, blocks, threads, grid * 8, st, a, tile_rows, grid, desc, part);
+    else if (a.kv.Dh == 128) launch_k(k_attn_join<128>, blocks, threads, grid * 8, st, a, tile_rows, grid, desc, part);
+    else launch_k(k_attn_join<256>, blocks, threads, grid * 8, st, a, tile_rows, grid, desc, part);
     return check_launch();
 }
 

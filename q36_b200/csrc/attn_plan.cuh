@@ -42,6 +42,11 @@ __device__ __forceinline__ long long seq_units(const AttnArgs &a, const SeqSpans
     return (long long)s.tiles * a.kv.Hkv * (s.u_hi - s.u_lo);
 }
 
+// (32 bits nearly always do)
+__device__ __forceinline__ long long div64(long long a, unsigned b) {
+    return a >> 32 ? a / b : (long long)((unsigned)a / b);
+}
+
 // Moves pos to the span that holds pos.at, from request pos.b (whose first unit is pos.seq_base) on.
 __device__ __forceinline__ void plan_locate(const AttnArgs &a, const SpanRule &r, PlanPos &pos) {
     for (;;) {
@@ -52,7 +57,7 @@ __device__ __forceinline__ void plan_locate(const AttnArgs &a, const SpanRule &r
         pos.b++;
     }
     const long long off = pos.at - pos.seq_base;
-    const int u = pos.s.u_hi - pos.s.u_lo, span = (int)(off / u);
+    const int u = pos.s.u_hi - pos.s.u_lo, span = (int)div64(off, u);
     pos.hk = span / pos.s.tiles;
     pos.rt = span - pos.hk * pos.s.tiles;
     pos.span_base = pos.seq_base + (long long)span * u;
@@ -80,7 +85,7 @@ __device__ __forceinline__ bool plan_start(const AttnArgs &a, const SpanRule &r,
         total += sm.sum[w];
     }
     const long long excl = before + inc - mine;
-    pos.per = max((total + gridDim.x - 1) / gridDim.x, (long long)min_units);
+    pos.per = max(div64(total + gridDim.x - 1, gridDim.x), (long long)min_units);
     pos.at = min(pos.per * blockIdx.x, total);
     pos.end = min(pos.at + pos.per, total);
     if (pos.at >= pos.end) return false;
@@ -118,7 +123,7 @@ struct AttnPart { int parts, slot, t0, n, hk, row0, rows, pad; };
 
 __device__ __forceinline__ AttnPart plan_parts(const AttnArgs &a, const SpanRule &r, const PlanSeg &g, const PlanPos &pos, int slot) {
     AttnPart p;
-    p.parts = (int)((g.span_base + g.units - 1) / pos.per - blockIdx.x) + 1;
+    p.parts = (int)(div64(g.span_base + g.units - 1, (unsigned)pos.per) - blockIdx.x) + 1;
     p.slot = slot;
     p.t0 = g.t0;
     p.n = g.n;

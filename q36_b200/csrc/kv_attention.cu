@@ -5,87 +5,146 @@
 
 namespace q36 {
 
-constexpr int JOIN_THREADS = 128;
+constexpr int JOIN_THREADS = 128, JOIN_PIECES = 256;
+constexpr int JOIN_ID = 0xffff, JOIN_LONG = 0x10000;      // list entries: the CTA, and whether its span is in more than 32 pieces
 
-// The join.  Row r of the span whose first piece CTA i had, if it had one of a cut span: piece p counts l_p 2^(m_p - m); a piece that
-// saw nothing has no row to read.
+// Which CTAs had the first piece of a cut span (n of them), into list[].  Every block finds out for itself and takes its share of (span,
+// rows): a block per CTA and row, most of which leave at once, took 7 us at 296 x 16 and 12 at 148 x 64.
+template <int THREADS>
+__device__ __forceinline__ int join_list(const AttnPart *desc, int grid, int *list) {
+    constexpr int PER = (DEC_MAX_OCC * 160 + THREADS - 1) / THREADS;      // all of them on their way at once, on up to 160 SMs
+    __shared__ int cnt[PER][THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int n = 0;
+    for (int base = 0; base < grid; base += PER * THREADS) {
+        int parts[PER];
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            const int i = base + k * THREADS + threadIdx.x;
+            parts[k] = i < grid ? desc[i].parts : 0;
+        }
+        unsigned in[PER];
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            in[k] = __ballot_sync(0xffffffffu, parts[k] > 0);
+            if (lane == 0) cnt[k][warp] = __popc(in[k]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < PER; k++) {
+            int at = n;
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; w++) {
+                if (w < warp) at += cnt[k][w];
+                n += cnt[k][w];
+            }
+            if (parts[k] > 0) list[at + __popc(in[k] & ((1u << lane) - 1))] = (base + k * THREADS + threadIdx.x) | (parts[k] > 32 ? JOIN_LONG : 0);      // in order: the blocks have to agree
+        }
+    }
+    __syncthreads();
+    return n;
+}
+
+// The join.  Row r of the span whose first piece CTA i had: piece p counts l_p 2^(m_p - m); a piece that saw nothing has no row to read.
 __device__ __forceinline__ const float *join_slot(const float *part, const AttnPart &d, int cta, int p, int stride) {
     return part + (size_t)(p == 0 ? d.slot : 2 * (cta + p)) * stride;
 }
 
-// Which CTAs had the first piece of a cut span (n of them), into list[].  Every block finds out for itself and takes its share of (span,
-// rows): a block per CTA and row, most of which leave at once, took 7 us at 296 x 16 and 12 at 148 x 64.
-__device__ __forceinline__ int join_list(const AttnPart *desc, int grid, int *list) {
-    __shared__ int cnt[JOIN_THREADS / 32];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int n = 0;
-    for (int i0 = 0; i0 < grid; i0 += JOIN_THREADS) {
-        const int i = i0 + threadIdx.x;
-        const bool cut = i < grid && desc[i].parts > 0;
-        const unsigned in = __ballot_sync(0xffffffffu, cut);
-        if (lane == 0) cnt[warp] = __popc(in);
-        __syncthreads();
-        int at = n;
-#pragma unroll
-        for (int w = 0; w < JOIN_THREADS / 32; w++) {
-            if (w < warp) at += cnt[w];
-            n += cnt[w];
-        }
-        if (cut) list[at + __popc(in & ((1u << lane) - 1))] = i;      // in order: the blocks have to agree
-        __syncthreads();
+// The weights of a row's pieces, lane p has those of pieces p, p + 32, ..: their sum, and the largest m.
+template <bool KEEP>
+__device__ __forceinline__ void join_weights(const AttnPart &d, const float *part, int cta, int stride, int r, int lane, float *w, float &first, float &m, float &l) {
+    m = -3.0e38f;
+    l = first = 0.f;
+    for (int p = lane; p < d.parts; p += 32) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
+    m = warp_max(m);
+    for (int p = lane; p < d.parts; p += 32) {
+        const float2 ml = *reinterpret_cast<const float2 *>(join_slot(part, d, cta, p, stride) + 2 * r);
+        const float f = ml.y * exp2f(ml.x - m);
+        if (p == lane) first = f;
+        l += f;
+        if (KEEP) w[p] = f;
     }
-    return n;
+    l = warp_sum(l);
+}
+// a lane's share of the weighted rows of pieces p0, p0 + step, ..: several on their way at a time
+template <int DH, typename W>
+__device__ __forceinline__ void join_rows(const AttnPart &d, const float *part, int cta, int stride, int tile_rows, int r, int lane, int p0, int step, W weight,
+                                          float4 (&o)[(DH + 127) / 128]) {
+    constexpr int N4 = (DH + 127) / 128, AT_ONCE = 8 / N4;
+#pragma unroll
+    for (int k = 0; k < N4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (; p0 < d.parts; p0 += step * AT_ONCE) {
+        float4 v[AT_ONCE][N4];
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; x++) {
+            const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, min(p0 + x * step, d.parts - 1), stride) + 2 * tile_rows + r * DH);
+#pragma unroll
+            for (int k = 0; k < N4; k++) v[x][k] = s[32 * k + (DH < 128 ? lane % (DH / 4) : lane)];
+        }
+#pragma unroll
+        for (int x = 0; x < AT_ONCE; x++) {
+            const float f = weight(p0 + x * step);      // (0 behind the last piece)
+            if (f == 0.f) continue;
+#pragma unroll
+            for (int k = 0; k < N4; k++) {
+                o[k].x = fmaf(f, v[x][k].x, o[k].x); o[k].y = fmaf(f, v[x][k].y, o[k].y); o[k].z = fmaf(f, v[x][k].z, o[k].z); o[k].w = fmaf(f, v[x][k].w, o[k].w);
+            }
+        }
+    }
+}
+template <int DH>
+__device__ __forceinline__ void join_store(const AttnArgs &a, const AttnPart &d, int r, int lane, int k, float4 o, float l) {
+    if (DH < 128 && lane >= DH / 4) return;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
 }
 
-// Spans in up to hundreds of pieces (few rows): block (i, r), the pieces over its threads.
+// Tiles of 8 or 16 rows.  Spans in up to 32 pieces: a block per span, a warp per row.  Longer ones: a block per row, its warps share
+// the pieces.
+constexpr int JOIN_WIDE = 256;
 template <int DH>
-__global__ void __launch_bounds__(JOIN_THREADS)
+__global__ void __launch_bounds__(JOIN_WIDE)
 k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
     Q36_GDS();
-    constexpr int C4 = DH / 4, LANES = JOIN_THREADS / C4;      // threads over the dims, and pieces in parallel
-    extern __shared__ float w[];                               // one weight per piece, then the list
-    __shared__ float red[2][JOIN_THREADS / 32];
-    __shared__ float4 acc[LANES][C4];
+    constexpr int N4 = (DH + 127) / 128, WARPS = JOIN_WIDE / 32;      // 16-byte pieces of a row per lane
+    extern __shared__ float w[];                                      // one weight per piece, then the list
+    __shared__ float4 acc[WARPS][N4][32];
     int *list = reinterpret_cast<int *>(w + grid);
-    const int n = join_list(desc, grid, list), tid = threadIdx.x;
+    const int n = join_list<JOIN_WIDE>(desc, grid, list), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int stride = attn_part_floats(tile_rows, DH);
+    float m, l, first;
+    float4 o[N4];
     for (int item = blockIdx.x; item < n * tile_rows; item += gridDim.x) {
-        const int cta = list[item / tile_rows], r = item % tile_rows;
-        const AttnPart d = desc[cta];
-        if (r >= d.rows) continue;
-        const int stride = attn_part_floats(tile_rows, DH);
-        float m = -3.0e38f;
-        for (int p = tid; p < d.parts; p += JOIN_THREADS) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
-        m = warp_max(m);
-        if ((tid & 31) == 0) red[0][tid >> 5] = m;
-        __syncthreads();
-        m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-        float l = 0.f;
-        for (int p = tid; p < d.parts; p += JOIN_THREADS) {
-            const float *s = join_slot(part, d, cta, p, stride);
-            l += w[p] = s[2 * r + 1] * exp2f(s[2 * r] - m);
-        }
-        l = warp_sum(l);
-        if ((tid & 31) == 0) red[1][tid >> 5] = l;
-        __syncthreads();
-        l = red[1][0] + red[1][1] + red[1][2] + red[1][3];
-        const int c = tid % C4, lane = tid / C4;
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-        for (int p = lane; p < d.parts; p += LANES) {
-            const float f = w[p];
-            if (f == 0.f) continue;
-            const float4 v = *reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * tile_rows + r * DH + 4 * c);
-            o.x = fmaf(f, v.x, o.x); o.y = fmaf(f, v.y, o.y); o.z = fmaf(f, v.z, o.z); o.w = fmaf(f, v.w, o.w);
-        }
-        acc[lane][c] = o;
-        __syncthreads();
-        if (lane == 0) {
+        const int cta = list[item % n] & JOIN_ID, row = item / n;
+        if (!(list[item % n] & JOIN_LONG)) {
+            if (row) continue;
+            const AttnPart d = desc[cta];
+            for (int r = warp; r < d.rows; r += WARPS) {
+                join_weights<false>(d, part, cta, stride, r, lane, nullptr, first, m, l);
+                join_rows<DH>(d, part, cta, stride, tile_rows, r, lane, 0, 1, [&](int p) { return p < 32 ? __shfl_sync(0xffffffffu, first, p) : 0.f; }, o);
 #pragma unroll
-            for (int i = 1; i < LANES; i++) { const float4 v = acc[i][c]; o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w; }
-            const float f = l == 0.f ? 0.f : 1.f / l;
-            attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * c, make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
-            if (c == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+                for (int k = 0; k < N4; k++) join_store<DH>(a, d, r, lane, k, o[k], l);
+                if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+            }
+            continue;
         }
+        const AttnPart d = desc[cta];
+        if (row >= d.rows) continue;
+        if (warp == 0) join_weights<true>(d, part, cta, stride, row, lane, w, first, m, l);
+        else join_weights<false>(d, part, cta, stride, row, lane, nullptr, first, m, l);
+        __syncthreads();
+        join_rows<DH>(d, part, cta, stride, tile_rows, row, lane, warp, WARPS, [&](int p) { return p < d.parts ? w[p] : 0.f; }, o);
+#pragma unroll
+        for (int k = 0; k < N4; k++) acc[warp][k][lane] = o[k];
+        __syncthreads();
+        if (warp < N4) {
+            float4 t = acc[0][warp][lane];
+#pragma unroll
+            for (int i = 1; i < WARPS; i++) { const float4 v = acc[i][warp][lane]; t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w; }
+            join_store<DH>(a, d, row, lane, warp, t, l);
+        }
+        if (threadIdx.x == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + row, m, l);
         __syncthreads();
     }
 }
@@ -97,58 +156,36 @@ k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict
     Q36_GDS();
     constexpr int N4 = (DH + 127) / 128;      // 16-byte pieces of a row per lane
     extern __shared__ int list[];
+    __shared__ float w[JOIN_THREADS / 32][JOIN_PIECES];      // (a tile kernel has one CTA per SM)
     constexpr int WARPS = JOIN_THREADS / 32;
-    const int n = join_list(desc, grid, list), lane = threadIdx.x & 31, groups = tile_rows / WARPS;
+    const int n = join_list<JOIN_THREADS>(desc, grid, list), lane = threadIdx.x & 31, groups = tile_rows / WARPS;
+    const int stride = attn_part_floats(tile_rows, DH);
     for (int item = blockIdx.x; item < n * groups; item += gridDim.x) {
-        const int cta = list[item / groups], r = item % groups * WARPS + (threadIdx.x >> 5);
+        const int cta = list[item / groups] & JOIN_ID, r = item % groups * WARPS + (threadIdx.x >> 5);
         const AttnPart d = desc[cta];
         if (r >= d.rows) continue;
-        const int stride = attn_part_floats(tile_rows, DH);
-        float m = -3.0e38f;
-        for (int p = lane; p < d.parts; p += 32) m = fmaxf(m, join_slot(part, d, cta, p, stride)[2 * r]);
-        m = warp_max(m);
-        float l = 0.f;
+        float m, l, first;
         float4 o[N4];
+        float *mine = w[threadIdx.x >> 5];
+        join_weights<true>(d, part, cta, stride, r, lane, mine, first, m, l);
+        __syncwarp();
+        join_rows<DH>(d, part, cta, stride, tile_rows, r, lane, 0, 1, [&](int p) { return p < d.parts ? mine[p] : 0.f; }, o);
 #pragma unroll
-        for (int k = 0; k < N4; k++) o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int p0 = 0; p0 < d.parts; p0 += 32) {
-            float mine = 0.f;
-            if (p0 + lane < d.parts) {
-                const float *s = join_slot(part, d, cta, p0 + lane, stride);
-                mine = s[2 * r + 1] * exp2f(s[2 * r] - m);
-            }
-            l += warp_sum(mine);
-#pragma unroll 4
-            for (int p = 0; p < min(32, d.parts - p0); p++) {
-                const float f = __shfl_sync(0xffffffffu, mine, p);
-                if (f == 0.f) continue;
-                const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p0 + p, stride) + 2 * tile_rows + r * DH);
-#pragma unroll
-                for (int k = 0; k < N4; k++) {
-                    if (DH < 128 && lane >= DH / 4) continue;
-                    const float4 v = s[32 * k + lane];
-                    o[k].x = fmaf(f, v.x, o[k].x); o[k].y = fmaf(f, v.y, o[k].y); o[k].z = fmaf(f, v.z, o[k].z); o[k].w = fmaf(f, v.w, o[k].w);
-                }
-            }
-        }
-        const float f = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-        for (int k = 0; k < N4; k++) {
-            if (DH < 128 && lane >= DH / 4) continue;
-            attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), make_float4(o[k].x * f, o[k].y * f, o[k].z * f, o[k].w * f));
-        }
+        for (int k = 0; k < N4; k++) join_store<DH>(a, d, r, lane, k, o[k], l);
         if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+        __syncwarp();
     }
 }
 
 int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st) {
-    const dim3 blocks((tile_rows > 16 ? 14 : 8) * sm_count()), threads(JOIN_THREADS);
     if (tile_rows > 16) {
+        const dim3 blocks(14 * sm_count()), threads(JOIN_THREADS);
         if (a.kv.Dh == 64) launch_k(k_attn_join_rows<64>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
         else if (a.kv.Dh == 128) launch_k(k_attn_join_rows<128>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
         else launch_k(k_attn_join_rows<256>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
         return check_launch();
     }
+    const dim3 blocks(6 * sm_count()), threads(JOIN_WIDE);
     if (a.kv.Dh == 64) launch_k(k_attn_join<64>, blocks, threads, grid * 8, st, a, tile_rows, grid, desc, part);
     else if (a.kv.Dh == 128) launch_k(k_attn_join<128>, blocks, threads, grid * 8, st, a, tile_rows, grid, desc, part);
     else launch_k(k_attn_join<256>, blocks, threads, grid * 8, st, a, tile_rows, grid, desc, part);

@@ -39,7 +39,7 @@ __device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t w, uint32_t (&h)[4]) {
         : "r"(w));
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -103,41 +103,80 @@ struct DecFrag {
     uint32_t k[2][W];      // K words of tokens g and g + 8: word b = dims 32b + 8j ..
     uint32_t v[2][W];      // V of token pairs j and j + 4, group g: first half token 2p, second half token 2p + 1
     uint32_t ks[2][SW];    // K scales of tokens g and g + 8
-    uint32_t vs[2];        // V scales of tokens g and g + 8, blocks VB j .. (bytes)
-    __device__ __forceinline__ void load(const uint8_t *reg, int bs, int tok, int g, int j) {
-        const uint8_t *vc = reg + bs * (DH / 2), *ksp = reg + bs * DH, *vsp = ksp + bs * NB;
+    uint32_t vs[VB];       // V scales of tokens g (low half) and g + 8, blocks VB j ..
+    // p: the region plus the group's first token's bytes of codes, and its scales; lane parts added by the caller
+    __device__ __forceinline__ void load_k(const uint8_t *pk, const uint8_t *ps) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            ld_words<W>(reg + kv_k_off(tok + g + 8 * h, j, 0, DH), k[h]);
-            ld_words<W>(vc + kv_v_off(tok + 2 * j + 8 * h, g, 0, DH), v[h]);
-            const uint8_t *kp = ksp + (tok + g + 8 * h) * NB, *vp = vsp + (tok + g + 8 * h) * NB;
+            ld_words<W>(pk + h * 8 * (DH / 2), k[h]);
+            const uint8_t *kp = ps + h * 8 * NB;
             if constexpr (NB == 2) ks[h][0] = __ldg(reinterpret_cast<const uint16_t *>(kp));
             else if constexpr (NB == 4) ks[h][0] = __ldg(reinterpret_cast<const uint32_t *>(kp));
             else { const uint2 u = __ldg(reinterpret_cast<const uint2 *>(kp)); ks[h][0] = u.x; ks[h][1] = u.y; }
-            if constexpr (NB == 8) vs[h] = __ldg(reinterpret_cast<const uint16_t *>(vp) + j);
-            else if constexpr (NB == 4) vs[h] = __ldg(vp + j);
-            else vs[h] = __ldg(vp + (j & 1));
         }
+    }
+    __device__ __forceinline__ void load_v(const uint8_t *pv, const uint8_t *ps) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) ld_words<W>(pv + h * 4 * DH, v[h]);
+#pragma unroll
+        for (int c = 0; c < VB; c++) vs[c] = __ldg(ps + c) | (uint32_t)__ldg(ps + c + 8 * NB) << 16;
     }
 };
 
-template <int DH, int NT>
+// The wide form's weights of block b: 2^(S + vs - M), M per row and block; moves M, and with it the block's sums.
+template <int DH, int NT, int TERMS, int VB>
+__device__ __forceinline__ void wide_weights(float (*Ms)[8 * NT], const uint32_t (&vs)[VB], const float (&s)[NT][4], uint32_t (&w)[TERMS][NT][2],
+                                             float (&o)[NT][DH / 32][2][4], int b, int lane) {
+    const int j = lane & 3;
+    const uint32_t vv = __shfl_sync(0xffffffffu, vs[b % VB], (lane & 28) | (b / VB));
+    const float v0 = (float)(vv & 0xffff) - 127.f, v1 = (float)(vv >> 16) - 127.f;
+#pragma unroll
+    for (int nt = 0; nt < NT; nt++) {
+        float p[4];
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            float *Mp = &Ms[b][nt * 8 + 2 * j + c];
+            const float x0 = s[nt][c] + v0, x1 = s[nt][c + 2] + v1;
+            __syncwarp();
+            float M = *Mp;
+            const float t = column_max(fmaxf(x0, x1));
+            if (t > M + (DEC_WIDE_MAX - DEC_WIDE_TOP)) {
+                const float f = ex2(M - t);
+                M = t;
+                o[nt][b][0][c] *= f; o[nt][b][0][c + 2] *= f;
+                o[nt][b][1][c] *= f; o[nt][b][1][c + 2] *= f;
+            }
+            __syncwarp();
+            if (lane < 4) *Mp = M;
+            p[c] = ex2(x0 - (M - DEC_WIDE_TOP));
+            p[c + 2] = ex2(x1 - (M - DEC_WIDE_TOP));
+        }
+        weights_f16<TERMS>(p, w, nt);
+    }
+}
+
+template <int DH, int NT, int TERMS>
 struct DecSmem {
     static constexpr int R = 8 * NT, LD = DH + 4;
     alignas(16) float o[DEC_WARPS][R][LD];
     float m[DEC_WARPS][R], l[DEC_WARPS][R], M[DEC_WARPS][DH / 32][R];      // M: the wide form's references
     alignas(16) uint16_t sc[DEC_WARPS][4][DH / 32][4];     // f16 2^(vs - anchor): [j][block][tokens 2j, 2j+1, 2j+8, 2j+9]
+    alignas(16) uint4 q[TERMS][NT][DH / 32][32];           // operand fragments of q, by lane
+    int hi[R], lo[R];                                      // first and last token that a row sees
     PlanSmem<DEC_THREADS> plan;
 };
 
 template <int DH, int NT, bool F32>
-__global__ void __launch_bounds__(DEC_THREADS)
+// What bounds it: instructions, 350 per warp and 16 tokens of 128 dims, each warp issuing one in five cycles: 16 warps per SM at 128 registers
+// are better than 12 at 168 (64 requests, 266,000 tokens: 38 against 43 us), 20 at 96 spill (48); wider accumulators
+// (256 dims, or 16 rows of 128) keep 8 warps at 255 (41 us at 112,000 tokens of 256; 46 with 12 warps, 72 with 16).
+__global__ void __launch_bounds__(DEC_THREADS, NT * DH <= 128 ? 4 : 2)
 k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restrict__ part) {
     constexpr int NB = DH / 32, R = 8 * NT, TERMS = F32 ? 2 : 1;
     using Frag = DecFrag<DH>;
     Q36_GDS();
     extern __shared__ __align__(16) uint8_t smem_raw[];
-    DecSmem<DH, NT> &sm = *reinterpret_cast<DecSmem<DH, NT> *>(smem_raw);
+    DecSmem<DH, NT, F32 ? 2 : 1> &sm = *reinterpret_cast<DecSmem<DH, NT, F32 ? 2 : 1> *>(smem_raw);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, j = lane & 3;
     const SpanRule rule{R, DEC_UNIT, all};
     PlanPos pos;
@@ -149,10 +188,9 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
     bool first = true;
     while (pos.at < pos.end) {
         const PlanSeg sg = plan_segment(pos);
-        // ---- q: operand fragments of the row tile, lane = (row g, quarter j): dims 32b + 8j + 4s + 0..3
-        uint32_t qf[TERMS][NT][NB][4];
+        // ---- q: operand fragments of the row tile, lane = (row g, quarter j): dims 32b + 8j + 4s + 0..3.  They are the same for
+        // every warp and stay in shared memory: a read per block and group costs less than the registers.
         float fac[NT][2];       // scale * log2(e) / 2^(power of two of the row), of columns 2j, 2j + 1
-        int hi[NT][2], lo[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
             const int r = sg.rt * R + nt * 8 + g, rows = sg.n * a.G;
@@ -162,15 +200,12 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
             float am = 0.f;
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                const size_t e = (size_t)(sg.t0 + i) * a.q_stride + (size_t)hq * DH + 32 * b + 8 * j;
-                if (!in) {
+                load8(a.q, (size_t)(sg.t0 + i) * a.q_stride + (size_t)hq * DH + 32 * b + 8 * j, !F32, x[b]);
 #pragma unroll
-                    for (int c = 0; c < 8; c++) x[b][c] = 0.f;
-                } else {
-                    load8(a.q, e, !F32 || a.q_bf16, x[b]);
+                for (int c = 0; c < 8; c++) {
+                    x[b][c] = in ? x[b][c] : 0.f;
+                    am = fmaxf(am, fabsf(x[b][c]));
                 }
-#pragma unroll
-                for (int c = 0; c < 8; c++) am = fmaxf(am, fabsf(x[b][c]));
             }
             am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
             am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
@@ -178,25 +213,28 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
             const int up = am > 0.f ? min(14 - ea, 126) : 0;
             const float f = __uint_as_float((uint32_t)(up + 127) << 23), inv = a.scale2 * __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int b = 0; b < NB; b++) {
+                if (b % DEC_WARPS != warp) continue;
+                uint32_t h[4], t[4];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const float x0 = x[b][2 * c] * f, x1 = x[b][2 * c + 1] * f;
-                    qf[0][nt][b][c] = pack_f16(x0, x1);
-                    if constexpr (F32) {
-                        const float2 h = unpack_f16(qf[0][nt][b][c]);
-                        qf[1][nt][b][c] = pack_f16(x0 - h.x, x1 - h.y);
-                    }
+                    h[c] = pack_f16(x0, x1);
+                    const float2 back = unpack_f16(h[c]);
+                    t[c] = pack_f16(x0 - back.x, x1 - back.y);
                 }
-            const int p = sg.len - sg.n + i, l0 = a.window > 0 ? p - a.window + 1 : 0;
-            const int ph = in ? p : -1;
-#pragma unroll
-            for (int c = 0; c < 2; c++) {
-                fac[nt][c] = __shfl_sync(0xffffffffu, inv, 8 * j + 4 * c);
-                hi[nt][c] = __shfl_sync(0xffffffffu, ph, 8 * j + 4 * c);
-                lo[nt][c] = __shfl_sync(0xffffffffu, l0, 8 * j + 4 * c);
+                sm.q[0][nt][b][lane] = make_uint4(h[0], h[1], h[2], h[3]);
+                if constexpr (F32) sm.q[1][nt][b][lane] = make_uint4(t[0], t[1], t[2], t[3]);
             }
+            const int p = sg.len - sg.n + i;
+            if (warp == 0 && j == 0) {
+                sm.hi[nt * 8 + g] = in ? p : -1;
+                sm.lo[nt * 8 + g] = a.window > 0 ? p - a.window + 1 : 0;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) fac[nt][c] = __shfl_sync(0xffffffffu, inv, 8 * j + 4 * c);
         }
+        __syncthreads();
         // tokens that every row of the tile sees (rows beyond the last one see none: their tile is never interior; its last rows'
         // results are not stored)
         const int i_first = sg.rt * R / a.G, i_last = min(sg.rt * R + R - 1, sg.n * a.G - 1) / a.G;
@@ -204,7 +242,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
         const int all_hi = sg.len - sg.n + i_first, all_lo = a.window > 0 ? sg.len - sg.n + i_last - a.window + 1 : 0;
 
         float m[NT][2], l[NT][2], o[NT][NB][2][4];
-        int anchor = 0;          // 0: no group read yet; -1: wide
+        int anchor = 0;          // 0: no group read yet
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -217,197 +255,247 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                     for (int c = 0; c < 4; c++) o[nt][b][u][c] = 0.f;
         }
 
-        // ---- this warp's groups: every DEC_WARPS-th.  Block ids come 32 groups at a time, one per lane.
+        // ---- this warp's groups: a quarter of the piece.  Block ids come 32 groups at a time, one per lane.
         const int *row = a.table + (size_t)sg.b * a.max_blocks;
-        const int n_mine = (sg.u1 - sg.u0 - warp + DEC_WARPS - 1) / DEC_WARPS, unit0 = sg.u_first + sg.u0 + warp;
+        const int n_all = sg.u1 - sg.u0, first_mine = n_all * warp / DEC_WARPS, n_mine = n_all * (warp + 1) / DEC_WARPS - first_mine;
+        const int unit0 = sg.u_first + sg.u0 + first_mine;
+        const uint8_t *head_base = a.kv.base + (size_t)sg.hk * a.kv.region();
+        const uint32_t block_bytes = (uint32_t)(a.kv.region() * a.kv.Hkv);
+        // a lane's part of the addresses: codes of K and V, scales of K and V
+        const uint32_t lane_k = g * (DH / 2) + j * (DH / 8), lane_v = a.kv.bs * (DH / 2) + j * DH + g * (DH / 8), lane_ks = a.kv.bs * DH + g * NB,
+                       lane_vs = lane_ks + a.kv.bs * NB + (NB >= 4 ? Frag::VB * j : j & 1);
         int ids = -1;
-        auto fetch_ids = [&](int k) {
-            const int gi = k + lane;
-            ids = -1;
-            if (gi < n_mine) {
-                const int col = ((unit0 + gi * DEC_WARPS) * DEC_UNIT) >> a.kv.log_bs;
-                if (col < a.max_blocks) ids = __ldg(row + col);
+        // group k's page and its first token there; false when the group is not there
+        auto page_of = [&](int k, const uint8_t *&reg, int &t) {
+            if ((k & 31) == 0) {
+                const int col = (unit0 + k + lane) * DEC_UNIT >> a.kv.log_bs;
+                ids = k + lane < n_mine && col < a.max_blocks ? __ldg(row + col) : -1;
             }
-        };
-        auto load_group = [&](int k, Frag &f) {
-            if ((k & 31) == 0) fetch_ids(k);
             const int id = __shfl_sync(0xffffffffu, ids, k & 31);
-            const bool ok = id >= 0 && id < a.kv.n_blocks;
-            if (ok) f.load(a.kv.at(id, sg.hk), a.kv.bs, ((unit0 + k * DEC_WARPS) * DEC_UNIT) & (a.kv.bs - 1), g, j);
-            return ok;
+            t = (unit0 + k) * DEC_UNIT & (a.kv.bs - 1);
+            reg = head_base + (size_t)(uint32_t)id * block_bytes;
+            return (unsigned)id < (unsigned)a.kv.n_blocks;
         };
-        Frag cur, nxt;
-        bool cur_ok = n_mine > 0 && load_group(0, cur);
-        for (int k = 0; k < n_mine; k++) {
-            const bool nxt_ok = k + 1 < n_mine && load_group(k + 1, nxt);
-            if (cur_ok) {
-                const int tok = (unit0 + k * DEC_WARPS) * DEC_UNIT;
-                const bool inner = tok >= all_lo && tok + DEC_UNIT - 1 <= all_hi;
-                // V exponents (own: tokens g, g + 8, blocks VB j ..): inside the window?
-                if (anchor >= 0) {
-                    int top = 0;
-                    bool out = false;
-                    const bool in0 = inner || (tok + g <= any_hi && tok + g >= any_lo), in1 = inner || (tok + g + 8 <= any_hi && tok + g + 8 >= any_lo);
-                    if (anchor == 0) {
+        // K of the next group is asked for when this group's has been used, V likewise: no second set of registers
+        Frag f;
+        const uint8_t *reg = head_base;
+        int t_in = 0;
+        bool ok = n_mine > 0 && page_of(0, reg, t_in), ok_next = false;
+        if (ok) {
+            f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
+            f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
+        }
+        int k = 0, tok = 0;
+        bool inner = false;
+        float s[NT][4];
+        uint32_t w[TERMS][NT][2];
+        // S of the group (log2 units), -infinity where a row does not see the token; K of the next one asked for; m moved when needed
+        auto scores = [&](bool with_o) {
 #pragma unroll
-                        for (int c = 0; c < Frag::VB; c++)
-                            top = max(top, max(in0 ? (int)(cur.vs[0] >> (8 * c)) & 0xff : 0, in1 ? (int)(cur.vs[1] >> (8 * c)) & 0xff : 0));
-                        anchor = (int)__reduce_max_sync(0xffffffffu, (unsigned)top);
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) s[nt][c] = 0.f;
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+                uint32_t k0[4], k1[4];
+                e2m1x8_to_f16x2(f.k[0][b], k0);
+                e2m1x8_to_f16x2(f.k[1][b], k1);
+                const float sc0 = __uint_as_float(((f.ks[0][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
+                const float sc1 = __uint_as_float(((f.ks[1][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int t = 0; t < TERMS; t++) {
+                        const uint4 q = sm.q[t][nt][b][lane];
+                        mma_f16(c, k0[0], k1[0], k0[1], k1[1], q.x, q.y);
+                        mma_f16(c, k0[2], k1[2], k0[3], k1[3], q.z, q.w);
                     }
-#pragma unroll
-                    for (int c = 0; c < Frag::VB; c++) {
-                        const int v0 = (int)(cur.vs[0] >> (8 * c)) & 0xff, v1 = (int)(cur.vs[1] >> (8 * c)) & 0xff;
-                        out |= in0 && v0 > 1 && (unsigned)(v0 - anchor + DEC_WIN_LO) > (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
-                        out |= in1 && v1 > 1 && (unsigned)(v1 - anchor + DEC_WIN_LO) > (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
-                    }
-                    __syncwarp();
-                    if (__any_sync(0xffffffffu, out)) {
-                        // the sums so far count 2^(m + anchor - 127)
-#pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int c = 0; c < 2; c++)
-                                for (int b = g; b < NB; b += 8)
-                                    sm.M[warp][b][nt * 8 + 2 * j + c] = m[nt][c] == DEC_NONE ? DEC_NONE : m[nt][c] + (float)(anchor - 127) + DEC_WIDE_TOP;
-                        anchor = -1;
-                        __syncwarp();
-                    } else if (NB >= 4 || j < NB) {
-#pragma unroll
-                        for (int c = 0; c < Frag::VB; c++) {
-                            const int b = Frag::VB * j + c;
-                            const int e0 = ((int)(cur.vs[0] >> (8 * c)) & 0xff) - anchor + 15, e1 = ((int)(cur.vs[1] >> (8 * c)) & 0xff) - anchor + 15;
-                            // (a block of zeros, or a token that no row sees: any finite factor)
-                            sm.sc[warp][g >> 1][b][g & 1] = (uint16_t)(min(max(e0, 0), 30) << 10);
-                            sm.sc[warp][g >> 1][b][2 + (g & 1)] = (uint16_t)(min(max(e1, 0), 30) << 10);
-                        }
-                    }
+                    s[nt][0] = fmaf(c[0], sc0, s[nt][0]);
+                    s[nt][1] = fmaf(c[1], sc0, s[nt][1]);
+                    s[nt][2] = fmaf(c[2], sc1, s[nt][2]);
+                    s[nt][3] = fmaf(c[3], sc1, s[nt][3]);
                 }
-                // scores
-                float s[NT][4];
+            }
+            if (ok_next) f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) s[nt][c] = 0.f;
-#pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    uint32_t k0[4], k1[4];
-                    e2m1x8_to_f16x2(cur.k[0][b], k0);
-                    e2m1x8_to_f16x2(cur.k[1][b], k1);
-                    const float sc0 = __uint_as_float(((cur.ks[0][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
-                    const float sc1 = __uint_as_float(((cur.ks[1][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        float c[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                        for (int t = 0; t < TERMS; t++) {
-                            mma_f16(c, k0[0], k1[0], k0[1], k1[1], qf[t][nt][b][0], qf[t][nt][b][1]);
-                            mma_f16(c, k0[2], k1[2], k0[3], k1[3], qf[t][nt][b][2], qf[t][nt][b][3]);
-                        }
-                        s[nt][0] = fmaf(c[0], sc0, s[nt][0]);
-                        s[nt][1] = fmaf(c[1], sc0, s[nt][1]);
-                        s[nt][2] = fmaf(c[2], sc1, s[nt][2]);
-                        s[nt][3] = fmaf(c[3], sc1, s[nt][3]);
-                    }
-                }
-                bool move = false;
+                for (int c = 0; c < 4; c++) s[nt][c] *= fac[nt][c & 1];
+            if (!inner) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
-                        float x = s[nt][c] * fac[nt][c & 1];
-                        if (!inner) {
-                            const int tt = tok + g + (c >> 1) * 8;
-                            if (tt > hi[nt][c & 1] || tt < lo[nt][c & 1]) x = -INFINITY;
-                        }
-                        s[nt][c] = x;
-                        move |= x > m[nt][c & 1] + DEC_MAX;
+                        const int tt = tok + g + (c >> 1) * 8, r = nt * 8 + 2 * j + (c & 1);
+                        if (tt > sm.hi[r] || tt < sm.lo[r]) s[nt][c] = -INFINITY;
                     }
-                if (__any_sync(0xffffffffu, move)) {
+            }
+            bool move = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) move |= fmaxf(s[nt][c], s[nt][c + 2]) > m[nt][c] + DEC_MAX;
+            if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 2; c++) {
+                        const float mn = fmaxf(m[nt][c], column_max(fmaxf(s[nt][c], s[nt][c + 2])) - DEC_TOP), by = ex2(m[nt][c] - mn);
+                        l[nt][c] *= by;
+                        m[nt][c] = mn;
+                        if (with_o) {
+#pragma unroll
+                            for (int b = 0; b < NB; b++)
+#pragma unroll
+                                for (int u = 0; u < 2; u++) { o[nt][b][u][c] *= by; o[nt][b][u][c + 2] *= by; }
+                        }
+                    }
+            }
+        };
+        // the f16 operand of two blocks of V: rows dims 4g + 2u (+1), columns tokens
+        auto v_codes = [&](int b2, uint32_t (&ev)[2][4], uint32_t (&od)[2][4]) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {       // [token pair j, j + 4][byte: block 2 b2 codes 0/1, 2/3, block 2 b2 + 1 codes ...]
+                const uint32_t A = f.v[e][b2], B = f.v[e][NB / 2 + b2];
+                e2m1x8_to_f16x2((A & 0x0f0f0f0fu) | ((B << 4) & 0xf0f0f0f0u), ev[e]);
+                e2m1x8_to_f16x2(((A >> 4) & 0x0f0f0f0fu) | (B & 0xf0f0f0f0u), od[e]);
+            }
+        };
+#pragma unroll 1
+        for (; k < n_mine; k++) {
+            ok_next = k + 1 < n_mine && page_of(k + 1, reg, t_in);
+            if (!ok) {
+                if (ok_next) {
+                    f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
+                    f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
+                }
+                ok = ok_next;
+                continue;
+            }
+            tok = (unit0 + k) * DEC_UNIT;
+            inner = tok >= all_lo && tok + DEC_UNIT - 1 <= all_hi;
+            // V exponents (own: tokens g, g + 8, blocks VB j ..): inside the window?  vs - (anchor - 8) of both tokens at once (a
+            // borrow between them comes with a low half that is outside); only when that says no, token by token.
+            auto seen = [&](int e) { const int t = tok + g + 8 * e; return t <= any_hi && t >= any_lo; };
+            if (anchor == 0) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int c = 0; c < Frag::VB; c++) top = max(top, max(seen(0) ? f.vs[c] & 0xffff : 0u, seen(1) ? f.vs[c] >> 16 : 0u));
+                anchor = (int)__reduce_max_sync(0xffffffffu, top);
+            }
+            constexpr uint32_t WIDTH2 = (DEC_WIN_LO + DEC_WIN_HI) * 0x10001u;
+            uint32_t d[Frag::VB], far = 0;
+#pragma unroll
+            for (int c = 0; c < Frag::VB; c++) {
+                d[c] = f.vs[c] - (uint32_t)(anchor - DEC_WIN_LO) * 0x10001u;
+                far |= __vmaxu2(d[c], WIDTH2) ^ WIDTH2;
+            }
+            if (__any_sync(0xffffffffu, far != 0)) {
+                bool out = false;
+#pragma unroll
+                for (int c = 0; c < Frag::VB; c++) {
+                    const int v0 = f.vs[c] & 0xffff, v1 = f.vs[c] >> 16, e0 = v0 - anchor + DEC_WIN_LO, e1 = v1 - anchor + DEC_WIN_LO;
+                    out |= seen(0) && v0 > 1 && (unsigned)e0 > (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
+                    out |= seen(1) && v1 > 1 && (unsigned)e1 > (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
+                    // (a block of zeros, or a token that no row sees: any finite factor)
+                    d[c] = (uint32_t)min(max(e0, 0), DEC_WIN_LO + DEC_WIN_HI) | (uint32_t)min(max(e1, 0), DEC_WIN_LO + DEC_WIN_HI) << 16;
+                }
+                if (__any_sync(0xffffffffu, out)) break;
+            }
+            __syncwarp();
+            if (NB >= 4 || j < NB) {
+#pragma unroll
+                for (int c = 0; c < Frag::VB; c++) {
+                    // f16 2^(vs - anchor): exponent field vs - anchor + 15
+                    const uint32_t e = (d[c] + (15 - DEC_WIN_LO) * 0x10001u) << 10;
+                    uint16_t *to = sm.sc[warp][g >> 1][Frag::VB * j + c];
+                    to[g & 1] = (uint16_t)e;
+                    to[2 + (g & 1)] = (uint16_t)(e >> 16);
+                }
+            }
+            scores(true);
+            // weights, transposed into the narrow operand: (token 2j, 2j+1 | 2j+8, 2j+9) of row g
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float p[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) p[c] = ex2(s[nt][c] - m[nt][c & 1]);
+                l[nt][0] += p[0] + p[2];
+                l[nt][1] += p[1] + p[3];
+                weights_f16<TERMS>(p, w, nt);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int b2 = 0; b2 < NB / 2; b2++) {
+                uint32_t ev[2][4], od[2][4];
+                v_codes(b2, ev, od);
+#pragma unroll
+                for (int bb = 0; bb < 2; bb++) {
+                    const int b = 2 * b2 + bb;
+                    const uint2 sc = *reinterpret_cast<const uint2 *>(sm.sc[warp][j][b]);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            const float mn = fmaxf(m[nt][c], column_max(fmaxf(s[nt][c], s[nt][c + 2])) - DEC_TOP), f = ex2(m[nt][c] - mn);
-                            l[nt][c] *= f;
-                            m[nt][c] = mn;
-                            if (anchor >= 0) {
+                        for (int t = 0; t < TERMS; t++) {
+                            const uint32_t x0 = hmul2(w[t][nt][0], sc.x), x1 = hmul2(w[t][nt][1], sc.y);
 #pragma unroll
-                                for (int b = 0; b < NB; b++)
-#pragma unroll
-                                    for (int u = 0; u < 2; u++) { o[nt][b][u][c] *= f; o[nt][b][u][c + 2] *= f; }
-                            }
+                            for (int u = 0; u < 2; u++)
+                                mma_f16(o[nt][b][u], ev[0][2 * bb + u], od[0][2 * bb + u], ev[1][2 * bb + u], od[1][2 * bb + u], x0, x1);
                         }
                 }
-                // weights, transposed into the narrow operand: (token 2j, 2j+1 | 2j+8, 2j+9) of row g
-                uint32_t w[TERMS][NT][2];
+            }
+            if (ok_next) f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
+            ok = ok_next;
+        }
+        const bool wide = k < n_mine;
+        if (wide) {
+            // the sums so far count 2^(m + anchor - 127)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    float p[4];
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        p[c] = ex2(s[nt][c] - m[nt][c & 1]);
-                        l[nt][c & 1] += p[c];
+                for (int c = 0; c < 2; c++)
+                    for (int b = g; b < NB; b += 8)
+                        sm.M[warp][b][nt * 8 + 2 * j + c] = m[nt][c] == DEC_NONE ? DEC_NONE : m[nt][c] + (float)(anchor - 127) + DEC_WIDE_TOP;
+            __syncwarp();
+#pragma unroll 1
+            for (bool fresh = true; k < n_mine; k++, fresh = false) {
+                if (!fresh) ok_next = k + 1 < n_mine && page_of(k + 1, reg, t_in);      // (the first group's has been looked up)
+                if (!ok) {
+                    if (ok_next) {
+                        f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
+                        f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
                     }
-                    if (anchor >= 0) weights_f16<TERMS>(p, w, nt);
+                    ok = ok_next;
+                    continue;
                 }
-                __syncwarp();
-                // output: A = V codes, rows dims 4g + 2u (+1), columns tokens
+                tok = (unit0 + k) * DEC_UNIT;
+                inner = tok >= all_lo && tok + DEC_UNIT - 1 <= all_hi;
+                scores(false);
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) l[nt][c & 1] += ex2(s[nt][c] - m[nt][c & 1]);
 #pragma unroll
                 for (int b2 = 0; b2 < NB / 2; b2++) {
-                    uint32_t ev[2][4], od[2][4];       // [token pair j, j + 4][byte: block 2 b2 codes 0/1, 2/3, block 2 b2 + 1 codes ...]
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const uint32_t A = cur.v[h][b2], B = cur.v[h][NB / 2 + b2];
-                        e2m1x8_to_f16x2((A & 0x0f0f0f0fu) | ((B << 4) & 0xf0f0f0f0u), ev[h]);
-                        e2m1x8_to_f16x2(((A >> 4) & 0x0f0f0f0fu) | (B & 0xf0f0f0f0u), od[h]);
-                    }
+                    uint32_t ev[2][4], od[2][4];
+                    v_codes(b2, ev, od);
 #pragma unroll
                     for (int bb = 0; bb < 2; bb++) {
                         const int b = 2 * b2 + bb;
-                        uint2 sc = make_uint2(0x3c003c00u, 0x3c003c00u);
-                        if (anchor >= 0) {
-                            sc = *reinterpret_cast<const uint2 *>(sm.sc[warp][j][b]);
-                        } else {
-                            // weights of this block alone: 2^(S + vs - M), M per row and block
-                            const float v0 = (float)__shfl_sync(0xffffffffu, (int)(cur.vs[0] >> (8 * (b % Frag::VB))) & 0xff, (lane & 28) | (b / Frag::VB)) - 127.f;
-                            const float v1 = (float)__shfl_sync(0xffffffffu, (int)(cur.vs[1] >> (8 * (b % Frag::VB))) & 0xff, (lane & 28) | (b / Frag::VB)) - 127.f;
-#pragma unroll
-                            for (int nt = 0; nt < NT; nt++) {
-                                float p[4];
-#pragma unroll
-                                for (int c = 0; c < 2; c++) {
-                                    float *Mp = &sm.M[warp][b][nt * 8 + 2 * j + c];
-                                    const float x0 = s[nt][c] + v0, x1 = s[nt][c + 2] + v1, M0 = *Mp;
-                                    float M = M0;
-                                    const float t = column_max(fmaxf(x0, x1));
-                                    if (t > M + (DEC_WIDE_MAX - DEC_WIDE_TOP)) {
-                                        const float f = ex2(M - t);
-                                        M = t;
-                                        o[nt][b][0][c] *= f; o[nt][b][0][c + 2] *= f;
-                                        o[nt][b][1][c] *= f; o[nt][b][1][c + 2] *= f;
-                                    }
-                                    __syncwarp();
-                                    if (g == 0) *Mp = M;
-                                    p[c] = ex2(x0 - (M - DEC_WIDE_TOP));
-                                    p[c + 2] = ex2(x1 - (M - DEC_WIDE_TOP));
-                                }
-                                weights_f16<TERMS>(p, w, nt);
-                            }
-                        }
+                        wide_weights<DH, NT, TERMS, Frag::VB>(sm.M[warp], f.vs, s, w, o, b, lane);
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                            for (int t = 0; t < TERMS; t++) {
-                                const uint32_t x0 = hmul2(w[t][nt][0], sc.x), x1 = hmul2(w[t][nt][1], sc.y);
+                            for (int t = 0; t < TERMS; t++)
 #pragma unroll
                                 for (int u = 0; u < 2; u++)
-                                    mma_f16(o[nt][b][u], ev[0][2 * bb + u], od[0][2 * bb + u], ev[1][2 * bb + u], od[1][2 * bb + u], x0, x1);
-                            }
+                                    mma_f16(o[nt][b][u], ev[0][2 * bb + u], od[0][2 * bb + u], ev[1][2 * bb + u], od[1][2 * bb + u], w[t][nt][0], w[t][nt][1]);
                     }
                 }
+                if (ok_next) f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
+                ok = ok_next;
             }
-            cur = nxt;
-            cur_ok = nxt_ok;
         }
 
         // ---- the warps' shares into one result
@@ -440,8 +528,8 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                 float f[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    const float ref = anchor >= 0 ? m[nt][c] : sm.M[warp][b][nt * 8 + 2 * j + c];
-                    f[c] = exp2f((ref - ma2[c]) + ((anchor >= 0 ? (float)(anchor - 127) : -DEC_WIDE_TOP) - lg[c]));
+                    const float ref = wide ? sm.M[warp][b][nt * 8 + 2 * j + c] : m[nt][c];
+                    f[c] = exp2f((ref - ma2[c]) + ((wide ? -DEC_WIDE_TOP : (float)(anchor - 127)) - lg[c]));
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
@@ -485,7 +573,7 @@ template <int DH, int NT, bool F32>
 static int run(const AttnArgs &a, int all, void *ws, cudaStream_t st) {
     static bool attr_done[MAX_DEVICES] = {false};
     static int occ[MAX_DEVICES] = {0};
-    const int smem = sizeof(DecSmem<DH, NT>), dev = current_device();
+    const int smem = sizeof(DecSmem<DH, NT, F32 ? 2 : 1>), dev = current_device();
     int rc;
     if (dev < 0) return Q36_MOE_EINVAL;
     if ((rc = ensure_smem_attr((const void *)k_attn_decode<DH, NT, F32>, smem, attr_done))) return rc;

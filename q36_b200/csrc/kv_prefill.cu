@@ -633,7 +633,7 @@ static int run_prefill(const AttnArgs &a, void *ws, cudaStream_t st) {
     static bool attr_done[MAX_DEVICES] = {false};
     int rc;
     if ((rc = ensure_smem_attr((const void *)k_attn_prefill<DH>, C::SMEM, attr_done))) return rc;
-    const int grid = sm_count();
+    const int grid = min(sm_count(), 256);      // (the join keeps a weight per piece)
     AttnPart *desc = (AttnPart *)ws;
     float *part = (float *)((uint8_t *)ws + attn_desc_bytes(grid));
     launch_k(k_attn_prefill<DH>, dim3(grid), dim3(PF_THREADS), C::SMEM, st, a, desc, part);

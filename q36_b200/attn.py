@@ -70,10 +70,14 @@ def _is_bf16(t, what) -> int:
     return 0
 
 
+# the current stream's handle without a Stream object around it (3 us of a call that takes 10)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 @contextlib.contextmanager
 def _on_device(dev, stream):
     with torch.cuda.device(dev), torch.cuda.stream(stream):
-        yield torch.cuda.current_stream(dev).cuda_stream
+        yield _raw_stream(dev)
 
 
 class _Here:
@@ -96,7 +100,7 @@ def _call(dev: int, stream=None):
     if dev < 0:
         _refuse("operands not on a CUDA device")
     if stream is None and dev == torch.cuda.current_device():
-        return _Here(torch.cuda.current_stream().cuda_stream)
+        return _Here(_raw_stream(dev))
     return _on_device(dev, stream)
 
 

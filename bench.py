@@ -62,6 +62,7 @@ def parse():
     ap.add_argument("-p", dest="pp", default="512,2048,4096", help="--table: prefill sizes")
     ap.add_argument("-n", dest="tg", type=int, default=128, help="--table: decode steps per repetition")
     ap.add_argument("-r", dest="reps", type=int, default=3, help="--table: repetitions")
+    ap.add_argument("-d", dest="depth", default="", help="--table: also the attention half of every layer, behind this many cached tokens (comma separated)")
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--no-config3", action="store_true", help="skip the fixed-batch line (64 tokens in all, split over the ranks)")
     ap.add_argument("--no-roofline", action="store_true")
@@ -783,6 +784,62 @@ def run_prefill_stack(args):
             sys.exit(3)
 
 
+def attn_stack(torch, moe, layers, T, depth, dev):
+    """One CUDA graph of the layers with their attention halves: T new tokens of one request behind `depth` cached ones.  Every layer
+    appends its rows to a 4-bit cache of its own, attends (16 heads of 128 on 2 kv heads), projects into the residual stream and
+    runs the MoE block on it.  Projections of q, k and v are not part of it: they come as random rows."""
+    from q36_b200 import attn
+    HQ, HKV, DH, BS = 16, 2, 128, 64
+    D = layers[0].D
+    g = torch.Generator(device=dev)
+    g.manual_seed(11)
+    rnd = lambda *s: torch.randn(s, device=dev, generator=g)  # noqa: E731
+    n_blocks = (depth + T + BS - 1) // BS
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    held = (depth + BS - 1) // BS
+    ids = torch.randperm(n_blocks, device=dev, generator=g).int()
+    table = torch.full((1, n_blocks), -1, dtype=torch.int32, device=dev)
+    table[0, :held] = ids[:held]
+    caches = [attn.KVCache(n_blocks, BS, HKV, DH, device=dev) for _ in layers]
+    if depth:
+        pos = torch.arange(depth, device=dev)
+        slots = (table[0, (pos // BS)] * BS + pos % BS).int()
+        for c in caches:
+            c.append(rnd(depth, HKV, DH).bfloat16(), rnd(depth, HKV, DH).bfloat16(), slots)
+    q, k, v = rnd(T, HQ, DH).bfloat16(), rnd(T, HKV, DH).bfloat16(), rnd(T, HKV, DH).bfloat16()
+    w_o = [(rnd(D, HQ * DH) / (HQ * DH) ** 0.5).bfloat16() for _ in layers]
+    router, ones, h0 = rnd(layers[0].E + 1, D) * 0.02, torch.ones(D, device=dev), rnd(T, D)
+    old, new, free, head = i32([depth]), i32([T]), ids[held:].contiguous(), i32([0])
+    h = h0.clone()
+    tables = attn.kv_tables(old, new, BS, free, head, table, T, n_blocks=n_blocks)
+
+    def step():
+        h.copy_(h0)
+        attn.kv_tables(old, new, BS, free, head, table, T, n_blocks=n_blocks, out=tables)
+        for layer, cache, w in zip(layers, caches, w_o):
+            cache.block(q, k, v, tables.slots, table, tables.cu_q, tables.kv_len, T, w, h)
+            layer.block(h, None, ones, router, ones)
+
+    side = torch.cuda.Stream(dev)
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+
+    def check():
+        attn.check_device_status(dev)
+        for layer in layers:
+            layer.check_device_status()
+        if int(tables.status):
+            raise RuntimeError("the step's tables report an unserved request")
+
+    for _ in range(3):
+        graph.replay()
+    return graph.replay, check
+
+
 def run_table(args):
     """The caller loop around the layer stack, reported the way the engine's own harness reports a model
     (bench.c:306-335: `pp<N>` = N prompt tokens through the stack once, `tg<N>` = N single-token steps, each mean
@@ -828,6 +885,19 @@ def run_table(args):
     st = stack_for(1)
     m, sd = rates(st, args.tg, args.tg)
     print(f"| {name} | tg{args.tg} | {m:.1f} \u00b1 {sd:.1f} |", flush=True)
+    for depth in [int(x) for x in args.depth.split(",") if x]:
+        for T, calls, label in [(int(x), 1, f"pp{x}") for x in args.pp.split(",") if x] + [(1, args.tg, f"tg{args.tg}")]:
+            run, check = attn_stack(torch, moe, layers, T, depth, dev)
+            out = []
+            for _ in range(max(1, args.reps)):
+                torch.cuda.synchronize()
+                t0 = time.perf_counter()
+                for _ in range(calls):
+                    run()
+                torch.cuda.synchronize()
+                out.append(calls * T / (time.perf_counter() - t0))
+            check()
+            print(f"| {name} + attention | {label} @ d{depth} | {statistics.fmean(out):.1f} \u00b1 {statistics.stdev(out) if len(out) > 1 else 0.0:.1f} |", flush=True)
     print("\n| batch B | step ms | vs B=1 |\n|---|---:|---:|")
     t1 = None
     for B in (1, 2, 4, 8, 16, 32):

@@ -118,6 +118,16 @@ int q36_attn_block(const void *q, const void *k, const void *v, int x_is_bf16, i
                    const int *kv_len, int n_seq, float scale, int window, const void *w_o, const float *bias_o, float *h,
                    int D, int T, int max_q, void *ws, uint64_t ws_bytes, void *stream);
 
+/* The long waits of the tensor core kernels (on a copy, on a product) are bounded.
+ * Synchronises the stream and returns Q36_MOE_EDEVICE when one gave up on the
+ * current device since the last call of this function (results written since then
+ * are not to be used; which one: q36_moe_last_cuda_error()), else 0.  One check
+ * covers every call before it, as q36_moe_ws_status does. */
+int q36_attn_status(void *stream);
+/* A 32-thread kernel that waits for what nobody completes, with a short limit, and
+ * records that it gave up: lets a test see q36_attn_status report it. */
+int q36_attn_selftest_wait_timeout(void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -29,6 +29,7 @@ _SIGS = {
     "q36_attn_block": (i32, [vp, vp, vp, i32, i64, i64, i64, vp, vp, i32, i32, i32, i32, i32, vp, i32, vp, vp, i32, f32, i32, vp, vp, vp, i32,
                              i32, i32, vp, u64, vp]),
 }
+_SIGS["q36_attn_status"] = _SIGS["q36_attn_selftest_wait_timeout"] = (i32, [vp])
 for _n, (_r, _a) in _SIGS.items():
     _f = getattr(lib, _n)
     _f.restype, _f.argtypes = _r, _a
@@ -125,6 +126,12 @@ def _rows3(t, h, d, what) -> int:
 
 def kv_block_bytes(block_size: int, n_kv_head: int, head_dim: int) -> int:
     return int(lib.q36_kv_block_bytes(block_size, n_kv_head, head_dim))
+
+
+def check_device_status(device=None) -> None:
+    """Raises when a bounded wait of the attention or product kernels gave up on the device since the last check."""
+    with torch.cuda.device(device):
+        check(lib.q36_attn_status(torch.cuda.current_stream().cuda_stream), "attn device status")
 
 
 class Tables(NamedTuple):

@@ -161,8 +161,9 @@ int launch_decode(const AttnArgs &a, int rows, int all, void *ws, cudaStream_t s
 uint64_t decode_ws_bytes(int Dh, int rows);
 int launch_prefill(const AttnArgs &a, void *ws, cudaStream_t st);
 uint64_t prefill_ws_bytes(int Dh);
-int prefill_wait_status(int *out, cudaStream_t st);
-int linear_wait_status(int *out, cudaStream_t st);
+int prefill_wait_status(int *out);
+int linear_wait_status(int *out);
+int launch_prefill_wait_timeout(cudaStream_t st);
 int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st);
 
 }  // namespace q36

@@ -297,4 +297,14 @@ int q36_attn_block(const void *q, const void *k, const void *v, int x_is_bf16, i
     return launch_linear(a.out, K, w_o, bias_o, Q36_ACT_NONE, h, 0, D, h, 0, D, T, D, K, cu_q + n_seq, st);
 }
 
+int q36_attn_status(void *stream) {
+    int where[2] = {0, 0}, rc;
+    if (cudaStreamSynchronize((cudaStream_t)stream) != cudaSuccess) return check_launch();
+    if ((rc = prefill_wait_status(&where[0])) || (rc = linear_wait_status(&where[1]))) return rc;
+    if (!where[0] && !where[1]) return Q36_MOE_OK;
+    last_cuda_error() = where[0] ? 300000 + where[0] : 400000 + where[1];
+    return Q36_MOE_EDEVICE;
+}
+int q36_attn_selftest_wait_timeout(void *stream) { return launch_prefill_wait_timeout((cudaStream_t)stream); }
+
 }  // extern "C"

@@ -650,10 +650,31 @@ int launch_prefill(const AttnArgs &a, void *ws, cudaStream_t st) {
     return a.kv.Dh == 128 ? run_prefill<128>(a, ws, st) : run_prefill<256>(a, ws, st);
 }
 
-// Where a bounded wait gave up since the process began (0: nowhere).
-int prefill_wait_status(int *out, cudaStream_t st) {
-    if (cudaMemcpyFromSymbolAsync(out, g_prefill_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess) return check_launch();
-    return cudaStreamSynchronize(st) == cudaSuccess ? Q36_MOE_OK : check_launch();
+// Where a bounded wait gave up (0: nowhere) since this was last asked, on the current device; the stream has been synchronised.
+int prefill_wait_status(int *out) {
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(out, g_prefill_status, sizeof(int)) != cudaSuccess) return check_launch();
+    if (*out && cudaMemcpyToSymbol(g_prefill_status, &zero, sizeof(int)) != cudaSuccess) return check_launch();
+    return Q36_MOE_OK;
+}
+
+// Waits for a barrier that nobody completes, 1024 polls, and records it as the roles above do.
+__global__ void k_prefill_wait_timeout() {
+    Q36_GDS();
+    __shared__ uint64_t bar;
+    __shared__ volatile int abort_flag;
+    if (threadIdx.x == 0) {
+        abort_flag = 0;
+        mbar_init(smem_u32(&bar), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) mbar_wait(smem_u32(&bar), 0, &abort_flag, &g_prefill_status, 0xA00, 1024u);
+    __syncthreads();
+}
+int launch_prefill_wait_timeout(cudaStream_t st) {
+    launch_k(k_prefill_wait_timeout, dim3(1), dim3(32), 0, st);
+    return check_launch();
 }
 
 }  // namespace q36

@@ -444,10 +444,12 @@ int launch_linear(const void *x, long long xs, const void *w, const float *bias,
     return run_tc<256, 1>(maps, e, T, N, K, rows_used, st);
 }
 
-// Where a bounded wait of the tile kernel gave up since the process began (0: nowhere).
-int linear_wait_status(int *out, cudaStream_t st) {
-    if (cudaMemcpyFromSymbolAsync(out, g_linear_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st) != cudaSuccess) return check_launch();
-    return cudaStreamSynchronize(st) == cudaSuccess ? Q36_MOE_OK : check_launch();
+// Where a bounded wait gave up (0: nowhere) since this was last asked, on the current device; the stream has been synchronised.
+int linear_wait_status(int *out) {
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(out, g_linear_status, sizeof(int)) != cudaSuccess) return check_launch();
+    if (*out && cudaMemcpyToSymbol(g_linear_status, &zero, sizeof(int)) != cudaSuccess) return check_launch();
+    return Q36_MOE_OK;
 }
 
 }  // namespace q36

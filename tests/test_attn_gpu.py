@@ -331,6 +331,29 @@ def test_max_q_chooses_kernels_only(attn):
         s.check(s.run())
 
 
+@pytest.mark.parametrize("heads,Dh", [((16, 2), 128), ((16, 2), 256), ((12, 4), 64), ((24, 2), 128)])
+def test_pieces_of_several_spans_on_one_cta(attn, heads, Dh):
+    """Prompts long enough that every CTA goes through pieces of several row tiles, some of them with one half empty: no wait
+    may give up, twice the same bits, and the rows of the request that the host can afford to check against 64 bits."""
+    import torch
+    rng = np.random.default_rng(10)
+    s = Setup(attn, rng, [(2100, 2600), (130, 9000), (1400, 1400), (1, 600), (300, 4000)], *heads, Dh, 64, "bf16")
+    a, b = s.run(), s.run()
+    attn.check_device_status()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    s.check(a, rows=[1, 3, 4])
+
+
+def test_a_wait_that_gives_up_is_reported_once(attn, moe):
+    import torch
+    st = torch.cuda.current_stream().cuda_stream
+    assert attn.lib.q36_attn_status(st) == moe.OK
+    assert attn.lib.q36_attn_selftest_wait_timeout(st) == moe.OK
+    with pytest.raises(attn.MoEError):
+        attn.check_device_status()
+    attn.check_device_status()
+
+
 def test_same_bits_twice_on_two_streams_and_from_a_graph(attn):
     """Two calls at once on two streams, a captured and replayed one, and the same call again: the same bits."""
     import torch

@@ -12,13 +12,13 @@ constexpr int TB_MAX_SEQ = 16384;
 // that no lengths overflow them.  Every CTA makes the sums for itself: 16 KB of lengths at 2000 requests come out of L2 in
 // less time than a second launch takes.
 struct TbReq { int rows, need, ok; };
-__device__ __forceinline__ TbReq tb_request(int old, int q, int bs, int max_blocks, int row_cap, int blk_cap, int &flags) {
+__device__ __forceinline__ TbReq tb_request(int old, int q, int log_bs, int max_blocks, int row_cap, int blk_cap, int &flags) {
     TbReq r;
     r.ok = 1;
     r.rows = min(max(q, 0), row_cap);
     r.need = 0;
     if (old < 0 || q < 0) { flags |= 4; r.ok = 0; return r; }
-    const long long held = ((long long)old + bs - 1) / bs, all = ((long long)old + q + bs - 1) / bs;
+    const long long last = (1 << log_bs) - 1, held = (old + last) >> log_bs, all = ((long long)old + q + last) >> log_bs;
     if (all > max_blocks) { flags |= 2; r.ok = 0; return r; }
     r.need = (int)min(all - held, (long long)blk_cap);
     return r;
@@ -36,21 +36,21 @@ __device__ __forceinline__ int bisect(const int *pre, int n, int v) {
 }
 
 __global__ void __launch_bounds__(TB_THREADS)
-k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int bs, int n_blocks, const int *__restrict__ free_blocks,
+k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int log_bs, int n_blocks, const int *__restrict__ free_blocks,
             int n_free, const int *free_head, int *block_table, int max_blocks, int *__restrict__ cu_q, int *kv_len,
             int *__restrict__ slots, int *__restrict__ positions, int T, int *free_head_out, int *status) {
     Q36_GDS();
     extern __shared__ int sm[];
     int *pre_r = sm, *pre_b = sm + B + 1;     // exclusive prefix sums; entry B: the total
     __shared__ int wr[TB_THREADS / 32], wb[TB_THREADS / 32], fl;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bs = 1 << log_bs;
     const int head = min(max(*free_head, 0), n_free), avail = n_free - head;
     const int row_cap = T + 1, blk_cap = avail + 1;
     if (tid == 0) fl = 0;
     const int per = (B + TB_THREADS - 1) / TB_THREADS, b0 = min(tid * per, B), b1 = min(b0 + per, B);
     int flags = 0, sr = 0, sb = 0;
     for (int b = b0; b < b1; b++) {
-        const TbReq r = tb_request(kv_old[b], q_len[b], bs, max_blocks, row_cap, blk_cap, flags);
+        const TbReq r = tb_request(kv_old[b], q_len[b], log_bs, max_blocks, row_cap, blk_cap, flags);
         pre_r[b] = sr;
         pre_b[b] = sb;
         sr = sat_add(sr, r.rows, row_cap);
@@ -79,9 +79,9 @@ k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int bs, int
     for (int i = first; i < min(total_new, avail); i += stride) {
         const int b = bisect(pre_b, B, i);
         const int old = kv_old[b];
-        const TbReq r = tb_request(old, q_len[b], bs, max_blocks, row_cap, blk_cap, dummy);
+        const TbReq r = tb_request(old, q_len[b], log_bs, max_blocks, row_cap, blk_cap, dummy);
         if (!served(b, r)) continue;
-        const int held = (old + bs - 1) / bs;
+        const int held = (old + bs - 1) >> log_bs;
         block_table[(size_t)b * max_blocks + held + (i - pre_b[b])] = free_blocks[head + i];
     }
     // rows; a row's block is an old table entry or a free-list entry (the table's new entries may not be written yet)
@@ -90,12 +90,12 @@ k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int bs, int
         if (t < total_rows) {
             const int b = bisect(pre_r, B, t);
             const int old = kv_old[b];
-            const TbReq r = tb_request(old, q_len[b], bs, max_blocks, row_cap, blk_cap, dummy);
+            const TbReq r = tb_request(old, q_len[b], log_bs, max_blocks, row_cap, blk_cap, dummy);
             if (served(b, r)) {
                 pos = old + (t - pre_r[b]);
-                const int held = (old + bs - 1) / bs, col = pos / bs;
+                const int held = (old + bs - 1) >> log_bs, col = pos >> log_bs;
                 const int blk = col < held ? block_table[(size_t)b * max_blocks + col] : free_blocks[head + pre_b[b] + (col - held)];
-                if (blk >= 0 && blk < n_blocks) slot = blk * bs + pos % bs;
+                if (blk >= 0 && blk < n_blocks) slot = blk * bs + (pos & (bs - 1));
             }
         }
         slots[t] = slot;
@@ -108,7 +108,7 @@ k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int bs, int
         int used = 0;
         for (int b = tid; b < B; b += TB_THREADS) {
             const int old = kv_old[b], q = q_len[b];
-            const TbReq r = tb_request(old, q, bs, max_blocks, row_cap, blk_cap, flags);
+            const TbReq r = tb_request(old, q, log_bs, max_blocks, row_cap, blk_cap, flags);
             const bool s = served(b, r);
             if (r.ok && r.need > 0 && pre_b[b] + r.need > avail) flags |= 1;
             if (r.rows > 0 && pre_r[b + 1] > T) flags |= 8;
@@ -149,21 +149,15 @@ __device__ __forceinline__ uint32_t f32x8_to_e2m1(const float (&v)[8]) {
     return r;
 }
 constexpr int KVC_THREADS = 256;
-// Four lanes per 32-element block, eight elements each: a row is read and its K codes are written in whole sectors.
-// blockIdx.y: 0 K, 1 V.
-__global__ void __launch_bounds__(KVC_THREADS)
-k_kv_append(const void *__restrict__ k, const void *__restrict__ v, int bf16, long long ks, long long vs, const int *__restrict__ slots,
-            KvGeom g, long long n8) {
-    Q36_GDS();
-    const long long i = (long long)blockIdx.x * KVC_THREADS + threadIdx.x;
-    const bool is_v = blockIdx.y;
-    const int row8 = g.Hkv * g.Dh / 8;
-    const bool in = i < n8;
-    const int t = in ? (int)(i / row8) : 0, r = in ? (int)(i - (long long)t * row8) : 0;
-    const int head = r / (g.Dh / 8), c = r - head * (g.Dh / 8), b = c >> 2, j = c & 3;
-    const int slot = in ? slots[t] : -1;
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (slot >= 0) load8(is_v ? v : k, (size_t)t * (is_v ? vs : ks) + (size_t)r * 8, bf16, x);
+// A thread's eight dims of a row of K and of V: token t, kv head, scale block b, quarter j of it.  Four lanes share a block, so that rows
+// are read and K codes written in whole sectors.
+struct RowPart { int t, head, b, j, r; };
+__device__ __forceinline__ RowPart row_part(const KvGeom &g, unsigned i) {
+    const unsigned row8 = g.Hkv * g.Dh / 8, head8 = g.Dh / 8, t = i / row8, r = i - t * row8, head = r / head8, c = r - head * head8;
+    return RowPart{(int)t, (int)head, (int)(c >> 2), (int)(c & 3), (int)r};
+}
+// eight values, and the whole block's largest magnitude's exponent -> codes; NaN counts as 0
+__device__ __forceinline__ uint32_t quant8(float (&x)[8], int &e2) {
     float am = 0.f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -172,46 +166,38 @@ k_kv_append(const void *__restrict__ k, const void *__restrict__ v, int bf16, lo
     }
     am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 1));
     am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, 2));
-    if (slot < 0 || (slot >> g.log_bs) >= g.n_blocks) return;
-    const int e2 = e2_of_amax_fp4(am);
+    e2 = e2_of_amax_fp4(am);
     const float inv = inv_scale_of_e2(e2);
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] *= inv;
-    const uint32_t codes = f32x8_to_e2m1(x);
-    uint8_t *reg = const_cast<uint8_t *>(g.at(slot >> g.log_bs, head));
-    const int tok = slot & (g.bs - 1), half = g.bs * g.Dh / 2;
-    if (!is_v) {
-        *reinterpret_cast<uint32_t *>(reg + kv_k_off(tok, j, b, g.Dh)) = codes;
-    } else {
-        *reinterpret_cast<uint16_t *>(reg + half + kv_v_off(tok, 2 * j, b, g.Dh)) = (uint16_t)codes;
-        *reinterpret_cast<uint16_t *>(reg + half + kv_v_off(tok, 2 * j + 1, b, g.Dh)) = (uint16_t)(codes >> 16);
+    return f32x8_to_e2m1(x);
+}
+__global__ void __launch_bounds__(KVC_THREADS)
+k_kv_append(const void *__restrict__ k, const void *__restrict__ v, int bf16, long long ks, long long vs, const int *__restrict__ slots, KvGeom g,
+            unsigned n8) {
+    Q36_GDS();
+    const unsigned i = blockIdx.x * KVC_THREADS + threadIdx.x;
+    const RowPart p = row_part(g, min(i, n8 - 1));
+    const int slot = i < n8 ? slots[p.t] : -1, block = slot >> g.log_bs;
+    const bool put = slot >= 0 && block < g.n_blocks;
+    float x[8] = {}, y[8] = {};
+    if (put) {
+        load8(k, (size_t)p.t * ks + (size_t)p.r * 8, bf16, x);
+        load8(v, (size_t)p.t * vs + (size_t)p.r * 8, bf16, y);
     }
-    if (j == 0) reg[2 * half + (is_v ? g.bs * (g.Dh / 32) : 0) + tok * (g.Dh / 32) + b] = (uint8_t)(127 + e2);
+    int ek, ev;
+    const uint32_t kc = quant8(x, ek), vc = quant8(y, ev);
+    if (!put) return;
+    uint8_t *reg = const_cast<uint8_t *>(g.at(block, p.head));
+    const int tok = slot & (g.bs - 1), half = g.bs * g.Dh / 2, nb = g.Dh / 32;
+    *reinterpret_cast<uint32_t *>(reg + kv_k_off(tok, p.j, p.b, g.Dh)) = kc;
+    *reinterpret_cast<uint16_t *>(reg + half + kv_v_off(tok, 2 * p.j, p.b, g.Dh)) = (uint16_t)vc;
+    *reinterpret_cast<uint16_t *>(reg + half + kv_v_off(tok, 2 * p.j + 1, p.b, g.Dh)) = (uint16_t)(vc >> 16);
+    if (p.j == 0) reg[2 * half + tok * nb + p.b] = (uint8_t)(127 + ek);
+    if (p.j == 1) reg[2 * half + (g.bs + tok) * nb + p.b] = (uint8_t)(127 + ev);
 }
 
-__global__ void __launch_bounds__(KVC_THREADS)
-k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *__restrict__ v, int bf16, long long n8) {
-    Q36_GDS();
-    const long long i = (long long)blockIdx.x * KVC_THREADS + threadIdx.x;
-    if (i >= n8) return;
-    const bool is_v = blockIdx.y;
-    const int row8 = g.Hkv * g.Dh / 8;
-    const int t = (int)(i / row8), r = (int)(i - (long long)t * row8);
-    const int head = r / (g.Dh / 8), c = r - head * (g.Dh / 8), b = c >> 2, j = c & 3;
-    const int slot = slots[t];
-    uint32_t codes = 0;
-    float sc = 0.f;
-    if (slot >= 0 && (slot >> g.log_bs) < g.n_blocks) {
-        const uint8_t *reg = g.at(slot >> g.log_bs, head);
-        const int tok = slot & (g.bs - 1), half = g.bs * g.Dh / 2;
-        if (!is_v) {
-            codes = *reinterpret_cast<const uint32_t *>(reg + kv_k_off(tok, j, b, g.Dh));
-        } else {
-            codes = *reinterpret_cast<const uint16_t *>(reg + half + kv_v_off(tok, 2 * j, b, g.Dh)) |
-                    (uint32_t)*reinterpret_cast<const uint16_t *>(reg + half + kv_v_off(tok, 2 * j + 1, b, g.Dh)) << 16;
-        }
-        sc = ue8m0_to_f32(reg[2 * half + (is_v ? g.bs * (g.Dh / 32) : 0) + tok * (g.Dh / 32) + b]);
-    }
+__device__ __forceinline__ void store8_exact(void *p, size_t at, int bf16, uint32_t codes, float sc) {
     float x[8];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -219,24 +205,56 @@ k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *_
         x[2 * e] = f.x * sc;
         x[2 * e + 1] = f.y * sc;
     }
-    void *dst = is_v ? v : k;
-    const size_t at = (size_t)i * 8;
     if (bf16) {      // exact: a code has two significant bits
         uint32_t w[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) w[e] = (__float_as_uint(x[2 * e]) >> 16) | (__float_as_uint(x[2 * e + 1]) & 0xffff0000u);
-        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(dst) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint16_t *>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-        float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(dst) + at);
+        float4 *o = reinterpret_cast<float4 *>(reinterpret_cast<float *>(p) + at);
         o[0] = make_float4(x[0], x[1], x[2], x[3]);
         o[1] = make_float4(x[4], x[5], x[6], x[7]);
     }
 }
+__global__ void __launch_bounds__(KVC_THREADS)
+k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *__restrict__ v, int bf16, unsigned n8) {
+    Q36_GDS();
+    const unsigned i = blockIdx.x * KVC_THREADS + threadIdx.x;
+    if (i >= n8) return;
+    const RowPart p = row_part(g, i);
+    const int slot = slots[p.t], block = slot >> g.log_bs;
+    uint32_t kc = 0, vc = 0;
+    float sk = 0.f, sv = 0.f;
+    if (slot >= 0 && block < g.n_blocks) {
+        const uint8_t *reg = g.at(block, p.head);
+        const int tok = slot & (g.bs - 1), half = g.bs * g.Dh / 2, nb = g.Dh / 32;
+        kc = *reinterpret_cast<const uint32_t *>(reg + kv_k_off(tok, p.j, p.b, g.Dh));
+        vc = *reinterpret_cast<const uint16_t *>(reg + half + kv_v_off(tok, 2 * p.j, p.b, g.Dh)) |
+             (uint32_t)*reinterpret_cast<const uint16_t *>(reg + half + kv_v_off(tok, 2 * p.j + 1, p.b, g.Dh)) << 16;
+        sk = ue8m0_to_f32(reg[2 * half + tok * nb + p.b]);
+        sv = ue8m0_to_f32(reg[2 * half + (g.bs + tok) * nb + p.b]);
+    }
+    store8_exact(k, (size_t)i * 8, bf16, kc, sk);
+    store8_exact(v, (size_t)i * 8, bf16, vc, sv);
+}
 
-int launch_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g, int T, cudaStream_t st) {
-    const long long n8 = (long long)T * g.Hkv * g.Dh / 8;
-    launch_k(k_kv_append, dim3((unsigned)((n8 + KVC_THREADS - 1) / KVC_THREADS), 2), dim3(KVC_THREADS), 0, st, k, v, bf16, ks, vs, slots, g, n8);
+// n8 < 2^31: rows are launched in lots of that many parts
+template <typename F>
+static int by_lots(KvGeom g, int T, F launch) {
+    const long long row8 = (long long)g.Hkv * g.Dh / 8;
+    const int lot = (int)min((long long)T, (1ll << 30) / row8);
+    for (int t = 0; t < T; t += lot) {
+        const int n = min(lot, T - t);
+        launch(t, (unsigned)(n * row8), dim3((unsigned)((n * row8 + KVC_THREADS - 1) / KVC_THREADS)));
+    }
     return check_launch();
+}
+int launch_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g, int T, cudaStream_t st) {
+    const int size = bf16 ? 2 : 4;
+    return by_lots(g, T, [&](int t, unsigned n8, dim3 grid) {
+        launch_k(k_kv_append, grid, dim3(KVC_THREADS), 0, st, (const void *)((const uint8_t *)k + (size_t)t * ks * size),
+                 (const void *)((const uint8_t *)v + (size_t)t * vs * size), bf16, ks, vs, slots + t, g, n8);
+    });
 }
 
 }  // namespace q36
@@ -266,8 +284,8 @@ int q36_kv_tables(const int *kv_old, const int *q_len, int n_seq, int block_size
     const long work = (long)T + n_seq;
     // in place: one block, since another could read what it has written
     const bool in_place = kv_len == kv_old || free_head_out == free_head;
-    const int grid = in_place ? 1 : (int)min((work + 2 * TB_THREADS - 1) / (2 * TB_THREADS), (long)sm_count());
-    launch_k(k_kv_tables, dim3(grid), dim3(TB_THREADS), smem, (cudaStream_t)stream, kv_old, q_len, n_seq, block_size, n_blocks, free_blocks, n_free,
+    const int grid = in_place ? 1 : (int)min((work + TB_THREADS - 1) / TB_THREADS, (long)sm_count());
+    launch_k(k_kv_tables, dim3(grid), dim3(TB_THREADS), smem, (cudaStream_t)stream, kv_old, q_len, n_seq, log2_of(block_size), n_blocks, free_blocks, n_free,
              free_head, block_table, max_blocks, cu_q, kv_len, slots, positions, T, free_head_out, status);
     return check_launch();
 }
@@ -289,10 +307,11 @@ int q36_kv_read(const void *cache, int n_blocks, int block_size, int n_kv_head, 
     if (n_blocks <= 0 || (int64_t)n_blocks * block_size > INT32_MAX || off16(k) || off16(v) || off16(cache)) return Q36_MOE_EINVAL;
     if (T == 0) return Q36_MOE_OK;
     const KvGeom g{(const uint8_t *)cache, n_blocks, block_size, log2_of(block_size), n_kv_head, head_dim};
-    const long long n8 = (long long)T * n_kv_head * head_dim / 8;
-    launch_k(k_kv_read, dim3((unsigned)((n8 + KVC_THREADS - 1) / KVC_THREADS), 2), dim3(KVC_THREADS), 0, (cudaStream_t)stream, g, slots, k, v,
-             x_is_bf16, n8);
-    return check_launch();
+    const size_t row = (size_t)n_kv_head * head_dim * (x_is_bf16 ? 2 : 4);
+    return by_lots(g, T, [&](int t, unsigned n8, dim3 grid) {
+        launch_k(k_kv_read, grid, dim3(KVC_THREADS), 0, (cudaStream_t)stream, g, slots + t, (void *)((uint8_t *)k + t * row),
+                 (void *)((uint8_t *)v + t * row), x_is_bf16, n8);
+    });
 }
 
 }  // extern "C"

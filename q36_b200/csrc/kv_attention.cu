@@ -149,37 +149,81 @@ k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ de
     }
 }
 
-// Many rows, few pieces: a warp per row.
+// Tiles of 128 or 256 rows, mostly in two or three pieces: a warp per four rows, so that the loads of all four are on their way at once.
 template <int DH>
 __global__ void __launch_bounds__(JOIN_THREADS)
 k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
     Q36_GDS();
-    constexpr int N4 = (DH + 127) / 128;      // 16-byte pieces of a row per lane
+    constexpr int N4 = (DH + 127) / 128, WARPS = JOIN_THREADS / 32, RB = 4;
     extern __shared__ int list[];
-    __shared__ float w[JOIN_THREADS / 32][JOIN_PIECES];      // (a tile kernel has one CTA per SM)
-    constexpr int WARPS = JOIN_THREADS / 32;
-    const int n = join_list<JOIN_THREADS>(desc, grid, list), lane = threadIdx.x & 31, groups = tile_rows / WARPS;
+    __shared__ float4 w[WARPS][JOIN_PIECES];      // four rows' weights of each piece (a tile kernel has one CTA per SM)
+    const int n = join_list<JOIN_THREADS>(desc, grid, list), lane = threadIdx.x & 31, warp = threadIdx.x >> 5, groups = tile_rows / (WARPS * RB);
     const int stride = attn_part_floats(tile_rows, DH);
     for (int item = blockIdx.x; item < n * groups; item += gridDim.x) {
-        const int cta = list[item / groups] & JOIN_ID, r = item % groups * WARPS + (threadIdx.x >> 5);
+        const int cta = list[item / groups] & JOIN_ID, r = (item % groups * WARPS + warp) * RB;
         const AttnPart d = desc[cta];
         if (r >= d.rows) continue;
-        float m, l, first;
-        float4 o[N4];
-        float *mine = w[threadIdx.x >> 5];
-        join_weights<true>(d, part, cta, stride, r, lane, mine, first, m, l);
-        __syncwarp();
-        join_rows<DH>(d, part, cta, stride, tile_rows, r, lane, 0, 1, [&](int p) { return p < d.parts ? mine[p] : 0.f; }, o);
+        float m[RB], l[RB] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int k = 0; k < N4; k++) join_store<DH>(a, d, r, lane, k, o[k], l);
-        if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
+        for (int i = 0; i < RB; i++) m[i] = -3.0e38f;
+        // (m, l) of the four rows lie side by side
+        for (int p = lane; p < d.parts; p += 32) {
+            const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * r);
+            const float4 x = s[0], y = s[1];
+            m[0] = fmaxf(m[0], x.x); m[1] = fmaxf(m[1], x.z); m[2] = fmaxf(m[2], y.x); m[3] = fmaxf(m[3], y.z);
+        }
+#pragma unroll
+        for (int i = 0; i < RB; i++) m[i] = warp_max(m[i]);
+        for (int p = lane; p < d.parts; p += 32) {
+            const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * r);
+            const float4 x = s[0], y = s[1];
+            const float4 f = make_float4(x.y * exp2f(x.x - m[0]), x.w * exp2f(x.z - m[1]), y.y * exp2f(y.x - m[2]), y.w * exp2f(y.z - m[3]));
+            w[warp][p] = f;
+            l[0] += f.x; l[1] += f.y; l[2] += f.z; l[3] += f.w;
+        }
+#pragma unroll
+        for (int i = 0; i < RB; i++) l[i] = warp_sum(l[i]);
+        __syncwarp();
+        float4 o[RB][N4];
+#pragma unroll
+        for (int i = 0; i < RB; i++)
+#pragma unroll
+            for (int k = 0; k < N4; k++) o[i][k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+        for (int p = 0; p < d.parts; p++) {
+            const float4 f4 = w[warp][p];
+            const float f[RB] = {f4.x, f4.y, f4.z, f4.w};
+            float4 v[RB][N4];
+#pragma unroll
+            for (int i = 0; i < RB; i++) {
+                const float4 *s = reinterpret_cast<const float4 *>(join_slot(part, d, cta, p, stride) + 2 * tile_rows + (r + i) * DH);
+#pragma unroll
+                for (int k = 0; k < N4; k++) v[i][k] = s[32 * k + (DH < 128 ? lane % (DH / 4) : lane)];
+            }
+#pragma unroll
+            for (int i = 0; i < RB; i++) {
+                if (f[i] == 0.f) continue;      // (a piece that saw nothing has no row: what was read is not used)
+#pragma unroll
+                for (int k = 0; k < N4; k++) {
+                    o[i][k].x = fmaf(f[i], v[i][k].x, o[i][k].x); o[i][k].y = fmaf(f[i], v[i][k].y, o[i][k].y);
+                    o[i][k].z = fmaf(f[i], v[i][k].z, o[i][k].z); o[i][k].w = fmaf(f[i], v[i][k].w, o[i][k].w);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < RB; i++) {
+            if (r + i >= d.rows) break;
+#pragma unroll
+            for (int k = 0; k < N4; k++) join_store<DH>(a, d, r + i, lane, k, o[i][k], l[i]);
+            if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r + i, m[i], l[i]);
+        }
         __syncwarp();
     }
 }
 
 int launch_attn_join(const AttnArgs &a, int tile_rows, int grid, const AttnPart *desc, const float *part, cudaStream_t st) {
     if (tile_rows > 16) {
-        const dim3 blocks(14 * sm_count()), threads(JOIN_THREADS);
+        const dim3 blocks(8 * sm_count()), threads(JOIN_THREADS);
         if (a.kv.Dh == 64) launch_k(k_attn_join_rows<64>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
         else if (a.kv.Dh == 128) launch_k(k_attn_join_rows<128>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);
         else launch_k(k_attn_join_rows<256>, blocks, threads, grid * 4, st, a, tile_rows, grid, desc, part);

@@ -601,7 +601,8 @@ uint64_t decode_ws_bytes(int Dh, int rows) {
 
 int launch_decode(const AttnArgs &a, int rows, int all, void *ws, cudaStream_t st) {
     const bool f32 = !a.q_bf16;
-    const int nt = decode_nt(a.kv.Dh, rows);
+    // (beside the tile kernel most of what is left has one new token)
+    const int nt = all ? decode_nt(a.kv.Dh, rows) : 1;
     if (a.kv.Dh == 64) {
         if (nt == 1) return f32 ? run<64, 1, true>(a, all, ws, st) : run<64, 1, false>(a, all, ws, st);
         return f32 ? run<64, 2, true>(a, all, ws, st) : run<64, 2, false>(a, all, ws, st);

@@ -23,7 +23,7 @@
  *            holds dims 32b + 8j .. 32b + 8j + 7, low nibble first (j < 4)
  *   V codes: token pair t/2, group g of 8, token t%2: halfword b of head_dim/32
  *            holds dims 32b + 4g .. 32b + 4g + 3, low nibble first
- *   scales:  [token][head_dim/32]
+ *   scales:  [token][head_dim/32], 1 .. 252 (what the writer makes)
  * The order inside a row is the one in which the lanes of a warp hold a tensor
  * core operand, so that attention reads a row with full-width loads.
  * A slot is block * block_size + offset; offsets into the cache are 64-bit. */
@@ -56,7 +56,8 @@ uint64_t q36_kv_block_bytes(int block_size, int n_kv_head, int head_dim);
  * gives zeros for its rows) and its slots are -1.  When the free list is too
  * short, the requests behind the first unserved one that need blocks are not
  * served either.  Block ids outside [0, n_blocks) give slot -1.
- * n_seq <= 16384; n_blocks * block_size < 2^31. */
+ * 1 <= n_seq <= 16384; T, n_free <= 2^29; n_blocks * block_size < 2^31;
+ * max_blocks * block_size <= 2^30.  The outputs may not overlap the inputs but as said. */
 int q36_kv_tables(const int *kv_old, const int *q_len, int n_seq, int block_size, int n_blocks, const int *free_blocks,
                   int n_free, const int *free_head, int *block_table, int max_blocks, int *cu_q, int *kv_len, int *slots,
                   int *positions, int T, int *free_head_out, int *status, void *stream);
@@ -75,7 +76,7 @@ int q36_kv_read(const void *cache, int n_blocks, int block_size, int n_kv_head, 
                 void *v, int x_is_bf16, int T, void *stream);
 
 /* Attention of q [T][n_head][head_dim] over the cache.  The rows of request b are
- * cu_q[b] .. cu_q[b+1]; with n = cu_q[b+1] - cu_q[b] its row i has position
+ * cu_q[b] .. cu_q[b+1], cu_q[0] = 0; with n = cu_q[b+1] - cu_q[b] its row i has position
  * p = kv_len[b] - n + i and sees the cached tokens j with p - window < j <= p
  * (window 0: all j <= p).  Query head h reads kv head h / (n_head / n_kv_head).
  * out [T][n_head][head_dim] has the type of q; lse (or NULL) [T][n_head] f32
@@ -85,7 +86,8 @@ int q36_kv_read(const void *cache, int n_blocks, int block_size, int n_kv_head, 
  * whose id is outside [0, n_blocks) are left out.
  * max_q: the largest number of new tokens of a request, as far as the host
  * knows it; it chooses kernels only, any value >= 1 gives right results.
- * n_head / n_kv_head <= 128, n_head <= 4096, n_seq <= 16384. */
+ * n_head / n_kv_head <= 128, n_head <= 4096, 1 <= n_seq <= 16384, T * n_head <= 2^30.
+ * f32 prompts run on the kernel for few rows: right at every length, a fifth of bf16's rate. */
 uint64_t q36_kv_attention_workspace_bytes(int n_head, int n_kv_head, int head_dim, int max_q);
 int q36_kv_attention(const void *q, int x_is_bf16, int64_t q_stride, const void *cache, int n_blocks, int block_size,
                      int n_head, int n_kv_head, int head_dim, const int *block_table, int max_blocks, const int *cu_q,
@@ -102,7 +104,7 @@ int q36_kv_attention(const void *q, int x_is_bf16, int64_t q_stride, const void 
  * bf16; strides between rows in elements.  Sums in f32, one rounding at the end.
  * residual may be y itself (same type and stride).  rows_used (or NULL): device
  * count of rows; rows of y from *rows_used on are left as they were.  K and
- * x_stride are multiples of 8. */
+ * x_stride are multiples of 8; T, N, K <= 2^30. */
 int q36_linear(const void *x, int64_t x_stride, const void *w, const float *bias, int act, const void *residual,
                int res_is_bf16, int64_t res_stride, void *y, int y_is_bf16, int64_t y_stride, int T, int N, int K,
                const int *rows_used, void *stream);

@@ -157,7 +157,7 @@ def kv_tables(kv_old, q_len, block_size, free_blocks, free_head, block_table, T,
     with _call(dev, stream) as st:
         if out is None:
             out = Tables(*torch.empty(2 * (B + T) + 3, dtype=_I32, device=kv_old.device).split_with_sizes(sizes))
-        rc = lib.q36_kv_tables(kv_old.data_ptr(), q_len.data_ptr(), B, block_size, n_blocks or (2**31 - 1) // block_size, free_blocks.data_ptr(),
+        rc = lib.q36_kv_tables(kv_old.data_ptr(), q_len.data_ptr(), B, block_size, (2**31 - 1) // max(block_size, 1) if n_blocks is None else n_blocks, free_blocks.data_ptr(),
                                free_blocks.numel(), free_head.data_ptr(), block_table.data_ptr(), block_table.shape[1], out.cu_q.data_ptr(),
                                out.kv_len.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(), T, out.free_head.data_ptr(),
                                out.status.data_ptr(), st)
@@ -176,10 +176,14 @@ class KVCache:
         if data is None:
             data = torch.zeros(shape, dtype=_U8, device=device)
         _need(data.shape == shape and data.dtype is _U8 and data.is_contiguous(), "KVCache (data)")
-        self.data, self.device, self._dev = data, data.device, data.get_device()
+        self._data, self.device, self._dev = data, data.device, data.get_device()
         self.n_blocks, self.block_size, self.n_kv_head, self.head_dim = n_blocks, block_size, n_kv_head, head_dim
         self._geom = (data.data_ptr(), n_blocks, block_size)
         self._ws = {}
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
 
     def _scratch(self, nbytes: int, st: int) -> torch.Tensor:
         """Scratch of a call; one per stream, since calls on two streams may run at the same time.  Under capture a graph
@@ -224,6 +228,8 @@ class KVCache:
         B = kv_len.numel()
         if q.dim() != 3 or cu_q.numel() != B + 1 or block_table.dim() != 2 or block_table.shape[0] != B:
             _refuse(f"{what} (q [T, n_head, head_dim], tables)")
+        if not 0 <= window < 2**31:
+            _refuse(f"{what} (window)")
         scale = self.head_dim ** -0.5 if scale is None else scale
         return (*self._geom, q.shape[1], self.n_kv_head, self.head_dim, block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(),
                 kv_len.data_ptr(), B, scale, window)
@@ -241,6 +247,8 @@ class KVCache:
                 _refuse(f"{what} (out)")
             os_ = _rows3(out, h, d, what)
         _on(what, self._dev, out, ws)
+        if ws is not None and not ws.is_contiguous():
+            _refuse(f"{what} (ws)")
         with _call(self._dev, stream) as st:
             if out is None:
                 out = torch.empty((T, h, d), dtype=q.dtype, device=self.device)
@@ -262,6 +270,7 @@ class KVCache:
         _need(k.dtype is q.dtype and v.dtype is q.dtype and k.shape[0] == T and v.shape[0] == T and slots.numel() == T, f"{what} (q, k, v, slots)")
         _need(w_o.dtype is _BF16 and w_o.is_contiguous() and w_o.dim() == 2 and w_o.shape[1] == n_head * self.head_dim, f"{what} (w_o)")
         D = w_o.shape[0]
+        _need(ws is None or ws.is_contiguous(), f"{what} (ws)")
         _need(h.dtype is _F32 and h.is_contiguous() and h.shape == (T, D), f"{what} (h)")
         _need(bias_o is None or (bias_o.dtype is _F32 and bias_o.is_contiguous() and bias_o.shape == (D,)), f"{what} (bias_o)")
         bf, qs = _is_bf16(q, what), _rows3(q, n_head, self.head_dim, what)

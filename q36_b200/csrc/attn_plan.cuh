@@ -43,8 +43,8 @@ __device__ __forceinline__ long long seq_units(const AttnArgs &a, const SeqSpans
 }
 
 // (32 bits nearly always do)
-__device__ __forceinline__ long long div64(long long a, unsigned b) {
-    return a >> 32 ? a / b : (long long)((unsigned)a / b);
+__device__ __forceinline__ long long div64(long long a, long long b) {
+    return (a | b) >> 32 ? a / b : (long long)((unsigned)a / (unsigned)b);
 }
 
 // Moves pos to the span that holds pos.at, from request pos.b (whose first unit is pos.seq_base) on.
@@ -123,7 +123,7 @@ struct AttnPart { int parts, slot, t0, n, hk, row0, rows, pad; };
 
 __device__ __forceinline__ AttnPart plan_parts(const AttnArgs &a, const SpanRule &r, const PlanSeg &g, const PlanPos &pos, int slot) {
     AttnPart p;
-    p.parts = (int)(div64(g.span_base + g.units - 1, (unsigned)pos.per) - blockIdx.x) + 1;
+    p.parts = (int)(div64(g.span_base + g.units - 1, pos.per) - blockIdx.x) + 1;
     p.slot = slot;
     p.t0 = g.t0;
     p.n = g.n;

@@ -258,16 +258,16 @@ int launch_attention(const AttnArgs &a, int max_q, void *ws, uint64_t ws_bytes, 
 using namespace q36;
 
 static bool off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
+static bool off4(const void *p) { return ((uintptr_t)p & 3) != 0; }
 
 // Checks what the attention entries have in common and fills in their arguments.
 static int attn_args(AttnArgs &a, const void *q, int x_is_bf16, int64_t q_stride, const void *cache, int n_blocks, int block_size, int n_head,
                      int n_kv_head, int head_dim, const int *block_table, int max_blocks, const int *cu_q, const int *kv_len, int n_seq,
                      float scale, int window, int T, int max_q) {
     if ((T && !q) || !cache || !block_table || !cu_q || !kv_len || !kv_geom_ok(block_size, n_kv_head, head_dim)) return Q36_MOE_EINVAL;
-    if (n_head <= 0 || n_head % n_kv_head || n_head / n_kv_head > 128 || n_head > 4096 || n_seq <= 0 || n_seq > 16384 || T < 0 || max_q <= 0 || window < 0) return Q36_MOE_EINVAL;
+    if (n_head <= 0 || n_head % n_kv_head || n_head / n_kv_head > 128 || n_head > 4096 || n_seq <= 0 || n_seq > 16384 || T < 0 || max_q <= 0 || window < 0 || T > (1 << 30) / n_head) return Q36_MOE_EINVAL;
     if (n_blocks <= 0 || (int64_t)n_blocks * block_size > INT32_MAX || max_blocks <= 0 || (int64_t)max_blocks * block_size > (1 << 30)) return Q36_MOE_EINVAL;
-    if (!isfinite(scale) || q_stride < (int64_t)n_head * head_dim || q_stride % (x_is_bf16 ? 8 : 4) || off16(q) || off16(cache)) return Q36_MOE_EINVAL;
-    if ((int64_t)T * n_head > INT32_MAX) return Q36_MOE_EINVAL;
+    if (!isfinite(scale * 1.4426950408889634f) || q_stride < (int64_t)n_head * head_dim || q_stride % (x_is_bf16 ? 8 : 4) || off16(q) || off16(cache)) return Q36_MOE_EINVAL;
     a.kv = KvGeom{(const uint8_t *)cache, n_blocks, block_size, log2_of(block_size), n_kv_head, head_dim};
     a.q = q;
     a.q_stride = q_stride;
@@ -279,7 +279,7 @@ static int attn_args(AttnArgs &a, const void *q, int x_is_bf16, int64_t q_stride
     a.T = T;
     a.Hq = n_head;
     a.G = n_head / n_kv_head;
-    a.window = window;
+    a.window = window < 1 << 30 ? window : 0;      // (no position is 2^30 or more: such a window hides nothing, and sums with it stay in 32 bits)
     a.scale2 = scale * 1.4426950408889634f;
     a.q_bf16 = x_is_bf16 != 0;
     return Q36_MOE_OK;
@@ -300,7 +300,7 @@ int q36_kv_attention(const void *q, int x_is_bf16, int64_t q_stride, const void 
     const int rc = attn_args(a, q, x_is_bf16, q_stride, cache, n_blocks, block_size, n_head, n_kv_head, head_dim, block_table, max_blocks, cu_q,
                              kv_len, n_seq, scale, window, T, max_q);
     if (rc) return rc;
-    if ((T && !out) || off16(out) || out_stride < (int64_t)n_head * head_dim || out_stride % (x_is_bf16 ? 8 : 4) || !ws || off16(ws)) return Q36_MOE_EINVAL;
+    if ((T && !out) || off16(out) || off4(lse) || out_stride < (int64_t)n_head * head_dim || out_stride % (x_is_bf16 ? 8 : 4) || !ws || off16(ws)) return Q36_MOE_EINVAL;
     if (ws_bytes < attention_ws_bytes(n_head, n_kv_head, head_dim, max_q)) return Q36_MOE_ENOSPACE;
     if (T == 0) return Q36_MOE_OK;
     a.out = out;
@@ -325,7 +325,7 @@ int q36_attn_block(const void *q, const void *k, const void *v, int x_is_bf16, i
                        n_seq, scale, window, T, max_q);
     if (rc) return rc;
     const int64_t row = (int64_t)n_kv_head * head_dim, vec = x_is_bf16 ? 8 : 4;
-    if ((T && (!k || !v || !slots || !h)) || !w_o || !ws || D <= 0 || off16(k) || off16(v) || off16(w_o) || off16(ws)) return Q36_MOE_EINVAL;
+    if ((T && (!k || !v || !slots || !h)) || !w_o || !ws || D <= 0 || D > (1 << 30) || off4(bias_o) || off4(h) || off16(k) || off16(v) || off16(w_o) || off16(ws)) return Q36_MOE_EINVAL;
     if (k_stride < row || v_stride < row || k_stride % vec || v_stride % vec) return Q36_MOE_EINVAL;
     if (ws_bytes < q36_attn_block_workspace_bytes(T, n_head, n_kv_head, head_dim, max_q)) return Q36_MOE_ENOSPACE;
     if (T == 0) return Q36_MOE_OK;

@@ -34,7 +34,7 @@ struct PfCfg {
     static constexpr int TM_S = KT, TM_O0 = 2 * NQ * KT;               // columns: two S of each row tile, then O of each
     static constexpr int TMEM = 512;
 };
-constexpr float PF_NONE = -1.0e30f;      // "no token yet": finite, so that differences stay defined
+constexpr float PF_NONE = -3.0e38f;      // "no token yet": finite, so that differences stay defined
 constexpr float PF_GROW = 8.f;
 // What a span costs beside its tokens (Q in, results out, the pipeline's start), in tokens.  Prompt of 8192, 2 x 256 spans: us at 1
 // 577, 192 450, 384 373, 512 374, 768 379.

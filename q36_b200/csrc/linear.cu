@@ -459,9 +459,9 @@ using namespace q36;
 extern "C" int q36_linear(const void *x, int64_t x_stride, const void *w, const float *bias, int act, const void *residual, int res_is_bf16,
                           int64_t res_stride, void *y, int y_is_bf16, int64_t y_stride, int T, int N, int K, const int *rows_used,
                           void *stream) {
-    if ((T && (!x || !y)) || !w || T < 0 || N <= 0 || K <= 0 || K % 8 || x_stride < K || x_stride % 8 || y_stride < N) return Q36_MOE_EINVAL;
+    if ((T && (!x || !y)) || !w || T < 0 || T > (1 << 30) || N <= 0 || N > (1 << 30) || K <= 0 || K > (1 << 30) || K % 8 || x_stride < K || x_stride % 8 || y_stride < N) return Q36_MOE_EINVAL;
     if (act < Q36_ACT_NONE || act > Q36_ACT_GELU_TANH || (residual && res_stride < N)) return Q36_MOE_EINVAL;
-    if ((((uintptr_t)x | (uintptr_t)w) & 15) || ((uintptr_t)y & (y_is_bf16 ? 1 : 3))) return Q36_MOE_EINVAL;
+    if ((((uintptr_t)x | (uintptr_t)w) & 15) || ((uintptr_t)bias & 3) || ((uintptr_t)y & (y_is_bf16 ? 1 : 3))) return Q36_MOE_EINVAL;
     if (residual && ((uintptr_t)residual & (res_is_bf16 ? 1 : 3))) return Q36_MOE_EINVAL;
     if (residual && residual == y && (!res_is_bf16 != !y_is_bf16 || res_stride != y_stride)) return Q36_MOE_EINVAL;
     if (T == 0) return Q36_MOE_OK;

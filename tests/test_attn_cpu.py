@@ -140,3 +140,29 @@ def test_binding_refuses_what_the_library_cannot_see(attn):
                dict(residual=z((2, 7))), dict(out=z((3, 8))), dict(rows_used=z(1, dtype=torch.int64))):
         with pytest.raises(attn.MoEError):
             attn.linear(**{**dict(x=x, w=w), **kw})
+
+
+def test_binding_refuses_numbers_that_would_wrap(attn):
+    """ctypes cuts integers to 32 bits without a word."""
+    import torch
+    i32 = torch.int32
+    kv = attn.KVCache(4, 16, 2, 64, device="cpu")
+    q, tab, cu, ln = torch.zeros((3, 4, 64)), torch.zeros((1, 2), dtype=i32), torch.zeros(2, dtype=i32), torch.zeros(1, dtype=i32)
+    for window in (-1, 2**31, 2**32 + 5):
+        with pytest.raises(attn.MoEError, match="window"):
+            kv.attention(q, tab, cu, ln, 1, window=window)
+    with pytest.raises(AttributeError):
+        kv.data = torch.zeros(1)                                            # its address is the library's
+
+
+def test_sizes_whose_sums_would_pass_32_bits_are_refused(attn, moe):
+    f = attn.lib.q36_kv_attention
+    for i, v in [(19, (1 << 30) // 16 + 1), (14, 3e38), (18, C.c_void_p(4098))]:
+        assert f(*_change(ATTN, i, v)) == moe.EINVAL, (i, v)
+    f = attn.lib.q36_linear
+    good = [P, 256, P, None, 0, None, 0, 0, P, 1, 64, 4, 64, 256, None, None]
+    for i, v in [(11, (1 << 30) + 1), (3, C.c_void_p(4098))]:
+        assert f(*_change(good, i, v)) == moe.EINVAL, (i, v)
+    big = _change(good, 12, (1 << 30) + 1)
+    big[10] = 1 << 31
+    assert f(*big) == moe.EINVAL

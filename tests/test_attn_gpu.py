@@ -323,6 +323,90 @@ def test_strided_rows(attn, x):
     assert (buf[:, :4] == 3).all() and (buf[:, 20:] == 3).all()
 
 
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+def test_any_scale_and_any_window(attn, x):
+    """Negative and zero scales; windows up to the largest integer, with fewer cached tokens than new ones."""
+    rng = np.random.default_rng(13)
+    s = Setup(attn, rng, [(1, 90), (200, 6000), (9, 4)], 16, 2, 128, 16, x)
+    for scale in (-0.1, 0.0):
+        s.check(s.run(scale=scale), scale=scale)
+    for window in (2**30 - 1, 2**30, 2**31 - 2, 2**31 - 1):
+        s.check(s.run(window=window), window=window)
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+def test_scores_of_any_size(attn, x):
+    """Scores of -2^100 and below: the one token whose score is 2^100 above the others' has all the weight."""
+    import torch
+    rng = np.random.default_rng(14)
+    s = Setup(attn, rng, [(1, 90), (200, 6000)], 16, 2, 128, 16, x)
+    k = torch.zeros((6090, 2, 128), device="cuda")
+    k[:, :, 0] = 2.0
+    k[[33, 90 + 4567], :, 0] = 1.0
+    slots = [int(s.table[b, j // 16]) * 16 + j % 16 for b, n in enumerate((90, 6000)) for j in range(n)]
+    v = cu(s.v, torch.float32)
+    s.kv.append(k, v, ints(slots))
+    s.q.zero_()
+    s.q[:, :, 0] = -(2.0 ** 100)
+    out, lse = s.run(scale=1.0)
+    want = torch.cat([v[33:34], v[90 + 4567:90 + 4568].expand(200, -1, -1)]).repeat_interleave(8, 1)
+    assert torch.equal(out.float(), want.to(out.dtype).float())                                    # (a 4-bit value is exact in both types)
+    assert (lse + 2.0 ** 100).abs().max() <= 2.0 ** 78                                             # 2^-22 of it
+
+
+def test_offsets_past_32_bits(attn):
+    """A cache of 9 GB whose pages lie on both sides of 2^31 and 2^32 bytes; rows of q, out, x, y and the residual 2^27 elements
+    apart.  The numbers are those of the same requests with everything close together."""
+    import torch
+    rng = np.random.default_rng(15)
+    for lens in ([(1, 1000), (1, 700)], [(70, 2500)]):
+        s = Setup(attn, rng, lens, 16, 2, 128, 16, "bf16")
+        want = s.run()
+        pages = 9 * 10**9 // s.kv.data[0].numel()
+        far = attn.KVCache(pages, 16, 2, 128, data=torch.empty((pages, 2, 16 * 128 * 17 // 16), dtype=torch.uint8, device="cuda"))
+        near = s.table.cpu().numpy()
+        ids = np.linspace(0, pages - 1, s.n_blocks).astype(np.int64)
+        far.data[torch.from_numpy(ids).cuda()] = s.kv.data
+        s.table = ints(np.where((near >= 0) & (near < s.n_blocks), ids[near.clip(0, s.n_blocks - 1)], -1))
+        s.kv = far
+        q = torch.empty((20, 1 << 27), dtype=torch.bfloat16, device="cuda")
+        if s.T <= 20:
+            wide = q[:s.T, :2048].unflatten(1, (16, 128))
+            wide.copy_(s.q)
+            s.q = wide
+            out, lse = s.run(out=q[:s.T, 4096:4096 + 2048].unflatten(1, (16, 128)))
+        else:
+            out, lse = s.run()
+        assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        k = cu(rng.standard_normal((2, 2, 128), dtype=np.float32))
+        last = ints([pages * 16 - 1, 5])
+        far.append(k, -k, last)
+        a, b = far.read(last)
+        assert torch.equal(a, -b) and (a - k).abs().max() < 1
+    x, w = q[:, :512].copy_(torch.randn(20, 512)), torch.randn(96, 512, device="cuda").bfloat16()
+    res = q[:, 1024:1024 + 96].copy_(torch.randn(20, 96))
+    want = attn.linear(x.contiguous(), w, residual=res.contiguous())
+    assert torch.equal(attn.linear(x, w, residual=res, out=q[:, 2048:2048 + 96]), want)
+    assert torch.equal(attn.linear(x[-3:], w, residual=res[-3:], out=q[-3:, 2048:2048 + 96]), attn.linear(x[-3:].contiguous(), w, residual=res[-3:].contiguous()))
+
+
+def test_more_rows_than_one_launch_takes(attn):
+    """Rows are written and read 2^30 eights at a time: those on both sides of the cut."""
+    import torch
+    H, Dh, T = 1024, 256, (1 << 30) // (1024 * 256 // 8) + 2
+    kv = attn.KVCache(1, 16, H, Dh)
+    k = torch.empty((T, H, Dh), dtype=torch.bfloat16, device="cuda")
+    rows = [0, T - 3, T - 2, T - 1]
+    slots = np.full(T, -1)
+    slots[rows] = [3, 9, 0, 15]
+    k[rows] = torch.randn((4, H, Dh), device="cuda").bfloat16()
+    kv.append(k, k, ints(slots))
+    del k
+    got, _ = kv.read(ints(slots), torch.bfloat16)
+    want, _ = kv.read(ints(slots[rows]), torch.bfloat16)
+    assert torch.equal(got[rows], want) and (want != 0).any(-1).all() and not got[1].any() and not got[T // 2].any()
+
+
 def test_max_q_chooses_kernels_only(attn):
     """Any stated largest number of new tokens gives right results."""
     rng = np.random.default_rng(8)

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 import torch
@@ -134,6 +135,17 @@ def check_device_status(device=None) -> None:
         check(lib.q36_attn_status(torch.cuda.current_stream().cuda_stream), "attn device status")
 
 
+# Workspace sizes by device (which is current) and sizes: a call of the library costs a microsecond.
+@functools.lru_cache(maxsize=1024)
+def _attention_ws(dev, n_head, n_kv_head, head_dim, max_q) -> int:
+    return int(lib.q36_kv_attention_workspace_bytes(n_head, n_kv_head, head_dim, max_q))
+
+
+@functools.lru_cache(maxsize=1024)
+def _block_ws(dev, T, n_head, n_kv_head, head_dim, max_q) -> int:
+    return int(lib.q36_attn_block_workspace_bytes(T, n_head, n_kv_head, head_dim, max_q))
+
+
 class Tables(NamedTuple):
     cu_q: torch.Tensor
     kv_len: torch.Tensor
@@ -254,7 +266,7 @@ class KVCache:
                 out = torch.empty((T, h, d), dtype=q.dtype, device=self.device)
             lse = torch.empty((T, h), dtype=_F32, device=self.device) if want_lse else None
             if ws is None:
-                ws = self._scratch(lib.q36_kv_attention_workspace_bytes(h, self.n_kv_head, d, max(max_q, 1)), st)
+                ws = self._scratch(_attention_ws(self._dev, h, self.n_kv_head, d, max(max_q, 1)), st)
             rc = lib.q36_kv_attention(q.data_ptr(), bf, qs, *args, out.data_ptr(), os_, ptr(lse), T, max_q, ws.data_ptr(), ws.numel(), st)
             if rc:
                 check(rc, what)
@@ -277,7 +289,7 @@ class KVCache:
         ks, vs = (_rows3(t, self.n_kv_head, self.head_dim, what) for t in (k, v))
         with _call(dev, stream) as st:
             if ws is None:
-                ws = self._scratch(lib.q36_attn_block_workspace_bytes(T, n_head, self.n_kv_head, self.head_dim, max(max_q, 1)), st)
+                ws = self._scratch(_block_ws(dev, T, n_head, self.n_kv_head, self.head_dim, max(max_q, 1)), st)
             rc = lib.q36_attn_block(q.data_ptr(), k.data_ptr(), v.data_ptr(), bf, qs, ks, vs, slots.data_ptr(), *args, w_o.data_ptr(), ptr(bias_o),
                                     h.data_ptr(), D, T, max_q, ws.data_ptr(), ws.numel(), st)
             if rc:

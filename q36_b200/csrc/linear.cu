@@ -157,13 +157,15 @@ k_linear_few(const uint16_t *__restrict__ x, long long xs, const uint16_t *__res
 // A tile is 128 columns of y (rows of W, the 128 lanes of the accumulator) by BN rows (its columns): in the epilogue a thread is
 // one column of y, so that bias is a register and a warp's accesses to residual and y are 32 neighbours.
 // SPLIT > 1: a cluster shares a tile, each CTA a part of K; the parts are added in rank order over distributed shared memory.
-constexpr int LT_M = 128, LT_K = 64, LT_EPI_WARPS = 8, LT_THREADS = 32 * (2 + LT_EPI_WARPS);
+constexpr int LT_M = 128, LT_K = 64;
 template <int BN, int SPLIT>
 struct LtCfg {
     static constexpr int STAGE = LT_M * LT_K * 2 + BN * LT_K * 2;
     static constexpr int STAGES = SPLIT > 1 ? (BN == 64 ? 3 : 4) : BN == 256 ? 4 : BN == 128 ? 6 : 8;
     static constexpr int PARTS = SPLIT > 1 ? BN * LT_M * 4 : 0;      // what the cluster's CTAs send: [rank][row of mine][column]
     static constexpr int SMEM = STAGE * STAGES + PARTS + 1024;
+    static constexpr int EPI = BN == 256 ? 16 : 8, GROUPS = EPI / 4;      // warps of the epilogue, in groups of a warp per 32 lanes of TMEM
+    static constexpr int THREADS = 32 * (2 + EPI);
 };
 struct LtMaps { CUtensorMap w, x; };
 __device__ int g_linear_status;      // where a wait gave up (0: nowhere)
@@ -182,7 +184,7 @@ __device__ __forceinline__ uint32_t map_cluster(uint32_t addr, int rank) {
 __device__ __forceinline__ void st_cluster(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
 template <int BN, int SPLIT>
-__global__ void __launch_bounds__(LT_THREADS, 1)
+__global__ void __launch_bounds__(LtCfg<BN, SPLIT>::THREADS, 1)
 k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K, const int *rows_used, int t_tiles, int n_tiles) {
     using C = LtCfg<BN, SPLIT>;
     constexpr int TM_COLS = SPLIT == 1 ? 2 * BN : BN;
@@ -200,7 +202,7 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
     if (tid == 0) {
         abort_flag = 0;
         for (int i = 0; i < C::STAGES; i++) { mbar_init(full0 + 8 * i, 1); mbar_init(empty0 + 8 * i, 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(accf0 + 8 * i, 1); mbar_init(acce0 + 8 * i, LT_EPI_WARPS); }
+        for (int i = 0; i < 2; i++) { mbar_init(accf0 + 8 * i, 1); mbar_init(acce0 + 8 * i, C::EPI); }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) {
@@ -273,7 +275,7 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
             }
         }
     } else {
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        const int q = warp & 3, group = (warp - 2) >> 2;
         uint32_t tc = 0;
         if (SPLIT > 1) cluster_wait();
         for (int i = first; i < tiles; i += step) {
@@ -281,16 +283,16 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
             place(i, n0, t0);
             if (t0 >= rows) continue;
             const uint32_t buf = SPLIT == 1 ? tc & 1 : 0;
-            const int n = n0 + 32 * q + lane, c0 = half * (BN / 2), c1 = c0 + BN / 2;
+            const int n = n0 + 32 * q + lane, c0 = group * (BN / C::GROUPS), c1 = c0 + BN / C::GROUPS;
             const float bias = e.bias && n < N ? e.bias[n] : 0.f;
             // The next tile's residual starts for L2 now, so that the loads below, 16 rows at a time, wait for L2 and not for HBM
             // (8000 x 4100 x 2048 with a bf16 residual: 126 us, 188 with plain loads).
             if (SPLIT == 1) {
-                if (tc == 0) prefetch_res<BN, 32 * LT_EPI_WARPS>(e, n0, LT_M, t0, rows, N, tid - 64);
+                if (tc == 0) prefetch_res<BN, 32 * C::EPI>(e, n0, LT_M, t0, rows, N, tid - 64);
                 if (i + step < tiles) {
                     int n2, t2;
                     place(i + step, n2, t2);
-                    prefetch_res<BN, 32 * LT_EPI_WARPS>(e, n2, LT_M, t2, rows, N, tid - 64);
+                    prefetch_res<BN, 32 * C::EPI>(e, n2, LT_M, t2, rows, N, tid - 64);
                 }
             }
             uint32_t res[2][16];       // one chunk ahead
@@ -385,12 +387,12 @@ static int run_tc(const LtMaps &maps, const Epilogue &e, int T, int N, int K, co
     const int t_tiles = (T + BN - 1) / BN, n_tiles = (N + LT_M - 1) / LT_M;
     const long tiles = (long)t_tiles * n_tiles;
     if (SPLIT == 1) {
-        launch_k(k_linear_tc<BN, SPLIT>, dim3((unsigned)min(tiles, (long)sm_count())), dim3(LT_THREADS), C::SMEM, st, maps, e, T, N, K, rows_used, t_tiles, n_tiles);
+        launch_k(k_linear_tc<BN, SPLIT>, dim3((unsigned)min(tiles, (long)sm_count())), dim3(C::THREADS), C::SMEM, st, maps, e, T, N, K, rows_used, t_tiles, n_tiles);
         return check_launch();
     }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(tiles * SPLIT));
-    cfg.blockDim = dim3(LT_THREADS);
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];

@@ -40,6 +40,14 @@ __device__ __forceinline__ void seq_span(const AttnArgs &a, int b, int &t0, int 
     len = min(max(a.kv_len[b], 0), a.max_blocks << a.kv.log_bs);
 }
 
+// One lane of a warp that runs as a whole: what it issues to the tensor core has its operands in uniform registers (an MMA of
+// 128 x 64 x 16 every 48 cycles, every 90 under `lane == 0`, which leaves that to be found out per instruction).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
 // eight elements from element e on
 __device__ __forceinline__ void load8(const void *p, size_t e, int bf16, float (&v)[8]) {
     if (bf16) {

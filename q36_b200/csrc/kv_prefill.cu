@@ -569,7 +569,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_ISSUE));
         const int i = (warp - 16) >> 1;
-        if (i < NQ && lane == 0) {
+        if (i < NQ && elect_one()) {
             // ------------------------------------------------------------ products of row tile i: S (even warps) or P V (odd)
             const bool do_s = (warp & 1) == 0;
             uint32_t kv = 0, n_mine = 0, qn = 0;       // tiles passed, products of this issuer, pieces

@@ -250,7 +250,7 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
                     for (uint32_t n = 0; n < TC_SPIN_LIMIT && !mbar_try(full0 + 8 * (i % C::STAGES), (i / C::STAGES) & 1); n++) {}
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (elect_one()) {
             uint32_t it = 0, tc = 0;
             bool ok = true;
             for (int i = first; i < tiles && ok; i += step) {

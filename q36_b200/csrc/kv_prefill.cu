@@ -171,6 +171,11 @@ __device__ __forceinline__ float pf_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -359,9 +364,9 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
                     float mc[KT / 32];
 #pragma unroll
                     for (int c = 0; c < KT / 32; c++) {
-                        mc[c] = __uint_as_float(v[c][0]);
+                        mc[c] = fmaxf(__uint_as_float(v[c][0]), __uint_as_float(v[c][1]));
 #pragma unroll
-                        for (int e = 1; e < 32; e++) mc[c] = fmaxf(mc[c], __uint_as_float(v[c][e]));
+                        for (int e = 2; e < 32; e += 2) mc[c] = max3(mc[c], __uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1]));
                     }
                     float mx = mc[0];
 #pragma unroll

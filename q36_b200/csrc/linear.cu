@@ -423,10 +423,10 @@ int launch_linear(const void *x, long long xs, const void *w, const float *bias,
         launch_k(k_linear_few, dim3((N + LS_COLS - 1) / LS_COLS), dim3(LS_THREADS), 0, st, (const uint16_t *)x, xs, (const uint16_t *)w, e, T, N, K, rows_used);
         return check_launch();
     }
-    // Tile height and split of K by what an SM has to load (150 KB per us, two CTAs of 32 or 64 rows at a time), what the exchange
-    // of a cluster costs (2.3 us at 128 rows) and what a second round of CTAs costs.  Measured us at 2048 columns, K 2048, for
-    // (rows, split): 64 tokens (32, 4) 6.9, (64, 8) 7.5, (64, 1) 13.5; 200 tokens (64, 4) 9.3, (128, 4) 9.2, (32, 8) 23; 300
-    // tokens (64, 2) 10.9, (128, 4) 17.3; 1000 tokens (128, 1) 15.8, (256, 1) 17.0, (128, 4) 36.
+    // Tile height and split of K by what an SM has to load (166 KB per us, at least 0.22 us per 64 of K; two CTAs of 32 or 64 rows at a
+    // time), what the exchange of a cluster costs and what a second round of CTAs costs.  Measured us at 2048 columns, K 2048, for
+    // (rows, split): 64 tokens (32, 4) 6.6, (64, 8) 7.6, (64, 1) 10.9; 200 tokens (32, 2) 8.6, (64, 4) 9.4, (32, 4) 13.4; 300
+    // tokens (64, 1) 11.2, (128, 4) 17.0; 1000 tokens (128, 1) 12.5, (256, 1) 15.6, (128, 4) 35.
     int bn = 0, split = 1;
     float best = 0.f;
     const int steps = (K + LT_K - 1) / LT_K, sms = sm_count();
@@ -434,7 +434,9 @@ int launch_linear(const void *x, long long xs, const void *w, const float *bias,
         for (int cs = 1; cs <= (cb == 256 ? 1 : 8) && (cs == 1 || steps >= 2 * cs); cs *= 2) {
             const long ctas = (long)((T + cb - 1) / cb) * ((N + LT_M - 1) / LT_M) * cs, per_sm = (ctas + sms - 1) / sms;
             const long rounds = cs == 1 ? 1 : (per_sm + (cb <= 64 ? 1 : 0)) / (cb <= 64 ? 2 : 1);
-            const float us = per_sm * ((steps + cs - 1) / cs) * (LT_M + cb) * (LT_K * 2 / 1024.f) / 150.f + (cs > 1 ? 0.018f * cb : 0.f) + 3.f * (rounds - 1);
+            const float kb = (LT_M + cb) * (LT_K * 2 / 1024.f);
+            const float us = cs == 1 ? per_sm * steps * fmaxf(0.22f, kb / 166.f)
+                                     : (steps + cs - 1) / cs * fmaxf(0.22f * rounds, per_sm * kb / 166.f) + 0.05f * cb + 4.9f * (rounds - 1);
             if (!bn || us < best) { best = us; bn = cb; split = cs; }
         }
     LtMaps maps;

@@ -8,11 +8,13 @@ namespace q36 {
 // rows: rows of a tile; unit: tokens of a unit; all: every request takes part, not only those that is_long leaves.
 struct SpanRule { int rows, unit, all; };
 
-// Which requests go to the tile kernel (bf16, when the host says that there may be any).  It does 128 or 256 rows at ten times the
-// rate of the other one, but a piece of work costs it 10 us to begin and end.  us of the few-row kernel / of this one, 16 heads of
-// 128 on 2: 16 new tokens (128 rows) CROSS
-constexpr int LONG_ROWS = 65, LONG_WORK = 1 << 20;
-__device__ __forceinline__ bool is_long(int rows, int len) { return rows >= LONG_ROWS && (long long)rows * len >= LONG_WORK; }
+// Which requests go to the tile kernel (bf16): those of 65 rows and more whose rows times cached tokens reach a.long_work.  It does 128
+// or 256 rows at five times the rate of the other one, but begins and ends in 40 us.  A batch amortises that, a short continuation alone
+// does not: 2^20 as a rule, 2^22 where the call has 1024 rows per kv head at most.  us of the few-row kernel / of the tile kernel, one
+// request, 16 heads of 128 on 2: 32 new tokens (256 rows) on 4096 23 / 42, on 32,768 78 / 63; 64 on 4096 31 / 43, on 32,768 139 / 65;
+// 128 on 512 20 / 25, on 4096 48 / 46, on 32,768 265 / 72.
+constexpr int LONG_ROWS = 65, LONG_WORK = 1 << 20, LONG_WORK_FEW = 1 << 22, LONG_FEW_ROWS = 1024;
+__device__ __forceinline__ bool is_long(const AttnArgs &a, int rows, int len) { return rows >= LONG_ROWS && (long long)rows * len >= a.long_work; }
 
 struct SeqSpans { int t0, n, len, tiles, u_lo, u_hi; };   // units [u_lo, u_hi) of the cached tokens that any row sees
 
@@ -20,7 +22,7 @@ __device__ __forceinline__ SeqSpans seq_spans(const AttnArgs &a, const SpanRule 
     SeqSpans s;
     seq_span(a, b, s.t0, s.n, s.len);
     const int rows = s.n * a.G;
-    s.tiles = rows > 0 && (r.all || !is_long(rows, s.len)) ? (rows + r.rows - 1) / r.rows : 0;
+    s.tiles = rows > 0 && (r.all || !is_long(a, rows, s.len)) ? (rows + r.rows - 1) / r.rows : 0;
     const int lo = a.window > 0 ? max(0, s.len - s.n - a.window + 1) : 0;
     s.u_lo = lo / r.unit;
     s.u_hi = max((s.len + r.unit - 1) / r.unit, s.u_lo + 1);     // (at least one: rows that see nothing are written too)

@@ -244,10 +244,13 @@ uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) {
     return rows < LONG_ROWS ? few : max(few, prefill_ws_bytes(Dh));      // (one after the other on the stream: the same memory)
 }
 
-int launch_attention(const AttnArgs &a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st) {
+int launch_attention(AttnArgs a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st) {
     (void)ws_bytes;
-    const int rows = rows_of(a.Hq, a.kv.Hkv, max_q);
-    if (!a.q_bf16 || rows < LONG_ROWS) return launch_decode(a, rows, 1, ws, st);
+    const long long all = (long long)a.T * a.G;
+    const int rows = (int)min((long long)rows_of(a.Hq, a.kv.Hkv, max_q), all);      // of one request, at most
+    a.long_work = all <= LONG_FEW_ROWS ? LONG_WORK_FEW : LONG_WORK;
+    const bool any = a.q_bf16 && rows >= LONG_ROWS && rows * ((long long)a.max_blocks << a.kv.log_bs) >= a.long_work;
+    if (!any) return launch_decode(a, rows, 1, ws, st);
     int rc;
     if ((rc = launch_decode(a, rows, 0, ws, st))) return rc;
     return launch_prefill(a, ws, st);

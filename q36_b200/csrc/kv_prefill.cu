@@ -56,7 +56,7 @@ __device__ __forceinline__ PfSeq pf_seq(const AttnArgs &a, int R, int b) {
     PfSeq s;
     seq_span(a, b, s.t0, s.n, s.len);
     s.c = R / a.G;
-    s.tiles = is_long(s.n * a.G, s.len) ? (s.n + s.c - 1) / s.c : 0;
+    s.tiles = is_long(a, s.n * a.G, s.len) ? (s.n + s.c - 1) / s.c : 0;
     return s;
 }
 __device__ __forceinline__ void pf_range(const AttnArgs &a, const PfSeq &s, int rt, int &lo, int &hi) {

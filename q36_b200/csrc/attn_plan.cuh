@@ -160,7 +160,7 @@ __device__ __forceinline__ void attn_store_lse(const AttnArgs &a, int t0, int n,
 
 constexpr int DEC_MAX_OCC = 4;
 int launch_decode(const AttnArgs &a, int rows, int all, void *ws, cudaStream_t st);
-uint64_t decode_ws_bytes(int Dh, int rows);
+uint64_t decode_ws_bytes(int Dh);
 int launch_prefill(const AttnArgs &a, void *ws, cudaStream_t st);
 uint64_t prefill_ws_bytes(int Dh);
 int prefill_wait_status(int *out);

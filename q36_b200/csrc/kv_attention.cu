@@ -240,7 +240,7 @@ static int rows_of(int Hq, int Hkv, int max_q) { return (int)min((long)(Hq / Hkv
 
 uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) {
     const int rows = rows_of(Hq, Hkv, max_q);
-    const uint64_t few = decode_ws_bytes(Dh, rows);
+    const uint64_t few = decode_ws_bytes(Dh);
     return rows < LONG_ROWS ? few : max(few, prefill_ws_bytes(Dh));      // (one after the other on the stream: the same memory)
 }
 

@@ -590,26 +590,31 @@ static int run(const AttnArgs &a, int all, void *ws, cudaStream_t st) {
     return launch_attn_join(a, 8 * NT, grid, desc, part, st);
 }
 
-// Rows per tile: 8 while a request's rows fit them, else 16 (halves what the cache is read); 256-wide heads keep 8, whose
-// accumulators are what 16 rows of 128 are.
-static int decode_nt(int Dh, int rows) { return Dh == 256 || rows <= 8 ? 1 : 2; }
-
-uint64_t decode_ws_bytes(int Dh, int rows) {
-    const int grid = sm_count() * DEC_MAX_OCC;
-    return attn_desc_bytes(grid) + 2ull * grid * attn_part_floats(8 * decode_nt(Dh, rows), Dh) * 4;
+// Rows per tile: 8, or 16 where that halves what is read and widened for no more instructions: 64-wide heads and f32 prompts, in calls
+// that fill the GPU and without a tile that is half empty.  us with 8 / 16: 64 requests, 266,000 tokens, 16 query heads per kv head of 64
+// 49 / 42, of 128 62 / 62, 20 query heads of 128 84 / 98; f32 prompt of 2048 394 / 336, of 8192 5690 / 4690; one request of 2000
+// tokens 15 / 21.  256-wide heads have accumulators for 8.
+static int decode_nt(const AttnArgs &a, int rows, int all) {
+    const bool gains = a.kv.Dh == 64 || (a.kv.Dh == 128 && !a.q_bf16 && rows >= 64);
+    return all && gains && (long long)a.T * a.G > 256 && (rows + 15) / 16 * 2 <= (rows + 7) / 8 ? 2 : 1;
 }
 
+uint64_t decode_ws_bytes(int Dh) {
+    const int grid = sm_count() * DEC_MAX_OCC;
+    return attn_desc_bytes(grid) + 2ull * grid * attn_part_floats(Dh == 256 ? 8 : 16, Dh) * 4;
+}
+
+// rows: of one request, at most; all: every request, not only those that the tile kernel leaves
 int launch_decode(const AttnArgs &a, int rows, int all, void *ws, cudaStream_t st) {
     const bool f32 = !a.q_bf16;
-    // (beside the tile kernel most of what is left has one new token)
-    const int nt = all ? decode_nt(a.kv.Dh, rows) : 1;
+    const int nt = decode_nt(a, rows, all);
     if (a.kv.Dh == 64) {
         if (nt == 1) return f32 ? run<64, 1, true>(a, all, ws, st) : run<64, 1, false>(a, all, ws, st);
         return f32 ? run<64, 2, true>(a, all, ws, st) : run<64, 2, false>(a, all, ws, st);
     }
     if (a.kv.Dh == 128) {
-        if (nt == 1) return f32 ? run<128, 1, true>(a, all, ws, st) : run<128, 1, false>(a, all, ws, st);
-        return f32 ? run<128, 2, true>(a, all, ws, st) : run<128, 2, false>(a, all, ws, st);
+        if (!f32) return run<128, 1, false>(a, all, ws, st);
+        return nt == 1 ? run<128, 1, true>(a, all, ws, st) : run<128, 2, true>(a, all, ws, st);
     }
     return f32 ? run<256, 1, true>(a, all, ws, st) : run<256, 1, false>(a, all, ws, st);
 }

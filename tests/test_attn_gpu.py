@@ -324,6 +324,17 @@ def test_strided_rows(attn, x):
 
 
 @pytest.mark.parametrize("x", ["bf16", "f32"])
+@pytest.mark.parametrize("heads,Dh", [((32, 2), 64), ((24, 2), 64), ((40, 2), 64), ((32, 2), 128)])
+@pytest.mark.parametrize("q", [1, 9])
+def test_many_requests_with_a_tile_of_16_rows(attn, heads, Dh, x, q):
+    """Calls that fill the GPU: the wider tile, whole, with rows missing and with a second tile."""
+    rng = np.random.default_rng(16)
+    s = Setup(attn, rng, [(q, int(n)) for n in rng.integers(q, 700, 30)], *heads, Dh, 32, x)
+    s.check(s.run())
+    s.check(s.run(window=40), window=40)
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
 def test_any_scale_and_any_window(attn, x):
     """Negative and zero scales; windows up to the largest integer, with fewer cached tokens than new ones."""
     rng = np.random.default_rng(13)

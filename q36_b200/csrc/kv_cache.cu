@@ -152,8 +152,22 @@ constexpr int KVC_THREADS = 256;
 // A thread's eight dims of a row of K and of V: token t, kv head, scale block b, quarter j of it.  Four lanes share a block, so that rows
 // are read and K codes written in whole sectors.
 struct RowPart { int t, head, b, j, r; };
-__device__ __forceinline__ RowPart row_part(const KvGeom &g, unsigned i) {
-    const unsigned row8 = g.Hkv * g.Dh / 8, head8 = g.Dh / 8, t = i / row8, r = i - t * row8, head = r / head8, c = r - head * head8;
+// Parts per row and how to divide a part's number, below 2^31, by them: n m / 2^(31 + s) with m = ceil(2^(31 + s) / row8), 2^s >= row8, is at
+// most n / 2^31 2^-s above n / row8: less than the 1 / row8 that the next whole number is away.
+struct RowDiv {
+    unsigned row8, m;
+    int s, log_head8;
+};
+static RowDiv row_div(const KvGeom &g) {
+    RowDiv d;
+    d.row8 = g.Hkv * g.Dh / 8;
+    d.s = log2_of((int)d.row8);
+    d.m = (unsigned)(((1ull << (31 + d.s)) + d.row8 - 1) / d.row8);
+    d.log_head8 = log2_of(g.Dh / 8);
+    return d;
+}
+__device__ __forceinline__ RowPart row_part(const RowDiv &d, unsigned i) {
+    const unsigned t = __umulhi(i, d.m) >> (d.s - 1), r = i - t * d.row8, head = r >> d.log_head8, c = r & ((1u << d.log_head8) - 1);
     return RowPart{(int)t, (int)head, (int)(c >> 2), (int)(c & 3), (int)r};
 }
 // eight values, and the whole block's largest magnitude's exponent -> codes; NaN counts as 0
@@ -174,10 +188,10 @@ __device__ __forceinline__ uint32_t quant8(float (&x)[8], int &e2) {
 }
 __global__ void __launch_bounds__(KVC_THREADS)
 k_kv_append(const void *__restrict__ k, const void *__restrict__ v, int bf16, long long ks, long long vs, const int *__restrict__ slots, KvGeom g,
-            unsigned n8) {
+            RowDiv div, unsigned n8) {
     Q36_GDS();
     const unsigned i = blockIdx.x * KVC_THREADS + threadIdx.x;
-    const RowPart p = row_part(g, min(i, n8 - 1));
+    const RowPart p = row_part(div, min(i, n8 - 1));
     const int slot = i < n8 ? slots[p.t] : -1, block = slot >> g.log_bs;
     const bool put = slot >= 0 && block < g.n_blocks;
     float x[8] = {}, y[8] = {};
@@ -217,11 +231,11 @@ __device__ __forceinline__ void store8_exact(void *p, size_t at, int bf16, uint3
     }
 }
 __global__ void __launch_bounds__(KVC_THREADS)
-k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *__restrict__ v, int bf16, unsigned n8) {
+k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *__restrict__ v, int bf16, RowDiv div, unsigned n8) {
     Q36_GDS();
     const unsigned i = blockIdx.x * KVC_THREADS + threadIdx.x;
     if (i >= n8) return;
-    const RowPart p = row_part(g, i);
+    const RowPart p = row_part(div, i);
     const int slot = slots[p.t], block = slot >> g.log_bs;
     uint32_t kc = 0, vc = 0;
     float sk = 0.f, sv = 0.f;
@@ -241,19 +255,20 @@ k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *_
 // n8 < 2^31: rows are launched in lots of that many parts
 template <typename F>
 static int by_lots(KvGeom g, int T, F launch) {
-    const long long row8 = (long long)g.Hkv * g.Dh / 8;
+    const RowDiv div = row_div(g);
+    const long long row8 = div.row8;
     const int lot = (int)min((long long)T, (1ll << 30) / row8);
     for (int t = 0; t < T; t += lot) {
         const int n = min(lot, T - t);
-        launch(t, (unsigned)(n * row8), dim3((unsigned)((n * row8 + KVC_THREADS - 1) / KVC_THREADS)));
+        launch(t, div, (unsigned)(n * row8), dim3((unsigned)((n * row8 + KVC_THREADS - 1) / KVC_THREADS)));
     }
     return check_launch();
 }
 int launch_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g, int T, cudaStream_t st) {
     const int size = bf16 ? 2 : 4;
-    return by_lots(g, T, [&](int t, unsigned n8, dim3 grid) {
+    return by_lots(g, T, [&](int t, RowDiv div, unsigned n8, dim3 grid) {
         launch_k(k_kv_append, grid, dim3(KVC_THREADS), 0, st, (const void *)((const uint8_t *)k + (size_t)t * ks * size),
-                 (const void *)((const uint8_t *)v + (size_t)t * vs * size), bf16, ks, vs, slots + t, g, n8);
+                 (const void *)((const uint8_t *)v + (size_t)t * vs * size), bf16, ks, vs, slots + t, g, div, n8);
     });
 }
 
@@ -308,9 +323,9 @@ int q36_kv_read(const void *cache, int n_blocks, int block_size, int n_kv_head, 
     if (T == 0) return Q36_MOE_OK;
     const KvGeom g{(const uint8_t *)cache, n_blocks, block_size, log2_of(block_size), n_kv_head, head_dim};
     const size_t row = (size_t)n_kv_head * head_dim * (x_is_bf16 ? 2 : 4);
-    return by_lots(g, T, [&](int t, unsigned n8, dim3 grid) {
+    return by_lots(g, T, [&](int t, RowDiv div, unsigned n8, dim3 grid) {
         launch_k(k_kv_read, grid, dim3(KVC_THREADS), 0, (cudaStream_t)stream, g, slots + t, (void *)((uint8_t *)k + t * row),
-                 (void *)((uint8_t *)v + t * row), x_is_bf16, n8);
+                 (void *)((uint8_t *)v + t * row), x_is_bf16, div, n8);
     });
 }
 

@@ -2,11 +2,9 @@
  * key/value cache held in 4 bits, its tables, its writer and reader, attention
  * over it, and the matrix product that leads back into the residual stream.
  *
- * The engine keeps this half of a layer in attn_layer / pf_layer_moe
- * (q36_engine.cu:1957-1962, 3474-3527): append to the cache (k_kv_append,
- * q36_engine.cu:829), attention (k_attn_partial2 / k_attn_pf3,
- * q36_engine.cu:966, 2865), output projection, residual add.  q36_attn_block
- * runs that chain and leaves h where q36_moe_block takes it up.
+ * This half of a layer is: append to the cache, attention, output projection,
+ * residual add.  q36_attn_block runs that chain and leaves h where q36_moe_block
+ * takes it up.
  *
  * The conventions are those of q36_moe.h: device pointers, launch-only (no host
  * synchronisation, no allocation, capturable in a CUDA graph), a stream per
@@ -87,7 +85,7 @@ int q36_kv_read(const void *cache, int n_blocks, int block_size, int n_kv_head, 
  * max_q: the largest number of new tokens of a request, as far as the host
  * knows it; it chooses kernels only, any value >= 1 gives right results.
  * n_head / n_kv_head <= 128, n_head <= 4096, 1 <= n_seq <= 16384, T * n_head <= 2^30.
- * f32 prompts run on the kernel for few rows: right at every length, a fifth of bf16's rate. */
+ * f32 prompts run on the kernel for few rows: right at every length, 6 to 14 times bf16's time. */
 uint64_t q36_kv_attention_workspace_bytes(int n_head, int n_kv_head, int head_dim, int max_q);
 int q36_kv_attention(const void *q, int x_is_bf16, int64_t q_stride, const void *cache, int n_blocks, int block_size,
                      int n_head, int n_kv_head, int head_dim, const int *block_table, int max_blocks, const int *cu_q,

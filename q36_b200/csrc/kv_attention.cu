@@ -101,7 +101,7 @@ __device__ __forceinline__ void join_store(const AttnArgs &a, const AttnPart &d,
 }
 
 // Tiles of 8 or 16 rows.  Spans in up to 32 pieces: a block per span, a warp per row.  Longer ones: a block per row, its warps share
-// the pieces.
+// the pieces.  The latency of four reads in a row bounds it (list, piece, weights, rows): 7 to 8 us cold, 4 to 5 behind the kernel before it.
 constexpr int JOIN_WIDE = 256;
 template <int DH>
 __global__ void __launch_bounds__(JOIN_WIDE)
@@ -149,7 +149,8 @@ k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ de
     }
 }
 
-// Tiles of 128 or 256 rows, mostly in two or three pieces: a warp per four rows, so that the loads of all four are on their way at once.
+// Tiles of 128 or 256 rows, mostly in two or three pieces: a warp per four rows, so that the loads of all four are on their way at once
+// (three chunks of up to 777 tokens on up to 6000 beside 37 single tokens: 14.5 us, 25 with a row at a time).
 template <int DH>
 __global__ void __launch_bounds__(JOIN_THREADS)
 k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {

@@ -19,6 +19,8 @@
 // Work.  A unit is 16 tokens of one (request, kv head, row tile).  The units of all requests, in order, are cut into equal
 // ranges, one per CTA, so that ragged lengths load every SM alike.  A range's first and last pieces may be parts of what a
 // neighbour has the rest of: they go to the workspace and k_attn_join adds them up in a fixed order.
+// With the join, 16 heads of 128 on 2: 64 requests of 266,000 tokens together 38 us, of 524,000 54 (4.6 TB/s between the two; the first 20 us
+// are launches, plan, the first reads of a page, of its data, and the join), one of 700 tokens 10, one of 131,072 33.
 #include <math.h>
 
 #include "attn_plan.cuh"

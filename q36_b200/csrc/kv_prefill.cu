@@ -7,9 +7,15 @@
 //                      once (half a step 2^-8, as the output's), the sum of the unrounded weights in f32
 //   warps 8-11, 12-15  K, V: 4-bit rows -> bf16 operand tiles in shared memory (128-byte swizzle)
 //   warps 16 - 19      S = Q K^T and O += P V of each row tile on tcgen05 (f32 in TMEM; P is read from TMEM, where it takes S's
-//                      place): one thread issues an MMA per 90 cycles at most, which the pipe needs 32 to 64 for
+//                      place), an issuing warp for each, since they wait for different things
 // Every row tile has two S, so that the products of a tile run while the softmax is at the one before.
 // m is a lagging maximum: O is rescaled (in TMEM) only when a row would pass 2^8.
+//
+// What bounds it: nothing alone.  A tile takes 2300 cycles (2048 tokens behind 32,768, 16 heads of 128 on 2: 584 us, 970 TFLOP/s; prompt of
+// 8192 336 us, 819).  The tensor pipe needs 1320 of them (an MMA of 128 x 64 x 16 with both operands in shared memory takes 50 cycles,
+// shared memory's rate, one of 128 x 128 x 16 with P in TMEM 65), the exponentials 1070, the ALU 1330, issue slots two thirds.  Without the
+// exponentials the time stays, with twice the widening warps too, with both it falls by a tenth.  Tried without gain: a polynomial for
+// some of the exponentials, turns between the two row tiles' exponentials, sleeping waits, other register splits.
 //
 // Work: the spans (kv head, row tile) of all long requests, measured in the tokens they see, are cut into equal ranges, one per CTA;
 // cuts are moved down to tile boundaries.  Cut spans are joined as in the decode kernel.

@@ -93,7 +93,8 @@ __device__ __forceinline__ void finish(const Epilogue &e, int n, float bias, int
 }
 
 // ---------------------------------------------------------------- few rows: the weights' stream
-// Up to 8 rows.  A block has 16 columns of y (rows of W) and splits K over its warps; a lane reads 16 bytes of two rows of W
+// Up to 8 rows: the stream of W bounds it, and below 10 MB the latency of one round trip (1 x 2048 x 2048, 8.4 MB, 5.9 us).  A block has
+// 16 columns of y (rows of W) and splits K over its warps; a lane reads 16 bytes of two rows of W
 // and of one row of x, which is a fragment of m16n8k16 with k permuted alike on both sides.
 constexpr int LS_WARPS = 8, LS_THREADS = 32 * LS_WARPS, LS_COLS = 16;
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -156,6 +157,8 @@ k_linear_few(const uint16_t *__restrict__ x, long long xs, const uint16_t *__res
 // ---------------------------------------------------------------- tiles on tcgen05
 // A tile is 128 columns of y (rows of W, the 128 lanes of the accumulator) by BN rows (its columns): in the epilogue a thread is
 // one column of y, so that bias is a register and a warp's accesses to residual and y are 32 neighbours.
+// The tensor pipe bounds large products (4096 x 4096 x 4096 102 us, 1352 TFLOP/s; 8000 x 4100 x 2048 107 us alone, 112 with gelu_tanh, 122
+// with a bf16 residual, 135 with both and bias: 16 epilogue warps, 143 with 8), the loads from L2 those of few rows.
 // SPLIT > 1: a cluster shares a tile, each CTA a part of K; the parts are added in rank order over distributed shared memory.
 constexpr int LT_M = 128, LT_K = 64;
 template <int BN, int SPLIT>
@@ -286,7 +289,7 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
             const int n = n0 + 32 * q + lane, c0 = group * (BN / C::GROUPS), c1 = c0 + BN / C::GROUPS;
             const float bias = e.bias && n < N ? e.bias[n] : 0.f;
             // The next tile's residual starts for L2 now, so that the loads below, 16 rows at a time, wait for L2 and not for HBM
-            // (8000 x 4100 x 2048 with a bf16 residual: 126 us, 188 with plain loads).
+            // (8000 x 4100 x 2048 with a bf16 residual: 122 us, 188 with plain loads).
             if (SPLIT == 1) {
                 if (tc == 0) prefetch_res<BN, 32 * C::EPI>(e, n0, LT_M, t0, rows, N, tid - 64);
                 if (i + step < tiles) {

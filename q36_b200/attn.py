@@ -125,6 +125,11 @@ def _rows3(t, h, d, what) -> int:
     return s[0] if t.shape[0] > 1 else h * d
 
 
+# (strides given: a microsecond less than torch.empty)
+def _rows(T, h, d, dtype, device):
+    return torch.empty_strided((T, h, d), (h * d, d, 1), dtype=dtype, device=device)
+
+
 def kv_block_bytes(block_size: int, n_kv_head: int, head_dim: int) -> int:
     return int(lib.q36_kv_block_bytes(block_size, n_kv_head, head_dim))
 
@@ -168,7 +173,7 @@ def kv_tables(kv_old, q_len, block_size, free_blocks, free_head, block_table, T,
         _need(all(t.numel() == n for t, n in zip(out, sizes)), "kv_tables (out)")
     with _call(dev, stream) as st:
         if out is None:
-            out = Tables(*torch.empty(2 * (B + T) + 3, dtype=_I32, device=kv_old.device).split_with_sizes(sizes))
+            out = Tables(*torch.unsafe_split_with_sizes(torch.empty(2 * (B + T) + 3, dtype=_I32, device=kv_old.device), sizes))
         rc = lib.q36_kv_tables(kv_old.data_ptr(), q_len.data_ptr(), B, block_size, (2**31 - 1) // max(block_size, 1) if n_blocks is None else n_blocks, free_blocks.data_ptr(),
                                free_blocks.numel(), free_head.data_ptr(), block_table.data_ptr(), block_table.shape[1], out.cu_q.data_ptr(),
                                out.kv_len.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(), T, out.free_head.data_ptr(),
@@ -228,7 +233,7 @@ class KVCache:
         if dtype is not _BF16 and dtype is not _F32:
             _refuse("kv_read (bf16 or f32)")
         with _call(dev, stream) as st:
-            k, v = torch.empty((2, T, self.n_kv_head, self.head_dim), dtype=dtype, device=self.device).unbind(0)
+            k, v = _rows(T, self.n_kv_head, self.head_dim, dtype, self.device), _rows(T, self.n_kv_head, self.head_dim, dtype, self.device)
             rc = lib.q36_kv_read(*self._geom, self.n_kv_head, self.head_dim, slots.data_ptr(), k.data_ptr(), v.data_ptr(), int(dtype is _BF16), T, st)
             if rc:
                 check(rc, "kv_read")
@@ -263,7 +268,7 @@ class KVCache:
             _refuse(f"{what} (ws)")
         with _call(self._dev, stream) as st:
             if out is None:
-                out = torch.empty((T, h, d), dtype=q.dtype, device=self.device)
+                out = _rows(T, h, d, q.dtype, self.device)
             lse = torch.empty((T, h), dtype=_F32, device=self.device) if want_lse else None
             if ws is None:
                 ws = self._scratch(_attention_ws(self._dev, h, self.n_kv_head, d, max(max_q, 1)), st)
@@ -326,7 +331,7 @@ def linear(x, w, bias=None, act="none", residual=None, out=None, out_dtype=None,
         _ints("linear", dev, rows_used)
     with _call(dev, stream) as st:
         if out is None:
-            out = torch.empty((T, N), dtype=out_dtype, device=x.device)
+            out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=x.device)
         rc = lib.q36_linear(x.data_ptr(), xs, w.data_ptr(), ptr(bias), ACTS[act], ptr(residual), rbf, rs, out.data_ptr(), _is_bf16(out, "linear"), ys,
                             T, N, K, ptr(rows_used), st)
         if rc:

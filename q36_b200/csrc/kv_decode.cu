@@ -19,8 +19,8 @@
 // Work.  A unit is 16 tokens of one (request, kv head, row tile).  The units of all requests, in order, are cut into equal
 // ranges, one per CTA, so that ragged lengths load every SM alike.  A range's first and last pieces may be parts of what a
 // neighbour has the rest of: they go to the workspace and k_attn_join adds them up in a fixed order.
-// With the join, 16 heads of 128 on 2: 64 requests of 266,000 tokens together 38 us, of 524,000 54 (4.6 TB/s between the two; the first 20 us
-// are launches, plan, the first reads of a page, of its data, and the join), one of 700 tokens 10, one of 131,072 33.
+// With the join, 16 heads of 128 on 2: 64 requests of 266,000 tokens together 35 us, of 524,000 49 (5.0 TB/s between the two; the first 20 us
+// are launches, plan, the first reads of a page, of its data, and the join), one of 700 tokens 10, one of 131,072 32.
 #include <math.h>
 
 #include "attn_plan.cuh"
@@ -84,44 +84,75 @@ __device__ __forceinline__ void weights_f16(const float (&p)[4], uint32_t (&w)[T
         w[1][nt][1] = transpose8x8(pack_f16(p[2] - h1.x, p[3] - h1.y));
     }
 }
-template <int W>
-__device__ __forceinline__ void ld_words(const uint8_t *p, uint32_t (&r)[W]) {
-    if constexpr (W == 2) {
-        const uint2 v = __ldg(reinterpret_cast<const uint2 *>(p));
-        r[0] = v.x; r[1] = v.y;
-    } else {
-#pragma unroll
-        for (int i = 0; i < W / 4; i++) {
-            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(p) + i);
-            r[4 * i] = v.x; r[4 * i + 1] = v.y; r[4 * i + 2] = v.z; r[4 * i + 3] = v.w;
-        }
-    }
+// BYTES from global to shared memory behind the thread's back; what a thread has asked for is there for itself after cp_wait
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t to, const uint8_t *from) {
+    if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+    else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-// What a lane holds of 16 tokens.  Lane (g, j): g = lane / 4, j = lane % 4.
+// What a lane holds of 16 tokens, and where it waits in shared memory until then.  Lane (g, j): g = lane / 4, j = lane % 4.  A lane
+// copies exactly what it reads itself (scales of a token come as a word), so that nobody waits for anybody else.
 template <int DH>
 struct DecFrag {
     static constexpr int NB = DH / 32, W = DH / 32, SW = (NB + 3) / 4, VB = NB >= 4 ? NB / 4 : 1;
+    static constexpr int CB = W == 2 ? 8 : 16, NCH = W * 4 / CB, SB = NB == 8 ? 8 : 4;         // a piece of codes, pieces of a token half, a piece of scales
+    static constexpr int CODES = 4 * NCH * 32 * CB, STAGE = CODES + 4 * 32 * SB, STAGES = 2;
     uint32_t k[2][W];      // K words of tokens g and g + 8: word b = dims 32b + 8j ..
     uint32_t v[2][W];      // V of token pairs j and j + 4, group g: first half token 2p, second half token 2p + 1
     uint32_t ks[2][SW];    // K scales of tokens g and g + 8
     uint32_t vs[VB];       // V scales of tokens g (low half) and g + 8, blocks VB j ..
-    // p: the region plus the group's first token's bytes of codes, and its scales; lane parts added by the caller
-    __device__ __forceinline__ void load_k(const uint8_t *pk, const uint8_t *ps) {
+    // pk, pv, pks, pvs: this lane's part of the group's codes and scales
+    static __device__ __forceinline__ void copy(uint32_t st, const uint8_t *pk, const uint8_t *pv, const uint8_t *pks, const uint8_t *pvs, int lane) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            ld_words<W>(pk + h * 8 * (DH / 2), k[h]);
-            const uint8_t *kp = ps + h * 8 * NB;
-            if constexpr (NB == 2) ks[h][0] = __ldg(reinterpret_cast<const uint16_t *>(kp));
-            else if constexpr (NB == 4) ks[h][0] = __ldg(reinterpret_cast<const uint32_t *>(kp));
-            else { const uint2 u = __ldg(reinterpret_cast<const uint2 *>(kp)); ks[h][0] = u.x; ks[h][1] = u.y; }
+#pragma unroll
+            for (int c = 0; c < NCH; c++) cp_async<CB>(st + ((h * NCH + c) * 32 + lane) * CB, pk + h * 8 * (DH / 2) + c * CB);
+            cp_async<SB>(st + CODES + (h * 32 + lane) * SB, pks + h * 8 * NB);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            cp_async<SB>(st + CODES + ((2 + h) * 32 + lane) * SB, pvs + h * 8 * NB);
+#pragma unroll
+            for (int c = 0; c < NCH; c++) cp_async<CB>(st + (((2 + h) * NCH + c) * 32 + lane) * CB, pv + h * 4 * DH + c * CB);
         }
     }
-    __device__ __forceinline__ void load_v(const uint8_t *pv, const uint8_t *ps) {
+    static __device__ __forceinline__ void get(const uint8_t *st, int half, int lane, uint32_t (&r)[W]) {
 #pragma unroll
-        for (int h = 0; h < 2; h++) ld_words<W>(pv + h * 4 * DH, v[h]);
+        for (int c = 0; c < NCH; c++) {
+            const uint8_t *p = st + ((half * NCH + c) * 32 + lane) * CB;
+            if constexpr (CB == 8) {
+                const uint2 u = *reinterpret_cast<const uint2 *>(p);
+                r[0] = u.x; r[1] = u.y;
+            } else {
+                const uint4 u = *reinterpret_cast<const uint4 *>(p);
+                r[4 * c] = u.x; r[4 * c + 1] = u.y; r[4 * c + 2] = u.z; r[4 * c + 3] = u.w;
+            }
+        }
+    }
+    __device__ __forceinline__ void get_k(const uint8_t *st, int lane) {
 #pragma unroll
-        for (int c = 0; c < VB; c++) vs[c] = __ldg(ps + c) | (uint32_t)__ldg(ps + c + 8 * NB) << 16;
+        for (int h = 0; h < 2; h++) {
+            get(st, h, lane, k[h]);
+            const uint32_t *p = reinterpret_cast<const uint32_t *>(st + CODES + (h * 32 + lane) * SB);
+            if constexpr (NB == 2) ks[h][0] = *p >> (lane & 4 ? 16 : 0);      // (the word has two tokens; what is above is not looked at)
+            else ks[h][0] = p[0];
+            if constexpr (NB == 8) ks[h][1] = p[1];
+        }
+    }
+    __device__ __forceinline__ void get_v(const uint8_t *st, int lane) {
+        get(st, 2, lane, v[0]);
+        get(st, 3, lane, v[1]);
+    }
+    __device__ __forceinline__ void get_vs(const uint8_t *st, int lane) {
+        const int j = lane & 3, word = NB == 8 ? j >> 1 : 0, first = NB == 8 ? 2 * (j & 1) : NB == 4 ? j : (lane & 4) / 2 + (j & 1);
+        const uint8_t *p = st + CODES + (2 * 32 + lane) * SB + 4 * word;
+        const uint32_t a = *reinterpret_cast<const uint32_t *>(p), b = *reinterpret_cast<const uint32_t *>(p + 32 * SB);
+#pragma unroll
+        for (int c = 0; c < VB; c++) vs[c] = __byte_perm(a, b, (first + c) * 0x11 | (first + c + 4) * 0x1100) & 0x00ff00ffu;
     }
 };
 
@@ -160,7 +191,11 @@ __device__ __forceinline__ void wide_weights(float (*Ms)[8 * NT], const uint32_t
 template <int DH, int NT, int TERMS>
 struct DecSmem {
     static constexpr int R = 8 * NT, LD = DH + 4;
-    alignas(16) float o[DEC_WARPS][R][LD];
+    // (the stages are empty when a piece's results are added up)
+    union {
+        alignas(16) float o[DEC_WARPS][R][LD];
+        alignas(16) uint8_t st[DEC_WARPS][DecFrag<DH>::STAGES][DecFrag<DH>::STAGE];
+    };
     float m[DEC_WARPS][R], l[DEC_WARPS][R], M[DEC_WARPS][DH / 32][R];      // M: the wide form's references
     alignas(16) uint16_t sc[DEC_WARPS][4][DH / 32][4];     // f16 2^(vs - anchor): [j][block][tokens 2j, 2j+1, 2j+8, 2j+9]
     alignas(16) uint4 q[TERMS][NT][DH / 32][32];           // operand fragments of q, by lane
@@ -169,9 +204,11 @@ struct DecSmem {
 };
 
 template <int DH, int NT, bool F32>
-// What bounds it: instructions, 350 per warp and 16 tokens of 128 dims, each warp issuing one in five cycles: 16 warps per SM at 128 registers
-// are better than 12 at 168 (64 requests, 266,000 tokens: 38 against 43 us), 20 at 96 spill (48); wider accumulators
-// (256 dims, or 16 rows of 128) keep 8 warps at 255 (41 us at 112,000 tokens of 256; 46 with 12 warps, 72 with 16).
+// What bounds it: instructions, 350 per warp and 16 tokens of 128 dims.  16 warps per SM at 128 registers are better than 20 at 102
+// (64 requests, 266,000 tokens: 35 against 39 us) and 12 at 168 (43); wider accumulators (256 dims, or 16 rows of 128) keep 8 warps at 255
+// (37 us at 112,000 tokens of 256; 38 with 12 warps).  Tokens come by asynchronous copies one group ahead (35 us; 38 with loads into
+// registers behind their last use), two ahead gain nothing.  The stages share their place with the results: with a place of their own, 35.3,
+// and 33.2 against 32.0 for one request of 131,072, since more shared memory leaves less of L1.
 __global__ void __launch_bounds__(DEC_THREADS, NT * DH <= 128 ? 4 : 2)
 k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restrict__ part) {
     constexpr int NB = DH / 32, R = 8 * NT, TERMS = F32 ? 2 : 1;
@@ -263,9 +300,10 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
         const int unit0 = sg.u_first + sg.u0 + first_mine;
         const uint8_t *head_base = a.kv.base + (size_t)sg.hk * a.kv.region();
         const uint32_t block_bytes = (uint32_t)(a.kv.region() * a.kv.Hkv);
-        // a lane's part of the addresses: codes of K and V, scales of K and V
-        const uint32_t lane_k = g * (DH / 2) + j * (DH / 8), lane_v = a.kv.bs * (DH / 2) + j * DH + g * (DH / 8), lane_ks = a.kv.bs * DH + g * NB,
-                       lane_vs = lane_ks + a.kv.bs * NB + (NB >= 4 ? Frag::VB * j : j & 1);
+        // a lane's part of the addresses: codes of K and V, scales of K and V (of 64 dims a token has two bytes of scales: the word with them)
+        const uint32_t sc_row = (NB == 2 ? g & ~1 : g) * NB;
+        const uint32_t lane_k = g * (DH / 2) + j * (DH / 8), lane_v = a.kv.bs * (DH / 2) + j * DH + g * (DH / 8), lane_ks = a.kv.bs * DH + sc_row,
+                       lane_vs = lane_ks + a.kv.bs * NB;
         int ids = -1;
         // group k's page and its first token there; false when the group is not there
         auto page_of = [&](int k, const uint8_t *&reg, int &t) {
@@ -278,21 +316,40 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
             reg = head_base + (size_t)(uint32_t)id * block_bytes;
             return (unsigned)id < (unsigned)a.kv.n_blocks;
         };
-        // K of the next group is asked for when this group's has been used, V likewise: no second set of registers
+        // Groups are asked for one ahead; `there`: a bit per stage, whether its group exists.
+        constexpr int ST = Frag::STAGES;
         Frag f;
-        const uint8_t *reg = head_base;
-        int t_in = 0;
-        bool ok = n_mine > 0 && page_of(0, reg, t_in), ok_next = false;
-        if (ok) {
-            f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
-            f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
-        }
+        uint32_t there = 0;
+        uint8_t *stages = sm.st[warp][0];
+        auto ask = [&](int k) {
+            const uint8_t *reg;
+            int t;
+            const uint32_t s = (uint32_t)k % ST;
+            const bool is = k < n_mine && page_of(k, reg, t);
+            if (is)
+                Frag::copy((uint32_t)__cvta_generic_to_shared(stages) + s * Frag::STAGE, reg + t * (DH / 2) + lane_k, reg + t * (DH / 2) + lane_v, reg + t * NB + lane_ks,
+                           reg + t * NB + lane_vs, lane);
+            cp_commit();
+            there = (there & ~(1u << s)) | (uint32_t)is << s;
+        };
+        const uint8_t *st = stages;
+        // group k's stage, and whether there is anything in it
+        auto arrive = [&](int k) {
+            ask(k + ST - 1);
+            cp_wait<ST - 1>();
+            const uint32_t s = (uint32_t)k % ST;
+            st = stages + s * Frag::STAGE;
+            return (there >> s & 1) != 0;
+        };
+#pragma unroll
+        for (int k = 0; k < ST - 1; k++) ask(k);
         int k = 0, tok = 0;
         bool inner = false;
         float s[NT][4];
         uint32_t w[TERMS][NT][2];
-        // S of the group (log2 units), -infinity where a row does not see the token; K of the next one asked for; m moved when needed
+        // S of the group (log2 units), -infinity where a row does not see the token; m moved when needed
         auto scores = [&](bool with_o) {
+            f.get_k(st, lane);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -319,7 +376,6 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                     s[nt][3] = fmaf(c[3], sc1, s[nt][3]);
                 }
             }
-            if (ok_next) f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -366,15 +422,8 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
         };
 #pragma unroll 1
         for (; k < n_mine; k++) {
-            ok_next = k + 1 < n_mine && page_of(k + 1, reg, t_in);
-            if (!ok) {
-                if (ok_next) {
-                    f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
-                    f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
-                }
-                ok = ok_next;
-                continue;
-            }
+            if (!arrive(k)) continue;
+            f.get_vs(st, lane);
             tok = (unit0 + k) * DEC_UNIT;
             inner = tok >= all_lo && tok + DEC_UNIT - 1 <= all_hi;
             // V exponents (own: tokens g, g + 8, blocks VB j ..): inside the window?  vs - (anchor - 8) of both tokens at once (a
@@ -427,6 +476,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                 l[nt][1] += p[1] + p[3];
                 weights_f16<TERMS>(p, w, nt);
             }
+            f.get_v(st, lane);
             __syncwarp();
 #pragma unroll
             for (int b2 = 0; b2 < NB / 2; b2++) {
@@ -447,8 +497,6 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                         }
                 }
             }
-            if (ok_next) f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
-            ok = ok_next;
         }
         const bool wide = k < n_mine;
         if (wide) {
@@ -462,15 +510,9 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
             __syncwarp();
 #pragma unroll 1
             for (bool fresh = true; k < n_mine; k++, fresh = false) {
-                if (!fresh) ok_next = k + 1 < n_mine && page_of(k + 1, reg, t_in);      // (the first group's has been looked up)
-                if (!ok) {
-                    if (ok_next) {
-                        f.load_k(reg + t_in * (DH / 2) + lane_k, reg + t_in * NB + lane_ks);
-                        f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
-                    }
-                    ok = ok_next;
-                    continue;
-                }
+                if (!fresh && !arrive(k)) continue;      // (the first group is there)
+                f.get_vs(st, lane);
+                f.get_v(st, lane);
                 tok = (unit0 + k) * DEC_UNIT;
                 inner = tok >= all_lo && tok + DEC_UNIT - 1 <= all_hi;
                 scores(false);
@@ -495,8 +537,6 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                                     mma_f16(o[nt][b][u], ev[0][2 * bb + u], od[0][2 * bb + u], ev[1][2 * bb + u], od[1][2 * bb + u], w[t][nt][0], w[t][nt][1]);
                     }
                 }
-                if (ok_next) f.load_v(reg + t_in * (DH / 2) + lane_v, reg + t_in * NB + lane_vs);
-                ok = ok_next;
             }
         }
 

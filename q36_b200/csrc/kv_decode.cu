@@ -309,7 +309,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
         auto page_of = [&](int k, const uint8_t *&reg, int &t) {
             if ((k & 31) == 0) {
                 const int col = (unit0 + k + lane) * DEC_UNIT >> a.kv.log_bs;
-                ids = k + lane < n_mine && col < a.max_blocks ? __ldg(row + col) : -1;
+                ids = k + lane < n_mine && col < a.max_blocks ? row[col] : -1;
             }
             const int id = __shfl_sync(0xffffffffu, ids, k & 31);
             t = (unit0 + k) * DEC_UNIT & (a.kv.bs - 1);

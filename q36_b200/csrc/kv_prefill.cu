@@ -206,9 +206,9 @@ struct PfBars { uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], s_full[2]
 // 1, 2 or 4 bytes
 template <int BYTES>
 __device__ __forceinline__ uint32_t ld_part(const uint8_t *p) {
-    if constexpr (BYTES == 1) return __ldg(p);
-    else if constexpr (BYTES == 2) return __ldg(reinterpret_cast<const uint16_t *>(p));
-    else return __ldg(reinterpret_cast<const uint32_t *>(p));
+    if constexpr (BYTES == 1) return *p;
+    else if constexpr (BYTES == 2) return *reinterpret_cast<const uint16_t *>(p);
+    else return *reinterpret_cast<const uint32_t *>(p);
 }
 
 template <int DH>
@@ -321,7 +321,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
 #pragma unroll
                     for (int k = 0; k < 8; k++) off[k] = __shfl_sync(0xffffffffu, q_off, (k0 + k) * RPI + lane / CPR);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = __ldg(reinterpret_cast<const uint4 *>(q + (off[k] < 0 ? q_first : off[k])));
+                    for (int k = 0; k < 8; k++) v[k] = *reinterpret_cast<const uint4 *>(q + (off[k] < 0 ? q_first : off[k]));
 #pragma unroll
                     for (int k = 0; k < 8; k++) {
                         const uint32_t keep = off[k] < 0 ? 0u : ~0u;
@@ -501,7 +501,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
             const int *row = a.table + (size_t)pos.b * a.max_blocks;
             auto page = [&](int j) {
                 const int t = j * KT + tl, col = t >> a.kv.log_bs;
-                return j < g.j1 && t < pos.s.len && col < a.max_blocks ? __ldg(row + col) : -1;
+                return j < g.j1 && t < pos.s.len && col < a.max_blocks ? row[col] : -1;
             };
             constexpr int RAW = BPT == 1 ? 8 : 4 * BPT;
             struct Half { uint32_t w[RAW], scale; bool has; };
@@ -516,13 +516,13 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
 #pragma unroll
                     for (int q = 0; q < 4; q++) {       // word q of every block
                         if constexpr (BPT == 4) {
-                            const uint4 u = __ldg(reinterpret_cast<const uint4 *>(src + q * (DH / 8)));
+                            const uint4 u = *reinterpret_cast<const uint4 *>(src + q * (DH / 8));
                             f.w[4 * q] = u.x; f.w[4 * q + 1] = u.y; f.w[4 * q + 2] = u.z; f.w[4 * q + 3] = u.w;
                         } else if constexpr (BPT == 2) {
-                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
+                            const uint2 u = *reinterpret_cast<const uint2 *>(src + q * (DH / 8));
                             f.w[2 * q] = u.x; f.w[2 * q + 1] = u.y;
                         } else {
-                            f.w[q] = __ldg(reinterpret_cast<const uint32_t *>(src + q * (DH / 8)));
+                            f.w[q] = *reinterpret_cast<const uint32_t *>(src + q * (DH / 8));
                         }
                     }
                 } else {
@@ -530,7 +530,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
 #pragma unroll
                     for (int q = 0; q < 8; q++) {       // four dims of every block
                         if constexpr (BPT == 4) {
-                            const uint2 u = __ldg(reinterpret_cast<const uint2 *>(src + q * (DH / 8)));
+                            const uint2 u = *reinterpret_cast<const uint2 *>(src + q * (DH / 8));
                             f.w[2 * q] = u.x; f.w[2 * q + 1] = u.y;
                         } else {
                             f.w[q] = ld_part<2 * BPT>(src + q * (DH / 8));

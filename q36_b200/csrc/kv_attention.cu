@@ -105,7 +105,7 @@ __device__ __forceinline__ void join_store(const AttnArgs &a, const AttnPart &d,
 constexpr int JOIN_WIDE = 256;
 template <int DH>
 __global__ void __launch_bounds__(JOIN_WIDE)
-k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
+k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *desc, const float *part) {
     Q36_GDS();
     constexpr int N4 = (DH + 127) / 128, WARPS = JOIN_WIDE / 32;      // 16-byte pieces of a row per lane
     extern __shared__ float w[];                                      // one weight per piece, then the list
@@ -153,7 +153,7 @@ k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ de
 // (three chunks of up to 777 tokens on up to 6000 beside 37 single tokens: 14.5 us, 25 with a row at a time).
 template <int DH>
 __global__ void __launch_bounds__(JOIN_THREADS)
-k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *__restrict__ desc, const float *__restrict__ part) {
+k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *desc, const float *part) {
     Q36_GDS();
     constexpr int N4 = (DH + 127) / 128, WARPS = JOIN_THREADS / 32, RB = 4;
     extern __shared__ int list[];

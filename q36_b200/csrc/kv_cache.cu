@@ -36,7 +36,7 @@ __device__ __forceinline__ int bisect(const int *pre, int n, int v) {
 }
 
 __global__ void __launch_bounds__(TB_THREADS)
-k_kv_tables(const int *kv_old, const int *__restrict__ q_len, int B, int log_bs, int n_blocks, const int *__restrict__ free_blocks,
+k_kv_tables(const int *kv_old, const int *q_len, int B, int log_bs, int n_blocks, const int *free_blocks,
             int n_free, const int *free_head, int *block_table, int max_blocks, int *__restrict__ cu_q, int *kv_len,
             int *__restrict__ slots, int *__restrict__ positions, int T, int *free_head_out, int *status) {
     Q36_GDS();
@@ -189,7 +189,7 @@ __device__ __forceinline__ uint32_t quant8(float (&x)[8], int &e2) {
     return f32x8_to_e2m1(x);
 }
 __global__ void __launch_bounds__(KVC_THREADS)
-k_kv_append(const void *__restrict__ k, const void *__restrict__ v, int bf16, long long ks, long long vs, const int *__restrict__ slots, KvGeom g,
+k_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g,
             RowDiv div, unsigned n8) {
     Q36_GDS();
     const unsigned i = blockIdx.x * KVC_THREADS + threadIdx.x;
@@ -233,7 +233,7 @@ __device__ __forceinline__ void store8_exact(void *p, size_t at, int bf16, uint3
     }
 }
 __global__ void __launch_bounds__(KVC_THREADS)
-k_kv_read(KvGeom g, const int *__restrict__ slots, void *__restrict__ k, void *__restrict__ v, int bf16, RowDiv div, unsigned n8) {
+k_kv_read(KvGeom g, const int *slots, void *__restrict__ k, void *__restrict__ v, int bf16, RowDiv div, unsigned n8) {
     Q36_GDS();
     const unsigned i = blockIdx.x * KVC_THREADS + threadIdx.x;
     if (i >= n8) return;

@@ -103,7 +103,7 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __global__ void __launch_bounds__(LS_THREADS)
-k_linear_few(const uint16_t *__restrict__ x, long long xs, const uint16_t *__restrict__ w, Epilogue e, int T, int N, int K, const int *rows_used) {
+k_linear_few(const uint16_t *x, long long xs, const uint16_t *__restrict__ w, Epilogue e, int T, int N, int K, const int *rows_used) {
     constexpr int U = 8;      // steps of 32 k in flight
     cudaTriggerProgrammaticLaunchCompletion();
     __shared__ float red[LS_WARPS][8][LS_COLS + 1];

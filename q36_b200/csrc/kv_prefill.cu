@@ -46,6 +46,10 @@ constexpr float PF_GROW = 8.f;
 // 577, 192 450, 384 373, 512 374, 768 379.
 constexpr int PF_SPAN = 448;
 constexpr int PF_MIN = 1024;        // the smallest range of a CTA
+// Places for the bad pages of a tile, which go from the group that widens K to the softmax without a barrier of their own.  K runs up to 9
+// tiles ahead of a softmax: behind a span whose second row tile is empty, that tile's issuers pass the stages on, so only V holds K back.
+// K's tile X + 10 needs S of X + 6, that the product of X + 4, that V of X + 4, that the second row tile's product of X, and that its softmax of X.
+constexpr int PF_BAD_RING = 16;
 __device__ int g_prefill_status;         // where a wait gave up (0: nowhere)
 
 // ---------------------------------------------------------------- plan
@@ -222,7 +226,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
     extern __shared__ uint8_t raw[];
     uint8_t *smem = (uint8_t *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
     __shared__ PfBars bars;
-    __shared__ uint32_t tmem_s, bad_s[8][2];      // bad_s: tokens of a tile whose page is bad; a ring of 8: K runs up to 5 tiles ahead of the softmax
+    __shared__ uint32_t tmem_s, bad_s[PF_BAD_RING][2];      // bad_s: tokens of a tile whose page is bad
     __shared__ volatile int abort_flag;
     __shared__ long long plan_sum[PF_THREADS / 32], plan_base;
     __shared__ int plan_b;
@@ -345,7 +349,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
                     __syncwarp();
                     tc_fence_after();
                     const uint32_t s_col = tmem + lanes + (2 * i + x) * C::TM_S;
-                    const uint32_t st = (kt + (j - g.j0)) & 7;       // its place in bad_s
+                    const uint32_t st = (kt + (j - g.j0)) % PF_BAD_RING;       // its place in bad_s
                     uint32_t bad = 0;
 #pragma unroll
                     for (int w = 0; w < KT / 32; w++) bad |= bad_s[st][w];
@@ -567,7 +571,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
                 if (!is_v && half == 0) {
                     // tokens of the request whose page is bad
                     const uint32_t bad = __ballot_sync(0xffffffffu, !cur.has && j * KT + tl < pos.s.len);
-                    if (lane == 0) bad_s[kc & 7][tl >> 5] = bad;
+                    if (lane == 0) bad_s[kc % PF_BAD_RING][tl >> 5] = bad;
                 }
                 cur = nxt;
                 nxt = far;

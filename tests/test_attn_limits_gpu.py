@@ -1,0 +1,52 @@
+"""The attention side of a layer at the limits of what it takes, against plain 64-bit forms; bounds as in test_attn_gpu.py."""
+import numpy as np
+import pytest
+
+import attn_ref as R
+from test_attn_gpu import Setup, cu, ints
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def attn(moe):
+    from q36_b200 import attn
+    return attn
+
+
+def own_rows(s, k, v):
+    """The cached rows of a Setup's requests, all of them, replaced."""
+    tab = s.table.cpu().numpy()
+    slots = ints(np.concatenate([tab[b, np.arange(n) // s.bs] * s.bs + np.arange(n) % s.bs for b, (_, n) in enumerate(s.lens)]))
+    s.kv.append(cu(np.asarray(k, np.float32)), cu(np.asarray(v, np.float32)), slots)
+    s.k, s.v = (t.double().cpu().numpy() for t in s.kv.read(slots))
+
+
+@pytest.mark.parametrize("Dh", [64, 128])
+def test_bad_pages_behind_a_half_empty_row_tile(attn, Dh):
+    """Requests of 32 + 16 new tokens of 8 heads: a row tile of 256 rows, then one whose second half has none, on the same CTA.  The second
+    half of the first one is slow (its rows' scores grow by 2^9 a tile or so, so that the sums move with every tile), and pages of its
+    last tiles and of the next row tile's first ones are bad, each tile in a pattern of its own."""
+    import torch
+    rng = np.random.default_rng(17)
+    s = Setup(attn, rng, [(48, int(n)) for n in rng.integers(2740, 3400, 40)], 16, 2, Dh, 16, "bf16")
+    half = Dh // 2
+    k, v = rng.standard_normal((len(s.k), 2, Dh)), rng.standard_normal((len(s.k), 2, Dh))
+    tile = np.concatenate([np.arange(n) // 64 * half / (n // 64 + 1) for _, n in s.lens])
+    k[:, :, :half] = np.arange(half) < tile[:, None, None]
+    own_rows(s, k, v)
+    grows = torch.arange(s.T, device="cuda") % 48
+    s.q[:, :, :half] = torch.where((grows >= 16) & (grows < 32), 1.0, -1.0)[:, None, None] * 6.5 * Dh ** 0.5
+    drop = []
+    for b, (_, n) in enumerate(s.lens):
+        pages = -(-n // 16)
+        bad = np.zeros(pages, bool)
+        bad[1:48], bad[-24:-1] = rng.random(47) < 0.4, rng.random(23) < 0.4
+        s.table[b, :pages][torch.from_numpy(bad).cuda()] = int(rng.choice([-1, s.n_blocks, 2**31 - 1]))
+        drop.append(bad.repeat(16)[:n])
+    first = s.run()
+    s.check(first, drop=drop)
+    for _ in range(50):
+        out, lse = s.run()
+        assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
+    attn.check_device_status()

@@ -9,7 +9,9 @@
  * The conventions are those of q36_moe.h: device pointers, launch-only (no host
  * synchronisation, no allocation, capturable in a CUDA graph), a stream per
  * call, a Q36_MOE_* status back.  The library keeps no state between calls;
- * calls that may run at the same time need a workspace each.  Pointers, and
+ * calls that may run at the same time need a workspace each, and so do calls
+ * that two host threads make at a time, on one stream too: a call is several
+ * launches, which hand partial results over in it.  Pointers, and
  * the rows that strides lead to, must lie on 16 bytes where a 16-byte vector
  * is read or written: q, k, v, x, w, out, the cache and the workspace.
  *

@@ -9,6 +9,7 @@ from __future__ import annotations
 import contextlib
 import ctypes as C
 import functools
+import threading
 from typing import NamedTuple
 
 import torch
@@ -183,6 +184,9 @@ def kv_tables(kv_old, q_len, block_size, free_blocks, free_head, block_table, T,
     return out
 
 
+_NO_LOCK = contextlib.nullcontext()      # (a caller with a workspace of its own)
+
+
 class KVCache:
     """The paged 4-bit cache of one layer: uint8 [n_blocks, n_kv_head, bytes]."""
 
@@ -196,15 +200,16 @@ class KVCache:
         self._data, self.device, self._dev = data, data.device, data.get_device()
         self.n_blocks, self.block_size, self.n_kv_head, self.head_dim = n_blocks, block_size, n_kv_head, head_dim
         self._geom = (data.data_ptr(), n_blocks, block_size)
-        self._ws = {}
+        self._ws, self._lock = {}, threading.Lock()
 
     @property
     def data(self) -> torch.Tensor:
         return self._data
 
     def _scratch(self, nbytes: int, st: int) -> torch.Tensor:
-        """Scratch of a call; one per stream, since calls on two streams may run at the same time.  Under capture a graph
-        gets one of its own, which it keeps: replays of two graphs may run at the same time too."""
+        """Scratch of a call; one per stream, since calls on two streams may run at the same time.  Calls of two threads on one
+        stream hold the lock from here to their last launch: a call's launches hand its parts over in here, and another call's may not
+        come between them.  Under capture a graph gets one of its own, which it keeps: replays of two graphs may run at the same time too."""
         if torch.cuda.is_current_stream_capturing():
             return torch.empty(nbytes, dtype=_U8, device=self.device)
         ws = self._ws.get(st)
@@ -270,9 +275,10 @@ class KVCache:
             if out is None:
                 out = _rows(T, h, d, q.dtype, self.device)
             lse = torch.empty((T, h), dtype=_F32, device=self.device) if want_lse else None
-            if ws is None:
-                ws = self._scratch(_attention_ws(self._dev, h, self.n_kv_head, d, max(max_q, 1)), st)
-            rc = lib.q36_kv_attention(q.data_ptr(), bf, qs, *args, out.data_ptr(), os_, ptr(lse), T, max_q, ws.data_ptr(), ws.numel(), st)
+            with self._lock if ws is None else _NO_LOCK:
+                if ws is None:
+                    ws = self._scratch(_attention_ws(self._dev, h, self.n_kv_head, d, max(max_q, 1)), st)
+                rc = lib.q36_kv_attention(q.data_ptr(), bf, qs, *args, out.data_ptr(), os_, ptr(lse), T, max_q, ws.data_ptr(), ws.numel(), st)
             if rc:
                 check(rc, what)
         return (out, lse) if want_lse else out
@@ -293,10 +299,11 @@ class KVCache:
         bf, qs = _is_bf16(q, what), _rows3(q, n_head, self.head_dim, what)
         ks, vs = (_rows3(t, self.n_kv_head, self.head_dim, what) for t in (k, v))
         with _call(dev, stream) as st:
-            if ws is None:
-                ws = self._scratch(_block_ws(dev, T, n_head, self.n_kv_head, self.head_dim, max(max_q, 1)), st)
-            rc = lib.q36_attn_block(q.data_ptr(), k.data_ptr(), v.data_ptr(), bf, qs, ks, vs, slots.data_ptr(), *args, w_o.data_ptr(), ptr(bias_o),
-                                    h.data_ptr(), D, T, max_q, ws.data_ptr(), ws.numel(), st)
+            with self._lock if ws is None else _NO_LOCK:
+                if ws is None:
+                    ws = self._scratch(_block_ws(dev, T, n_head, self.n_kv_head, self.head_dim, max(max_q, 1)), st)
+                rc = lib.q36_attn_block(q.data_ptr(), k.data_ptr(), v.data_ptr(), bf, qs, ks, vs, slots.data_ptr(), *args, w_o.data_ptr(), ptr(bias_o),
+                                        h.data_ptr(), D, T, max_q, ws.data_ptr(), ws.numel(), st)
             if rc:
                 check(rc, what)
         return h

@@ -50,3 +50,35 @@ def test_bad_pages_behind_a_half_empty_row_tile(attn, Dh):
         out, lse = s.run()
         assert torch.equal(out, first[0]) and torch.equal(lse, first[1])
     attn.check_device_status()
+
+
+def test_two_threads_on_one_stream(attn):
+    """Different requests on the same cache and the same (default) stream from two host threads: the bits of one thread alone."""
+    import threading
+    import torch
+    rng = np.random.default_rng(18)
+    a = Setup(attn, rng, [(1, int(n)) for n in rng.integers(500, 3000, 40)], 16, 2, 128, 16, "bf16")
+    b = Setup(attn, rng, [(1, 9000), (3, 20), (300, 4000)], 16, 2, 128, 16, "bf16")
+    both = attn.KVCache(a.n_blocks + b.n_blocks, 16, 2, 128, data=torch.cat([a.kv.data, b.kv.data]))
+    b.table = torch.where((b.table >= 0) & (b.table < b.n_blocks), b.table + a.n_blocks, -1)
+    a.table = torch.where(a.table < a.n_blocks, a.table, -1)
+    a.kv = b.kv = both
+    want = [s.run() for s in (a, b)]
+    a.check(want[0])
+    got = [[], []]
+    start = threading.Barrier(2)
+
+    def work(i, s):
+        start.wait()
+        for _ in range(200):
+            got[i].append(s.run())
+
+    threads = [threading.Thread(target=work, args=(i, s)) for i, s in enumerate((a, b))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert len(got[i]) == 200
+        assert all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i])

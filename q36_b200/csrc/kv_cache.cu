@@ -297,7 +297,8 @@ int q36_kv_tables(const int *kv_old, const int *q_len, int n_seq, int block_size
     const int smem = 2 * (n_seq + 1) * 4;
     static bool attr_done[MAX_DEVICES] = {false};
     int rc;
-    if (smem > 48 * 1024 && (rc = ensure_smem_attr((const void *)k_kv_tables, 2 * (TB_MAX_SEQ + 1) * 4, attr_done))) return rc;
+    // (whatever the size: the limit without it, 48 KB, counts the kernel's static arrays too)
+    if ((rc = ensure_smem_attr((const void *)k_kv_tables, 2 * (TB_MAX_SEQ + 1) * 4, attr_done))) return rc;
     const long work = (long)T + n_seq;
     // in place: one block, since another could read what it has written
     const bool in_place = kv_len == kv_old || free_head_out == free_head;

@@ -82,3 +82,31 @@ def test_two_threads_on_one_stream(attn):
     for i in range(2):
         assert len(got[i]) == 200
         assert all(torch.equal(o, want[i][0]) and torch.equal(l, want[i][1]) for o, l in got[i])
+
+
+def tables_of(attn, B):
+    """Tables of B requests, every entry."""
+    import torch
+    rng = np.random.default_rng(B)
+    old, new = rng.integers(0, 60, B), np.where(rng.random(B) < 0.02, rng.integers(0, 40, B), 1)
+    T, width, free = int(new.sum()) + 3, 8, 3 * B
+    ids = rng.permutation(free + B * width).astype(np.int32)
+    table = ids[free:].reshape(B, width)
+    want = R.tables(old.tolist(), new.tolist(), 16, ids[:free].tolist(), 2, table, T, len(ids))
+    t = ints(table)
+    g = attn.kv_tables(ints(old), ints(new), 16, ints(ids[:free]), ints([2]), t, T, n_blocks=len(ids))
+    for got, exp in zip((t, g.cu_q, g.kv_len, g.slots, g.positions, g.free_head, g.status), want):
+        np.testing.assert_array_equal(got.cpu().numpy().reshape(np.shape(exp)), exp)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("B", [6127, 6143, 6144, 16384])
+def test_tables_of_many_requests_as_a_process_first_call(B):
+    """Sizes around 48 KB of shared memory, the limit of a launch that has not asked for more, and the largest."""
+    import os
+    import subprocess
+    import sys
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = f"import sys; sys.path[:0] = {[here, os.path.dirname(here)]!r}; from test_attn_limits_gpu import tables_of; from q36_b200 import attn; tables_of(attn, {B})"
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

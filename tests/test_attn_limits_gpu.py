@@ -110,3 +110,24 @@ def test_tables_of_many_requests_as_a_process_first_call(B):
     code = f"import sys; sys.path[:0] = {[here, os.path.dirname(here)]!r}; from test_attn_limits_gpu import tables_of; from q36_b200 import attn; tables_of(attn, {B})"
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+@pytest.mark.parametrize("Dh", [64, 128, 256])
+def test_tiny_values_beside_ordinary_ones(attn, Dh, x):
+    """V blocks of about 1e-38, whose scale byte is that of a block of zeros, and blocks of zeros among blocks of about 1: token by token, in
+    all tokens of a block of dims, and in a request's first tokens."""
+    rng = np.random.default_rng(19)
+    s = Setup(attn, rng, [(1, 777), (40, 300), (1, 64), (1, 500), (200, 6000)], 16, 2, Dh, 32, x)
+    n, nb = len(s.k), Dh // 32
+    size = rng.choice([1.0, 1.0, 1e-38, 0.0], (n, 2, nb))
+    size[:, 0, 0] = 1e-38
+    size[777:1077] = np.where(size[777:1077] == 1.0, 1.0, 1e-38)
+    size[1141:1141 + 40] = np.where(np.arange(40) % 2, 1e-38, 0.0)[:, None, None]
+    size[1141 + 40:1641] = 1.0
+    own_rows(s, rng.standard_normal((n, 2, Dh)), rng.standard_normal((n, 2, Dh)) * size.repeat(32, -1))
+    assert 0 < np.abs(s.v[:1077, 0, :32]).max() < 1e-36
+    got = s.run()
+    s.check(got)
+    tiny = got[0].float().cpu().numpy()[:41, :8, :32]                            # kv head 0, block 0: tiny in every token of requests 0 and 1
+    assert np.abs(tiny).max() < 1e-36

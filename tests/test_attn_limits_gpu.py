@@ -131,3 +131,45 @@ def test_tiny_values_beside_ordinary_ones(attn, Dh, x):
     s.check(got)
     tiny = got[0].float().cpu().numpy()[:41, :8, :32]                            # kv head 0, block 0: tiny in every token of requests 0 and 1
     assert np.abs(tiny).max() < 1e-36
+
+
+def act64(v, act):
+    """The activations in 64 bits, without cancellation; their limit at -infinity."""
+    from math import erfc
+    with np.errstate(over="ignore", invalid="ignore"):
+        u = 2 * np.sqrt(2 / np.pi) * (v + 0.044715 * v ** 3)
+        y = {"none": lambda: v, "relu": lambda: np.maximum(v, 0), "silu": lambda: v / (1 + np.exp(-v)), "gelu_tanh": lambda: v / (1 + np.exp(-u)),
+             "gelu": lambda: 0.5 * v * np.vectorize(erfc)(-v / np.sqrt(2))}[act]()
+    return np.where((v == -np.inf) & (act != "none"), 0.0, y), v if act == "silu" else u
+
+
+@pytest.mark.parametrize("y", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 260])
+@pytest.mark.parametrize("act", ["none", "relu", "silu", "gelu", "gelu_tanh"])
+def test_activations_of_sums_of_any_size(attn, act, T, y):
+    """Relative to the result.  silu and gelu_tanh, in half steps 2^-24: the argument of the exponential has six roundings (gelu_tanh), its
+    base-2 form two, of |u| each, which count as they stand in a result that goes as e^u; the exponentials 2^-22 twice, the quotient
+    and the products: 20; and the last steps of the smallest numbers, 2^-149.  gelu below 0: 1 + erf in f32, 2^-20 in all."""
+    import torch
+    v = torch.tensor([-75, -100, -87.5, -95, -103, -104.5, -130, -1e4, -1e13, -1e31, -3e38, -torch.inf, -10, -6, -4, -1, -1e-30, 0, 1e-30, 0.5, 3, 12,
+                      20, 90, 130, 1e13, 1e31, 3e38, torch.inf, torch.nan]).bfloat16().cuda()
+    w = torch.zeros((len(v), 8), dtype=torch.bfloat16, device="cuda")
+    w[:, 0] = 1
+    x = torch.zeros((T, 8), dtype=torch.bfloat16, device="cuda")
+    got = np.zeros((len(v), len(v)))
+    for i in range(len(v)):                                                       # one at a time: 0 times infinity is no number
+        x[:, 0] = v[i]
+        out = attn.linear(x, w, act=act, out_dtype=torch.bfloat16 if y == "bf16" else torch.float32)
+        assert torch.equal(out.nan_to_num(7.0), out[:1].expand_as(out).nan_to_num(7.0))
+        got[i] = out[0].double().cpu().numpy()
+    vd = v.double().cpu().numpy()
+    want, u = act64(vd, act)
+    assert np.isnan(got[-1]).all()
+    for i in range(len(v) - 1):
+        if np.isinf(want[i]):
+            assert (got[i] == want[i]).all(), vd[i]
+            continue
+        rel = {"silu": 20 + 2 * abs(u[i]), "gelu_tanh": 20 + 8 * abs(u[i])}.get(act, 4) * 2.0 ** -24 if want[i] else 0.0
+        tol = rel * abs(want[i]) + 4 * 2.0 ** -149 + (2.0 ** -20 if act == "gelu" and vd[i] < 0 else 0.0)
+        tol += (2.0 ** -8 * abs(want[i]) + 2.0 ** -134) if y == "bf16" else 0.0
+        assert (np.abs(got[i] - want[i]) <= tol).all(), (vd[i], got[i][0], want[i], tol)

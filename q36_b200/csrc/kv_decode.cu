@@ -11,7 +11,7 @@
 // below 2^11, so the strongest token of any block of dims has at least 2^-1 there and f16 is precise down to 2^-14.
 // When an exponent leaves the window (a block of V 2^8 times weaker, 2^4 times stronger than the first tokens'), the warp goes over
 // to a reference per row and block of dims and rounds the weights of every block by themselves, which holds for any exponents.
-// Blocks of zeros need no place in the window: scale byte 1 and no code but zero (values up to 6 * 2^-126 have that byte too, and do).
+// Blocks of scale byte 1 need no place in the window: zeros, or values up to 6 * 2^-126, which count as zeros beside an anchor 2^9 or more above.
 // The normaliser is the sum of the unrounded weights in f32.
 // q enters as f16 after an exact power of two per row (bf16 and f16 fit); f32 activations enter as two f16 terms, and so do
 // their weights, which leaves 2^-22.
@@ -31,6 +31,7 @@ constexpr int DEC_WARPS = 4, DEC_THREADS = 32 * DEC_WARPS, DEC_UNIT = 16;
 constexpr float DEC_NONE = -3.0e38f;      // "no token yet" of the running references: finite, so that differences stay defined
 constexpr float DEC_TOP = 7.f, DEC_MAX = 11.f;        // log2 of the largest weight when the reference moves, and when it has to
 constexpr int DEC_WIN_LO = 8, DEC_WIN_HI = 4;         // window of V exponents around the anchor
+constexpr uint32_t DEC_NO_BLOCK = 32 - (15 - DEC_WIN_LO);     // the place in the window whose f16 factor is -0
 constexpr float DEC_WIDE_TOP = 11.f, DEC_WIDE_MAX = 15.f;   // the same with a reference per block of dims
 
 // the four bytes of w, two E2M1 codes each (low nibble first), as f16x2
@@ -146,20 +147,6 @@ struct DecFrag {
     __device__ __forceinline__ void get_v(const uint8_t *st, int lane) {
         get(st, 2, lane, v[0]);
         get(st, 3, lane, v[1]);
-    }
-    // Which blocks of V have a code other than zero: bit c (bit 4 + c) for block VB j + c of token g (g + 8), where vs has its scale.  v is there.
-    __device__ __forceinline__ uint32_t v_blocks(int lane) const {
-        uint32_t has = 0;      // bit NB t + b: block b of token 2j, 2j + 1, 2j + 8, 2j + 9
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-                if (v[t >> 1][(t & 1) * (NB / 2) + b / 2] >> (16 * (b & 1)) & 0x7777u) has |= 1u << (NB * t + b);
-#pragma unroll
-        for (int x = 4; x < 32; x <<= 1) has |= __shfl_xor_sync(0xffffffffu, has, x);      // the eight lanes have four dims each
-        const int g = lane >> 2, j = lane & 3, first = NB >= 4 ? VB * j : j & 1;
-        has = __shfl_sync(0xffffffffu, has, g >> 1) >> (NB * (g & 1) + first);
-        return (has & ((1u << VB) - 1)) | (has >> (2 * NB) & ((1u << VB) - 1)) << 4;
     }
     __device__ __forceinline__ void get_vs(const uint8_t *st, int lane) {
         const int j = lane & 3, word = NB == 8 ? j >> 1 : 0, first = NB == 8 ? 2 * (j & 1) : NB == 4 ? j : (lane & 4) / 2 + (j & 1);
@@ -458,15 +445,14 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
             }
             if (__any_sync(0xffffffffu, far != 0)) {
                 bool out = false;
-                f.get_v(st, lane);
-                const uint32_t codes = f.v_blocks(lane);
 #pragma unroll
                 for (int c = 0; c < Frag::VB; c++) {
                     const int v0 = f.vs[c] & 0xffff, v1 = f.vs[c] >> 16, e0 = v0 - anchor + DEC_WIN_LO, e1 = v1 - anchor + DEC_WIN_LO;
-                    out |= seen(0) && (v0 > 1 || (codes >> c & 1)) && (unsigned)e0 > (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
-                    out |= seen(1) && (v1 > 1 || (codes >> c & 16)) && (unsigned)e1 > (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
-                    // (a block of zeros, or a token that no row sees: any finite factor)
-                    d[c] = (uint32_t)min(max(e0, 0), DEC_WIN_LO + DEC_WIN_HI) | (uint32_t)min(max(e1, 0), DEC_WIN_LO + DEC_WIN_HI) << 16;
+                    const bool in0 = (unsigned)e0 <= (unsigned)(DEC_WIN_LO + DEC_WIN_HI), in1 = (unsigned)e1 <= (unsigned)(DEC_WIN_LO + DEC_WIN_HI);
+                    out |= seen(0) && v0 > 1 && !in0;
+                    out |= seen(1) && v1 > 1 && !in1;
+                    // (scale byte 1, or a token that no row sees: a factor of -0)
+                    d[c] = (in0 ? (uint32_t)e0 : DEC_NO_BLOCK) | (in1 ? (uint32_t)e1 : DEC_NO_BLOCK) << 16;
                 }
                 if (__any_sync(0xffffffffu, out)) break;
             }

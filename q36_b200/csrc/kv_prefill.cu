@@ -42,6 +42,7 @@ struct PfCfg {
 };
 constexpr float PF_NONE = -3.0e38f;      // "no token yet": finite, so that differences stay defined
 constexpr float PF_GROW = 8.f;
+constexpr float PF_LARGE = 1 << 20;
 // What a span costs beside its tokens (Q in, results out, the pipeline's start), in tokens.  Prompt of 8192, 2 x 256 spans: us at 1
 // 577, 192 450, 384 373, 512 374, 768 379.
 constexpr int PF_SPAN = 448;
@@ -339,7 +340,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
             }
             const int p = pos.s.len - pos.s.n + tok_i;              // position; the row sees [lo_r, p]
             const int hi_r = mine ? p : -1, lo_r = a.window > 0 ? p - a.window + 1 : 0;
-            float m = PF_NONE, l = 0.f;
+            float m = PF_NONE, l = 0.f, limit = PF_NONE;       // limit: what a score must pass to move m
             if (active) {
                 const int t_first = min((pos.rt * pos.s.c * a.G + i * 128) / a.G, pos.s.n - 1), t_last = min((pos.rt * pos.s.c * a.G + min(i * 128 + 127, rows - 1)) / a.G, pos.s.n - 1);
                 const int all_hi = pos.s.len - pos.s.n + t_first, all_lo = a.window > 0 ? pos.s.len - pos.s.n + t_last - a.window + 1 : 0;
@@ -382,11 +383,24 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
 #pragma unroll
                     for (int c = 1; c < KT / 32; c++) mx = fmaxf(mx, mc[c]);
                     const float top = mx == -INFINITY ? mx : mx * scale2;
-                    const bool grow = top > m + PF_GROW;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float mn = grow ? top : m, f = pf_ex2(m - mn);
+                    float k1 = scale2, m1 = -m;
+                    if (__any_sync(0xffffffffu, top > limit)) {
+                        const float mn = top > m + PF_GROW ? top : m, f = pf_ex2(m - mn);
                         l *= f;
                         m = mn;
+                        m1 = -m;
+                        limit = m + PF_GROW;
+                        // The multiply-add below rounds once where m has been rounded already: it is off by up to 2^-24 |m|.  So large scores are
+                        // rounded first, like m, in every tile of these rows.
+                        if (__any_sync(0xffffffffu, fabsf(m) >= PF_LARGE && m != PF_NONE)) {
+                            limit = -INFINITY;
+                            k1 = 1.f;
+                            m1 = 0.f;
+#pragma unroll
+                            for (int c = 0; c < KT / 32; c++)
+#pragma unroll
+                                for (int e = 0; e < 32; e++) v[c][e] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(v[c][e]), scale2), m));
+                        }
                         if (j > g.j0) {
                             // O holds the tiles before this one
                             if (!(ok = mbar_wait(bar(bars.o_done[i][x ^ 1]), ((sc - 1) >> 1) & 1, &abort_flag, &g_prefill_status, 0x600, TC_SPIN_LIMIT, 0))) break;
@@ -405,7 +419,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
                         }
                     }
                     float2 sum[4] = {{0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}, {0.f, 0.f}};
-                    const float2 k2 = {scale2, scale2}, m2 = {-m, -m};
+                    const float2 k2 = {k1, k1}, m2 = {m1, m1};
 #pragma unroll
                     for (int c = 0; c < KT / 32; c++) {
                         uint32_t w[16];

@@ -173,3 +173,32 @@ def test_activations_of_sums_of_any_size(attn, act, T, y):
         tol = rel * abs(want[i]) + 4 * 2.0 ** -149 + (2.0 ** -20 if act == "gelu" and vd[i] < 0 else 0.0)
         tol += (2.0 ** -8 * abs(want[i]) + 2.0 ** -134) if y == "bf16" else 0.0
         assert (np.abs(got[i] - want[i]) <= tol).all(), (vd[i], got[i][0], want[i], tol)
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+@pytest.mark.parametrize("Dh", [64, 128, 256])
+@pytest.mark.parametrize("e", [18, 24, 32, 45, 100])
+def test_scores_of_2_to_the_e(attn, Dh, x, e):
+    """Scores of either sign that differ by far more than f32's steps at their size: the token with the largest has all the weight.  A
+    score errs by (Dh + 8) 2^-24 of the sum of |q||k| (test_attn_gpu.py); rows whose best two are closer than eight times that are left out."""
+    rng = np.random.default_rng(21 + e)
+    s = Setup(attn, rng, [(1, 300), (150, 3500), (70, 4000)], 16, 2, Dh, 32, x)
+    s.q *= 2.0 ** e
+    out, lse = (t.double().cpu().numpy() for t in s.run())
+    q, scale, t0, j0, clear = s.q.double().cpu().numpy(), Dh ** -0.5, 0, 0, []
+    for n, kv in s.lens:
+        for h in range(16):
+            k, v, qq = s.k[j0:j0 + kv, h // 8], s.v[j0:j0 + kv, h // 8], q[t0:t0 + n, h]
+            seen = np.arange(kv) <= kv - n + np.arange(n)[:, None]
+            sc = np.where(seen, qq @ k.T * scale, -np.inf)
+            err = np.where(seen, np.abs(qq) @ np.abs(k).T * scale, 0).max(-1) * (Dh + 8) * 2.0 ** -24
+            best = sc.argmax(-1)
+            top, second = np.partition(sc, -2, -1)[:, -1], np.partition(sc, -2, -1)[:, -2]
+            ok = top - second > 8 * err + 60
+            # A 4-bit value is exact in both types.  (Below 2^20 a weight need not be a power of two: its rounding to bf16, and the output's.)
+            near = np.where(np.abs(top) * 1.4427 < 1.01 * 2 ** 20, 2.0 ** -7, 0)[ok, None] * np.abs(v[best[ok]])
+            assert (np.abs(out[t0:t0 + n, h][ok] - v[best[ok]]) <= near).all()
+            assert (np.abs(lse[t0:t0 + n, h] - top) <= err + 2.0 ** -22 * np.abs(top) + np.log(kv)).all()
+            clear.append(ok.mean())
+        t0, j0 = t0 + n, j0 + kv
+    assert np.mean(clear) > 0.8

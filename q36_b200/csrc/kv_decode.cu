@@ -11,6 +11,7 @@
 // below 2^11, so the strongest token of any block of dims has at least 2^-1 there and f16 is precise down to 2^-14.
 // When an exponent leaves the window (a block of V 2^8 times weaker, 2^4 times stronger than the first tokens'), the warp goes over
 // to a reference per row and block of dims and rounds the weights of every block by themselves, which holds for any exponents.
+// It does so too at K exponents of 65 and more, whose sums with q as it is in f16 would not all fit f32: there they are kept 2^23 lower.
 // Blocks of scale byte 1 need no place in the window: zeros, or values up to 6 * 2^-126, which count as zeros beside an anchor 2^9 or more above.
 // The normaliser is the sum of the unrounded weights in f32.
 // q enters as f16 after an exact power of two per row (bf16 and f16 fit); f32 activations enter as two f16 terms, and so do
@@ -33,6 +34,9 @@ constexpr float DEC_TOP = 7.f, DEC_MAX = 11.f;        // log2 of the largest wei
 constexpr int DEC_WIN_LO = 8, DEC_WIN_HI = 4;         // window of V exponents around the anchor
 constexpr uint32_t DEC_NO_BLOCK = 32 - (15 - DEC_WIN_LO);     // the place in the window whose f16 factor is -0
 constexpr float DEC_WIDE_TOP = 11.f, DEC_WIDE_MAX = 15.f;   // the same with a reference per block of dims
+// What the wide form takes off K's scales until its sums meet the rows' powers of two: eight blocks' sums of 32 products, below 32 * 6 * 2^15
+// as q is in f16, stay in f32 at exponents up to 125; 2^-126 remains a number.
+constexpr float DEC_K_DOWN = 1.f / (1 << 23);
 
 // the four bytes of w, two E2M1 codes each (low nibble first), as f16x2
 __device__ __forceinline__ void e2m1x8_to_f16x2(uint32_t w, uint32_t (&h)[4]) {
@@ -134,15 +138,26 @@ struct DecFrag {
             }
         }
     }
+    static __device__ __forceinline__ void get_ks(const uint8_t *st, int h, int lane, uint32_t (&r)[SW]) {
+        const uint32_t *p = reinterpret_cast<const uint32_t *>(st + CODES + (h * 32 + lane) * SB);
+        if constexpr (NB == 2) r[0] = *p >> (lane & 4 ? 16 : 0);      // (the word has two tokens; what is above is not looked at)
+        else r[0] = p[0];
+        if constexpr (NB == 8) r[1] = p[1];
+    }
     __device__ __forceinline__ void get_k(const uint8_t *st, int lane) {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
             get(st, h, lane, k[h]);
-            const uint32_t *p = reinterpret_cast<const uint32_t *>(st + CODES + (h * 32 + lane) * SB);
-            if constexpr (NB == 2) ks[h][0] = *p >> (lane & 4 ? 16 : 0);      // (the word has two tokens; what is above is not looked at)
-            else ks[h][0] = p[0];
-            if constexpr (NB == 8) ks[h][1] = p[1];
+            get_ks(st, h, lane, ks[h]);
         }
+    }
+    // not zero: token g + 8h has a K exponent of 65 or more (a scale byte with its two top bits set)
+    static __device__ __forceinline__ uint32_t high_k(const uint8_t *st, int h, int lane) {
+        uint32_t r[SW], any = 0;
+        get_ks(st, h, lane, r);
+#pragma unroll
+        for (int w = 0; w < SW; w++) any |= r[w] & (r[w] << 1);
+        return any & (NB == 2 ? 0x8080u : 0x80808080u);
     }
     __device__ __forceinline__ void get_v(const uint8_t *st, int lane) {
         get(st, 2, lane, v[0]);
@@ -349,7 +364,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
         float s[NT][4];
         uint32_t w[TERMS][NT][2];
         // S of the group (log2 units), -infinity where a row does not see the token; m moved when needed
-        auto scores = [&](bool with_o) {
+        auto scores = [&](bool is_wide) {
             f.get_k(st, lane);
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
@@ -360,8 +375,9 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                 uint32_t k0[4], k1[4];
                 e2m1x8_to_f16x2(f.k[0][b], k0);
                 e2m1x8_to_f16x2(f.k[1][b], k1);
-                const float sc0 = __uint_as_float(((f.ks[0][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
-                const float sc1 = __uint_as_float(((f.ks[1][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
+                float sc0 = __uint_as_float(((f.ks[0][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
+                float sc1 = __uint_as_float(((f.ks[1][b / 4] >> (8 * (b & 3))) & 0xff) << 23);
+                if (is_wide) { sc0 *= DEC_K_DOWN; sc1 *= DEC_K_DOWN; }
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -380,7 +396,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int c = 0; c < 4; c++) s[nt][c] *= fac[nt][c & 1];
+                for (int c = 0; c < 4; c++) s[nt][c] = is_wide ? s[nt][c] * fac[nt][c & 1] * (1.f / DEC_K_DOWN) : s[nt][c] * fac[nt][c & 1];
             if (!inner) {
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
@@ -403,7 +419,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                         const float mn = fmaxf(m[nt][c], column_max(fmaxf(s[nt][c], s[nt][c + 2])) - DEC_TOP), by = ex2(m[nt][c] - mn);
                         l[nt][c] *= by;
                         m[nt][c] = mn;
-                        if (with_o) {
+                        if (!is_wide) {
 #pragma unroll
                             for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -437,14 +453,14 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                 anchor = (int)__reduce_max_sync(0xffffffffu, top);
             }
             constexpr uint32_t WIDTH2 = (DEC_WIN_LO + DEC_WIN_HI) * 0x10001u;
-            uint32_t d[Frag::VB], far = 0;
+            uint32_t d[Frag::VB], far = Frag::high_k(st, 0, lane) | Frag::high_k(st, 1, lane);
 #pragma unroll
             for (int c = 0; c < Frag::VB; c++) {
                 d[c] = f.vs[c] - (uint32_t)(anchor - DEC_WIN_LO) * 0x10001u;
                 far |= __vmaxu2(d[c], WIDTH2) ^ WIDTH2;
             }
             if (__any_sync(0xffffffffu, far != 0)) {
-                bool out = false;
+                bool out = (seen(0) && Frag::high_k(st, 0, lane)) || (seen(1) && Frag::high_k(st, 1, lane));
 #pragma unroll
                 for (int c = 0; c < Frag::VB; c++) {
                     const int v0 = f.vs[c] & 0xffff, v1 = f.vs[c] >> 16, e0 = v0 - anchor + DEC_WIN_LO, e1 = v1 - anchor + DEC_WIN_LO;
@@ -467,7 +483,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                     to[2 + (g & 1)] = (uint16_t)(e >> 16);
                 }
             }
-            scores(true);
+            scores(false);
             // weights, transposed into the narrow operand: (token 2j, 2j+1 | 2j+8, 2j+9) of row g
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
@@ -517,7 +533,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                 f.get_v(st, lane);
                 tok = (unit0 + k) * DEC_UNIT;
                 inner = tok >= all_lo && tok + DEC_UNIT - 1 <= all_hi;
-                scores(false);
+                scores(true);
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll

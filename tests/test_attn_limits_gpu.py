@@ -202,3 +202,23 @@ def test_scores_of_2_to_the_e(attn, Dh, x, e):
             clear.append(ok.mean())
         t0, j0 = t0 + n, j0 + kv
     assert np.mean(clear) > 0.8
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+@pytest.mark.parametrize("Dh", [64, 128, 256])
+def test_keys_and_queries_of_opposite_sizes(attn, Dh, x):
+    """K of 2^e, q of 2^-e and scores of about 1, up to where K's scales end; some tokens' K far below the others'.  (One more rounding than the
+    bounds count, that of scale * 2^-126 to f32's smallest numbers: 2^-21 of a score, where they have (Dh + 8) 2^-24.)"""
+    rng = np.random.default_rng(20)
+    sizes = [(1, 400, 115), (1, 90, 122), (1, 300, -115), (1, 70, -122), (3, 200, 100), (1, 500, 64), (70, 4000, 115), (70, 4000, -115)]
+    s = Setup(attn, rng, [(n, kv) for n, kv, _ in sizes], 16, 2, Dh, 32, x)
+    e = np.concatenate([np.full(kv, e) for _, kv, e in sizes])
+    e = np.where(rng.random(len(e)) < 0.3, np.where(rng.random(len(e)) < 0.5, e - 20, 0), e).clip(-122)
+    own_rows(s, rng.standard_normal((len(s.k), 2, Dh)) * 2.0 ** e[:, None, None], rng.standard_normal((len(s.k), 2, Dh)))
+    at = 0
+    for n, _, e in sizes:
+        s.q[at:at + n] *= 2.0 ** -e
+        at += n
+    if x == "f32":
+        s.q = s.q.bfloat16().float() + s.q.bfloat16().float() * 2.0 ** -12
+    s.check(s.run())

@@ -59,6 +59,13 @@ def _ints(what, dev, *ts):
             _refuse(f"{what} (int32, contiguous, on the operands' device)")
 
 
+def _fits(what, *numbers):
+    """Numbers that ctypes would cut to 32 bits without a word."""
+    for n in numbers:
+        if not -2**31 <= n < 2**31:
+            _refuse(f"{what} ({n} does not fit 32 bits)")
+
+
 def _on(what, dev, *ts):
     for t in ts:
         if t is not None and t.get_device() != dev:
@@ -132,6 +139,7 @@ def _rows(T, h, d, dtype, device):
 
 
 def kv_block_bytes(block_size: int, n_kv_head: int, head_dim: int) -> int:
+    _fits("kv_block_bytes", block_size, n_kv_head, head_dim)
     return int(lib.q36_kv_block_bytes(block_size, n_kv_head, head_dim))
 
 
@@ -168,6 +176,10 @@ def kv_tables(kv_old, q_len, block_size, free_blocks, free_head, block_table, T,
     _ints("kv_tables", dev, kv_old, q_len, free_blocks, free_head, block_table)
     if q_len.numel() != B or block_table.dim() != 2 or block_table.shape[0] != B or free_head.numel() != 1:
         _refuse("kv_tables (shapes)")
+    _need(T >= 0, "kv_tables (T)")
+    if n_blocks is None:
+        n_blocks = (2**31 - 1) // max(block_size, 1)
+    _fits("kv_tables", B, T, block_size, n_blocks, free_blocks.numel(), block_table.shape[1])
     sizes = (B + 1, B, T, T, 1, 1)
     if out is not None:
         _ints("kv_tables", dev, *out)
@@ -175,7 +187,7 @@ def kv_tables(kv_old, q_len, block_size, free_blocks, free_head, block_table, T,
     with _call(dev, stream) as st:
         if out is None:
             out = Tables(*torch.unsafe_split_with_sizes(torch.empty(2 * (B + T) + 3, dtype=_I32, device=kv_old.device), sizes))
-        rc = lib.q36_kv_tables(kv_old.data_ptr(), q_len.data_ptr(), B, block_size, (2**31 - 1) // max(block_size, 1) if n_blocks is None else n_blocks, free_blocks.data_ptr(),
+        rc = lib.q36_kv_tables(kv_old.data_ptr(), q_len.data_ptr(), B, block_size, n_blocks, free_blocks.data_ptr(),
                                free_blocks.numel(), free_head.data_ptr(), block_table.data_ptr(), block_table.shape[1], out.cu_q.data_ptr(),
                                out.kv_len.data_ptr(), out.slots.data_ptr(), out.positions.data_ptr(), T, out.free_head.data_ptr(),
                                out.status.data_ptr(), st)
@@ -192,7 +204,7 @@ class KVCache:
 
     def __init__(self, n_blocks: int, block_size: int, n_kv_head: int, head_dim: int, device="cuda", data: torch.Tensor | None = None):
         nbytes = kv_block_bytes(block_size, n_kv_head, head_dim)
-        _need(nbytes > 0 and n_blocks > 0, "KVCache (geometry)")
+        _need(nbytes > 0 and 0 < n_blocks < 2**31, "KVCache (geometry)")
         shape = (n_blocks, n_kv_head, nbytes // n_kv_head)
         if data is None:
             data = torch.zeros(shape, dtype=_U8, device=device)
@@ -224,6 +236,7 @@ class KVCache:
         _on("kv_append", dev, k, v)
         if k.dtype is not v.dtype or k.shape != v.shape or T != k.shape[0]:
             _refuse("kv_append (k, v, slots)")
+        _fits("kv_append", T)
         bf = _is_bf16(k, "kv_append")
         ks, vs = (_rows3(t, self.n_kv_head, self.head_dim, "kv_append") for t in (k, v))
         with _call(dev, stream) as st:
@@ -237,6 +250,7 @@ class KVCache:
         _ints("kv_read", dev, slots)
         if dtype is not _BF16 and dtype is not _F32:
             _refuse("kv_read (bf16 or f32)")
+        _fits("kv_read", T)
         with _call(dev, stream) as st:
             k, v = _rows(T, self.n_kv_head, self.head_dim, dtype, self.device), _rows(T, self.n_kv_head, self.head_dim, dtype, self.device)
             rc = lib.q36_kv_read(*self._geom, self.n_kv_head, self.head_dim, slots.data_ptr(), k.data_ptr(), v.data_ptr(), int(dtype is _BF16), T, st)
@@ -244,7 +258,7 @@ class KVCache:
                 check(rc, "kv_read")
         return k, v
 
-    def _attn_args(self, q, block_table, cu_q, kv_len, scale, window, what):
+    def _attn_args(self, q, block_table, cu_q, kv_len, max_q, scale, window, what):
         _ints(what, self._dev, block_table, cu_q, kv_len)
         _on(what, self._dev, q)
         B = kv_len.numel()
@@ -252,6 +266,7 @@ class KVCache:
             _refuse(f"{what} (q [T, n_head, head_dim], tables)")
         if not 0 <= window < 2**31:
             _refuse(f"{what} (window)")
+        _fits(what, q.shape[0], max_q, block_table.shape[1])
         scale = self.head_dim ** -0.5 if scale is None else scale
         return (*self._geom, q.shape[1], self.n_kv_head, self.head_dim, block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(),
                 kv_len.data_ptr(), B, scale, window)
@@ -260,7 +275,7 @@ class KVCache:
         """q [T, n_head, head_dim] -> out of the same type (and the log-sum-exp [T, n_head] when want_lse).  max_q: the largest
         number of new tokens of a request, as far as known; it chooses kernels only."""
         what = "kv_attention"
-        args = self._attn_args(q, block_table, cu_q, kv_len, scale, window, what)
+        args = self._attn_args(q, block_table, cu_q, kv_len, max_q, scale, window, what)
         T, h, d = q.shape
         bf, qs = _is_bf16(q, what), _rows3(q, h, self.head_dim, what)
         os_ = h * d
@@ -286,7 +301,7 @@ class KVCache:
     def block(self, q, k, v, slots, block_table, cu_q, kv_len, max_q, w_o, h, bias_o=None, scale=None, window=0, ws=None, stream=None):
         """q36_attn_block: append k, v; attention; h [T, D] f32 += attention W_o^T + bias_o, in place."""
         what = "attn_block"
-        args = self._attn_args(q, block_table, cu_q, kv_len, scale, window, what)
+        args = self._attn_args(q, block_table, cu_q, kv_len, max_q, scale, window, what)
         dev, (T, n_head, _) = self._dev, q.shape
         _ints(what, dev, slots)
         _on(what, dev, k, v, w_o, h, bias_o, ws)
@@ -295,6 +310,7 @@ class KVCache:
         D = w_o.shape[0]
         _need(ws is None or ws.is_contiguous(), f"{what} (ws)")
         _need(h.dtype is _F32 and h.is_contiguous() and h.shape == (T, D), f"{what} (h)")
+        _fits(what, D)
         _need(bias_o is None or (bias_o.dtype is _F32 and bias_o.is_contiguous() and bias_o.shape == (D,)), f"{what} (bias_o)")
         bf, qs = _is_bf16(q, what), _rows3(q, n_head, self.head_dim, what)
         ks, vs = (_rows3(t, self.n_kv_head, self.head_dim, what) for t in (k, v))
@@ -318,6 +334,7 @@ def linear(x, w, bias=None, act="none", residual=None, out=None, out_dtype=None,
     (T, K), N, dev = x.shape, w.shape[0], x.get_device()
     if w.shape[1] != K or act not in ACTS:
         _refuse("linear (shapes, act)")
+    _fits("linear", T, N, K)
     _on("linear", dev, w, bias, residual, out)
     if bias is not None and (bias.dtype is not _F32 or not bias.is_contiguous() or bias.shape != (N,)):
         _refuse("linear (bias)")
@@ -336,6 +353,7 @@ def linear(x, w, bias=None, act="none", residual=None, out=None, out_dtype=None,
         _refuse("linear (out_dtype)")
     if rows_used is not None:
         _ints("linear", dev, rows_used)
+        _need(rows_used.numel() == 1, "linear (rows_used: one number)")
     with _call(dev, stream) as st:
         if out is None:
             out = torch.empty_strided((T, N), (N, 1), dtype=out_dtype, device=x.device)

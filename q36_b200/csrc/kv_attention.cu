@@ -46,12 +46,13 @@ __device__ __forceinline__ int join_list(const AttnPart *desc, int grid, int *li
     return n;
 }
 
-// The join.  Row r of the span whose first piece CTA i had: piece p counts l_p 2^(m_p - m); a piece that saw nothing has no row to read.
+// The join.  Row r of the span whose first piece CTA i had: piece p counts l_p 2^(m_p - m) / l, divided by the sum before it meets the row,
+// so that rows as large as f32 holds stay finite; a piece that saw nothing has no row to read.
 __device__ __forceinline__ const float *join_slot(const float *part, const AttnPart &d, int cta, int p, int stride) {
     return part + (size_t)(p == 0 ? d.slot : 2 * (cta + p)) * stride;
 }
 
-// The weights of a row's pieces, lane p has those of pieces p, p + 32, ..: their sum, and the largest m.
+// The weights of a row's pieces, lane p has those of pieces p, p + 32, ..; l: what they were divided by, m: the largest one.
 template <bool KEEP>
 __device__ __forceinline__ void join_weights(const AttnPart &d, const float *part, int cta, int stride, int r, int lane, float *w, float &first, float &m, float &l) {
     m = -3.0e38f;
@@ -66,6 +67,10 @@ __device__ __forceinline__ void join_weights(const AttnPart &d, const float *par
         if (KEEP) w[p] = f;
     }
     l = warp_sum(l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    first *= inv;
+    if (KEEP)
+        for (int p = lane; p < d.parts; p += 32) w[p] *= inv;
 }
 // a lane's share of the weighted rows of pieces p0, p0 + step, ..: several on their way at a time
 template <int DH, typename W>
@@ -94,10 +99,9 @@ __device__ __forceinline__ void join_rows(const AttnPart &d, const float *part, 
     }
 }
 template <int DH>
-__device__ __forceinline__ void join_store(const AttnArgs &a, const AttnPart &d, int r, int lane, int k, float4 o, float l) {
+__device__ __forceinline__ void join_store(const AttnArgs &a, const AttnPart &d, int r, int lane, int k, float4 o) {
     if (DH < 128 && lane >= DH / 4) return;
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), make_float4(o.x * f, o.y * f, o.z * f, o.w * f));
+    attn_store(a, d.t0, d.n, d.hk, d.row0 + r, 4 * (32 * k + lane), o);
 }
 
 // Tiles of 8 or 16 rows.  Spans in up to 32 pieces: a block per span, a warp per row.  Longer ones: a block per row, its warps share
@@ -124,7 +128,7 @@ k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *desc, const flo
                 join_weights<false>(d, part, cta, stride, r, lane, nullptr, first, m, l);
                 join_rows<DH>(d, part, cta, stride, tile_rows, r, lane, 0, 1, [&](int p) { return p < 32 ? __shfl_sync(0xffffffffu, first, p) : 0.f; }, o);
 #pragma unroll
-                for (int k = 0; k < N4; k++) join_store<DH>(a, d, r, lane, k, o[k], l);
+                for (int k = 0; k < N4; k++) join_store<DH>(a, d, r, lane, k, o[k]);
                 if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r, m, l);
             }
             continue;
@@ -142,7 +146,7 @@ k_attn_join(AttnArgs a, int tile_rows, int grid, const AttnPart *desc, const flo
             float4 t = acc[0][warp][lane];
 #pragma unroll
             for (int i = 1; i < WARPS; i++) { const float4 v = acc[i][warp][lane]; t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w; }
-            join_store<DH>(a, d, row, lane, warp, t, l);
+            join_store<DH>(a, d, row, lane, warp, t);
         }
         if (threadIdx.x == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + row, m, l);
         __syncthreads();
@@ -184,6 +188,15 @@ k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *desc, cons
         }
 #pragma unroll
         for (int i = 0; i < RB; i++) l[i] = warp_sum(l[i]);
+        {
+            float inv[RB];
+#pragma unroll
+            for (int i = 0; i < RB; i++) inv[i] = l[i] == 0.f ? 0.f : 1.f / l[i];
+            for (int p = lane; p < d.parts; p += 32) {
+                const float4 f = w[warp][p];
+                w[warp][p] = make_float4(f.x * inv[0], f.y * inv[1], f.z * inv[2], f.w * inv[3]);
+            }
+        }
         __syncwarp();
         float4 o[RB][N4];
 #pragma unroll
@@ -215,7 +228,7 @@ k_attn_join_rows(AttnArgs a, int tile_rows, int grid, const AttnPart *desc, cons
         for (int i = 0; i < RB; i++) {
             if (r + i >= d.rows) break;
 #pragma unroll
-            for (int k = 0; k < N4; k++) join_store<DH>(a, d, r + i, lane, k, o[i][k], l[i]);
+            for (int k = 0; k < N4; k++) join_store<DH>(a, d, r + i, lane, k, o[i][k]);
             if (lane == 0) attn_store_lse(a, d.t0, d.n, d.hk, d.row0 + r + i, m[i], l[i]);
         }
         __syncwarp();

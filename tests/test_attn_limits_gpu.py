@@ -222,3 +222,23 @@ def test_keys_and_queries_of_opposite_sizes(attn, Dh, x):
     if x == "f32":
         s.q = s.q.bfloat16().float() + s.q.bfloat16().float() * 2.0 ** -12
     s.check(s.run())
+
+
+VALUE_LENS = [[(1, 30000), (3, 400)]]
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+@pytest.mark.parametrize("Dh", [64, 128, 256])
+@pytest.mark.parametrize("e", [105, 124])
+@pytest.mark.parametrize("lens", VALUE_LENS)
+def test_values_up_to_the_largest(attn, lens, Dh, x, e):
+    """V of 2^e and some infinities (stored as 6 * 2^125), in spans that are cut and joined and in whole ones: sums of tens of thousands
+    of them times their weights, which have to be divided before they leave f32."""
+    rng = np.random.default_rng(22 + e)
+    s = Setup(attn, rng, lens, 16, 2, Dh, 64, x)
+    v = np.clip(rng.standard_normal((len(s.k), 2, Dh)) + 2, -2, 4) * 2.0 ** e
+    if e == 124:
+        v[rng.random(v.shape) < 0.01] = np.inf
+    own_rows(s, rng.standard_normal((len(s.k), 2, Dh)), v)
+    assert np.abs(s.v).max() >= 2.0 ** e and (e < 124 or np.abs(s.v).max() == 6 * 2.0 ** 125)
+    s.check(s.run())

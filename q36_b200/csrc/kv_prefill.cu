@@ -43,6 +43,9 @@ struct PfCfg {
 constexpr float PF_NONE = -3.0e38f;      // "no token yet": finite, so that differences stay defined
 constexpr float PF_GROW = 8.f;
 constexpr float PF_LARGE = 1 << 20;
+// V is widened 2^32 lower than it is, so that weights of up to 2^8 on as many tokens as memory holds stay in f32 at any of its exponents
+// (infinities are stored as 6 * 2^125); what falls out is below 2^-92.
+constexpr int PF_V_DOWN = 32;
 // What a span costs beside its tokens (Q in, results out, the pipeline's start), in tokens.  Prompt of 8192, 2 x 256 spans: us at 1
 // 577, 192 450, 384 373, 512 374, 768 379.
 constexpr int PF_SPAN = 448;
@@ -447,7 +450,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
                 tc_fence_after();
             }
             float *dst = part + (size_t)(2 * blockIdx.x + (first ? 0 : 1)) * attn_part_floats(R, DH);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const float inv = l == 0.f ? 0.f : 4294967296.f / l;      // (and 2^PF_V_DOWN)
             if (active) {
                 // through Q's place, so that a row leaves as a whole: bf16 at once, f32 in halves
                 const int n_pass = g.whole ? 1 : 2, dims = DH / n_pass;
@@ -512,6 +515,7 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_WIDEN));
         const int th = tid & 127, tl = th % KT, half = th / KT;
         const bool is_v = warp >= 12;
+        const int down = is_v ? PF_V_DOWN : 0;
         uint32_t kc = 0;
         bool ok = true;
         while (more && ok) {
@@ -525,7 +529,10 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
             struct Half { uint32_t w[RAW], scale; bool has; };
             auto fetch = [&](int j, int id, Half &f) {
                 f.has = id >= 0 && id < a.kv.n_blocks;
-                if (!f.has) return;
+                if (!f.has) {
+                    f.scale = 0;
+                    return;
+                }
                 const int t = (j * KT + tl) & (a.kv.bs - 1);
                 const uint8_t *reg = a.kv.at(id, pos.hk);
                 f.scale = ld_part<BPT>(reg + a.kv.bs * DH + (is_v ? a.kv.bs * NB : 0) + t * NB + half * BPT);
@@ -571,7 +578,8 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
                 uint8_t *dst = smem + NQ * C::Q_BYTES + ((is_v ? ST : 0) + st) * C::T_BYTES + tl * 128;
 #pragma unroll
                 for (int b = 0; b < BPT; b++) {
-                    const Lut t = make_lut((cur.scale >> (8 * b)) & 0xff, cur.has);
+                    const int sc = (int)(cur.scale >> (8 * b) & 0xff) - down;
+                    const Lut t = make_lut(sc, sc > 0);
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
                         uint32_t w;

@@ -224,7 +224,7 @@ def test_keys_and_queries_of_opposite_sizes(attn, Dh, x):
     s.check(s.run())
 
 
-VALUE_LENS = [[(1, 30000), (3, 400)]]
+VALUE_LENS = [[(1, 30000), (3, 400)], [(70, 4000), (200, 9000)]]
 
 
 @pytest.mark.parametrize("x", ["bf16", "f32"])

@@ -661,7 +661,13 @@ k_attn_prefill(AttnArgs a, AttnPart *__restrict__ desc, float *__restrict__ part
     __syncwarp();
     tc_fence_before();
     __syncthreads();
-    if (warp == 16) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    if (warp == 16) {
+        if (abort_flag)
+#pragma unroll 1
+            for (int i = 0; i < 200; i++) __nanosleep(1000);      // products and copies in flight land before the block gives its memory back
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    }
 }
 
 template <int DH>

@@ -366,7 +366,13 @@ k_linear_tc(const __grid_constant__ LtMaps maps, Epilogue e, int T, int N, int K
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
+    if (warp == 1) {
+        if (abort_flag)
+#pragma unroll 1
+            for (int i = 0; i < 200; i++) __nanosleep(1000);      // products and copies in flight land before the block gives its memory back
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TM_COLS) : "memory");
+    }
 }
 
 static int make_map_bf16(CUtensorMap *m, const void *base, long rows, long cols, long long stride, int box_rows) {

@@ -16,9 +16,13 @@ struct Epilogue {
 // x / (1 + h^2), and below 0 that times h^2, one h after the other: nothing leaves f32's range on the way, and the result goes to zero where
 // the function does, in relative precision.  -infinity counts as the lowest finite number, so that zero is its limit too.
 // 0.5 (1 + tanh u/2) is the logistic function of u.
-__device__ __forceinline__ float floor_finite(float x) { return fmaxf(x, -3.402823466e38f); }
+__device__ __forceinline__ float floor_finite(float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, 0fFF7FFFFF;" : "=f"(r) : "f"(x));
+    return r;
+}
 __device__ __forceinline__ float times_logistic(float x, float u) {
-    const float h = __expf(-0.5f * fabsf(u)), q = __fdividef(floor_finite(x), fmaf(h, h, 1.f));
+    const float h = __expf(-0.5f * fabsf(u)), q = __fdividef(x, fmaf(h, h, 1.f));
     return u < 0.f ? q * h * h : q;
 }
 template <int N>
@@ -30,15 +34,24 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
             break;
         case Q36_ACT_SILU:
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = times_logistic(v[i], v[i]);
+            for (int i = 0; i < N; i++) {
+                v[i] = floor_finite(v[i]);
+                v[i] = times_logistic(v[i], v[i]);
+            }
             break;
         case Q36_ACT_GELU:
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = 0.5f * floor_finite(v[i]) * (1.f + erff(v[i] * 0.70710678118654752f));
+            for (int i = 0; i < N; i++) {
+                v[i] = floor_finite(v[i]);
+                v[i] = 0.5f * v[i] * (1.f + erff(v[i] * 0.70710678118654752f));
+            }
             break;
         case Q36_ACT_GELU_TANH:
 #pragma unroll
-            for (int i = 0; i < N; i++) v[i] = times_logistic(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+            for (int i = 0; i < N; i++) {
+                v[i] = floor_finite(v[i]);
+                v[i] = times_logistic(v[i], 1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+            }
             break;
         default: break;
     }

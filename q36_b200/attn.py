@@ -111,6 +111,8 @@ def _call(dev: int, stream=None):
         _refuse("operands not on a CUDA device")
     if stream is None and dev == torch.cuda.current_device():
         return _Here(_raw_stream(dev))
+    if stream is not None and stream.device.index != dev:
+        _refuse("operands and stream on different devices")
     return _on_device(dev, stream)
 
 

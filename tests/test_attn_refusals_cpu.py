@@ -70,3 +70,13 @@ def test_linear(attn):
     big = torch.empty((2**32 + 8, 64), dtype=torch.bfloat16, device="meta")
     with pytest.raises(attn.MoEError, match="32 bits"):
         attn.linear(torch.empty((2, 64), dtype=torch.bfloat16, device="meta"), big)
+
+
+def test_a_stream_of_another_device(moe):
+    """Its device would become the current one, and the launch would be that device's with this one's addresses."""
+    import types
+    import torch
+    from q36_b200 import attn
+    for dev, index in ((0, 1), (3, 0)):
+        with pytest.raises(attn.MoEError, match="different devices"):
+            attn._call(dev, types.SimpleNamespace(device=torch.device("cuda", index)))

@@ -59,11 +59,8 @@ def _ints(what, dev, *ts):
             _refuse(f"{what} (int32, contiguous, on the operands' device)")
 
 
-def _fits(what, *numbers):
-    """Numbers that ctypes would cut to 32 bits without a word."""
-    for n in numbers:
-        if not -2**31 <= n < 2**31:
-            _refuse(f"{what} ({n} does not fit 32 bits)")
+# ctypes cuts integers to 32 bits without a word.  (Sizes whose tensors would not fit the GPU's memory are not looked at.)
+_INT_MAX = 2**31 - 1
 
 
 def _on(what, dev, *ts):
@@ -141,7 +138,7 @@ def _rows(T, h, d, dtype, device):
 
 
 def kv_block_bytes(block_size: int, n_kv_head: int, head_dim: int) -> int:
-    _fits("kv_block_bytes", block_size, n_kv_head, head_dim)
+    _need(max(block_size, n_kv_head, head_dim) <= _INT_MAX, "kv_block_bytes (32 bits)")
     return int(lib.q36_kv_block_bytes(block_size, n_kv_head, head_dim))
 
 
@@ -178,10 +175,10 @@ def kv_tables(kv_old, q_len, block_size, free_blocks, free_head, block_table, T,
     _ints("kv_tables", dev, kv_old, q_len, free_blocks, free_head, block_table)
     if q_len.numel() != B or block_table.dim() != 2 or block_table.shape[0] != B or free_head.numel() != 1:
         _refuse("kv_tables (shapes)")
-    _need(T >= 0, "kv_tables (T)")
     if n_blocks is None:
-        n_blocks = (2**31 - 1) // max(block_size, 1)
-    _fits("kv_tables", B, T, block_size, n_blocks, free_blocks.numel(), block_table.shape[1])
+        n_blocks = _INT_MAX // max(block_size, 1)
+    if T < 0 or B > _INT_MAX or T > _INT_MAX or block_size > _INT_MAX or n_blocks > _INT_MAX or free_blocks.numel() > _INT_MAX or block_table.shape[1] > _INT_MAX:
+        _refuse("kv_tables (sizes below 0 or beyond 32 bits)")
     sizes = (B + 1, B, T, T, 1, 1)
     if out is not None:
         _ints("kv_tables", dev, *out)
@@ -206,7 +203,7 @@ class KVCache:
 
     def __init__(self, n_blocks: int, block_size: int, n_kv_head: int, head_dim: int, device="cuda", data: torch.Tensor | None = None):
         nbytes = kv_block_bytes(block_size, n_kv_head, head_dim)
-        _need(nbytes > 0 and 0 < n_blocks < 2**31, "KVCache (geometry)")
+        _need(nbytes > 0 and 0 < n_blocks <= _INT_MAX, "KVCache (geometry)")
         shape = (n_blocks, n_kv_head, nbytes // n_kv_head)
         if data is None:
             data = torch.zeros(shape, dtype=_U8, device=device)
@@ -238,7 +235,6 @@ class KVCache:
         _on("kv_append", dev, k, v)
         if k.dtype is not v.dtype or k.shape != v.shape or T != k.shape[0]:
             _refuse("kv_append (k, v, slots)")
-        _fits("kv_append", T)
         bf = _is_bf16(k, "kv_append")
         ks, vs = (_rows3(t, self.n_kv_head, self.head_dim, "kv_append") for t in (k, v))
         with _call(dev, stream) as st:
@@ -252,7 +248,6 @@ class KVCache:
         _ints("kv_read", dev, slots)
         if dtype is not _BF16 and dtype is not _F32:
             _refuse("kv_read (bf16 or f32)")
-        _fits("kv_read", T)
         with _call(dev, stream) as st:
             k, v = _rows(T, self.n_kv_head, self.head_dim, dtype, self.device), _rows(T, self.n_kv_head, self.head_dim, dtype, self.device)
             rc = lib.q36_kv_read(*self._geom, self.n_kv_head, self.head_dim, slots.data_ptr(), k.data_ptr(), v.data_ptr(), int(dtype is _BF16), T, st)
@@ -268,7 +263,8 @@ class KVCache:
             _refuse(f"{what} (q [T, n_head, head_dim], tables)")
         if not 0 <= window < 2**31:
             _refuse(f"{what} (window)")
-        _fits(what, q.shape[0], max_q, block_table.shape[1])
+        if not 0 < max_q <= _INT_MAX or block_table.shape[1] > _INT_MAX:
+            _refuse(f"{what} (max_q, table: 1 to 2^31 - 1)")
         scale = self.head_dim ** -0.5 if scale is None else scale
         return (*self._geom, q.shape[1], self.n_kv_head, self.head_dim, block_table.data_ptr(), block_table.shape[1], cu_q.data_ptr(),
                 kv_len.data_ptr(), B, scale, window)
@@ -294,7 +290,7 @@ class KVCache:
             lse = torch.empty((T, h), dtype=_F32, device=self.device) if want_lse else None
             with self._lock if ws is None else _NO_LOCK:
                 if ws is None:
-                    ws = self._scratch(_attention_ws(self._dev, h, self.n_kv_head, d, max(max_q, 1)), st)
+                    ws = self._scratch(_attention_ws(self._dev, h, self.n_kv_head, d, max_q), st)
                 rc = lib.q36_kv_attention(q.data_ptr(), bf, qs, *args, out.data_ptr(), os_, ptr(lse), T, max_q, ws.data_ptr(), ws.numel(), st)
             if rc:
                 check(rc, what)
@@ -312,14 +308,13 @@ class KVCache:
         D = w_o.shape[0]
         _need(ws is None or ws.is_contiguous(), f"{what} (ws)")
         _need(h.dtype is _F32 and h.is_contiguous() and h.shape == (T, D), f"{what} (h)")
-        _fits(what, D)
         _need(bias_o is None or (bias_o.dtype is _F32 and bias_o.is_contiguous() and bias_o.shape == (D,)), f"{what} (bias_o)")
         bf, qs = _is_bf16(q, what), _rows3(q, n_head, self.head_dim, what)
         ks, vs = (_rows3(t, self.n_kv_head, self.head_dim, what) for t in (k, v))
         with _call(dev, stream) as st:
             with self._lock if ws is None else _NO_LOCK:
                 if ws is None:
-                    ws = self._scratch(_block_ws(dev, T, n_head, self.n_kv_head, self.head_dim, max(max_q, 1)), st)
+                    ws = self._scratch(_block_ws(dev, T, n_head, self.n_kv_head, self.head_dim, max_q), st)
                 rc = lib.q36_attn_block(q.data_ptr(), k.data_ptr(), v.data_ptr(), bf, qs, ks, vs, slots.data_ptr(), *args, w_o.data_ptr(), ptr(bias_o),
                                         h.data_ptr(), D, T, max_q, ws.data_ptr(), ws.numel(), st)
             if rc:
@@ -336,7 +331,8 @@ def linear(x, w, bias=None, act="none", residual=None, out=None, out_dtype=None,
     (T, K), N, dev = x.shape, w.shape[0], x.get_device()
     if w.shape[1] != K or act not in ACTS:
         _refuse("linear (shapes, act)")
-    _fits("linear", T, N, K)
+    if T > _INT_MAX or N > _INT_MAX or K > _INT_MAX:
+        _refuse("linear (sizes beyond 32 bits)")
     _on("linear", dev, w, bias, residual, out)
     if bias is not None and (bias.dtype is not _F32 or not bias.is_contiguous() or bias.shape != (N,)):
         _refuse("linear (bias)")

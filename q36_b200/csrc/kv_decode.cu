@@ -172,7 +172,8 @@ struct DecFrag {
     }
 };
 
-// The wide form's weights of block b: 2^(S + vs - M), M per row and block; moves M, and with it the block's sums.
+// The wide form's weights of block b: 2^(S - m + vs - M), M per row and block and relative to m, so that exponents of V are not lost beside
+// large scores; moves M, and with it the block's sums.  s: S - m.
 template <int DH, int NT, int TERMS, int VB>
 __device__ __forceinline__ void wide_weights(float (*Ms)[8 * NT], const uint32_t (&vs)[VB], const float (&s)[NT][4], uint32_t (&w)[TERMS][NT][2],
                                              float (&o)[NT][DH / 32][2][4], int b, int lane) {
@@ -197,8 +198,8 @@ __device__ __forceinline__ void wide_weights(float (*Ms)[8 * NT], const uint32_t
             }
             __syncwarp();
             if (lane < 4) *Mp = M;
-            p[c] = ex2(x0 - (M - DEC_WIDE_TOP));
-            p[c + 2] = ex2(x1 - (M - DEC_WIDE_TOP));
+            p[c] = ex2((x0 - M) + DEC_WIDE_TOP);
+            p[c + 2] = ex2((x1 - M) + DEC_WIDE_TOP);
         }
         weights_f16<TERMS>(p, w, nt);
     }
@@ -418,6 +419,14 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
                     for (int c = 0; c < 2; c++) {
                         const float mn = fmaxf(m[nt][c], column_max(fmaxf(s[nt][c], s[nt][c + 2])) - DEC_TOP), by = ex2(m[nt][c] - mn);
                         l[nt][c] *= by;
+                        if (is_wide && lane < 4) {
+                            // (they are relative to m)
+#pragma unroll
+                            for (int b = 0; b < NB; b++) {
+                                float *M = &sm.M[warp][b][nt * 8 + 2 * j + c];
+                                *M = fmaxf(*M + (m[nt][c] - mn), DEC_NONE);
+                            }
+                        }
                         m[nt][c] = mn;
                         if (!is_wide) {
 #pragma unroll
@@ -524,7 +533,7 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
 #pragma unroll
                 for (int c = 0; c < 2; c++)
                     for (int b = g; b < NB; b += 8)
-                        sm.M[warp][b][nt * 8 + 2 * j + c] = m[nt][c] == DEC_NONE ? DEC_NONE : m[nt][c] + (float)(anchor - 127) + DEC_WIDE_TOP;
+                        sm.M[warp][b][nt * 8 + 2 * j + c] = m[nt][c] == DEC_NONE ? DEC_NONE : (float)(anchor - 127) + DEC_WIDE_TOP;
             __syncwarp();
 #pragma unroll 1
             for (bool fresh = true; k < n_mine; k++, fresh = false) {
@@ -537,7 +546,10 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int c = 0; c < 4; c++) l[nt][c & 1] += ex2(s[nt][c] - m[nt][c & 1]);
+                    for (int c = 0; c < 4; c++) {
+                        s[nt][c] -= m[nt][c & 1];
+                        l[nt][c & 1] += ex2(s[nt][c]);
+                    }
 #pragma unroll
                 for (int b2 = 0; b2 < NB / 2; b2++) {
                     uint32_t ev[2][4], od[2][4];
@@ -584,12 +596,12 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
             }
 #pragma unroll
             for (int b = 0; b < NB; b++) {
-                // 2^reference / (2^ma la), the sum in the exponent: V may be as large or small as f32
+                // 2^(m + reference) / (2^ma la), the sum in the exponent: V may be as large or small as f32
                 float f[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    const float ref = wide ? sm.M[warp][b][nt * 8 + 2 * j + c] : m[nt][c];
-                    f[c] = exp2f((ref - ma2[c]) + ((wide ? -DEC_WIDE_TOP : (float)(anchor - 127)) - lg[c]));
+                    const float ref = wide ? sm.M[warp][b][nt * 8 + 2 * j + c] - DEC_WIDE_TOP : (float)(anchor - 127);
+                    f[c] = exp2f((m[nt][c] - ma2[c]) + (ref - lg[c]));
                 }
 #pragma unroll
                 for (int u = 0; u < 2; u++) {

@@ -52,6 +52,8 @@ uint64_t q36_kv_block_bytes(int block_size, int n_kv_head, int head_dim);
  *   *free_head_out   entries of the free list used so far (may be free_head itself)
  *   *status          0, or the sum of: 1 the free list is too short, 2 the table is
  *                    too narrow, 4 a negative length, 8 more rows than T
+ * With kv_len or free_head_out in place one thread block does the work: as fast for
+ * decoding steps, 30 to 40 us for prompts of 32,768 tokens together (4 otherwise).
  * A request that cannot be served takes no block: its kv_len is 0 (attention
  * gives zeros for its rows) and its slots are -1.  When the free list is too
  * short, the requests behind the first unserved one that need blocks are not
@@ -104,7 +106,7 @@ int q36_kv_attention(const void *q, int x_is_bf16, int64_t q_stride, const void 
 /* y [T][N] = act(x W^T + bias) + residual: x bf16 [T][K], w bf16 [N][K]
  * contiguous, bias f32 [N] or NULL, residual [T][N] f32 or bf16 or NULL, y f32 or
  * bf16; strides between rows in elements.  Sums in f32, one rounding at the end.
- * residual may be y itself (same type and stride).  rows_used (or NULL): device
+ * residual may be y itself (same type and stride); y overlaps nothing else.  rows_used (or NULL): device
  * count of rows; rows of y from *rows_used on are left as they were.  K and
  * x_stride are multiples of 8; T, N, K <= 2^30. */
 int q36_linear(const void *x, int64_t x_stride, const void *w, const float *bias, int act, const void *residual,
@@ -126,7 +128,8 @@ int q36_attn_block(const void *q, const void *k, const void *v, int x_is_bf16, i
  * Synchronises the stream and returns Q36_MOE_EDEVICE when one gave up on the
  * current device since the last call of this function (results written since then
  * are not to be used; which one: q36_moe_last_cuda_error()), else 0.  One check
- * covers every call before it, as q36_moe_ws_status does. */
+ * covers every call before it, as q36_moe_ws_status does: the record is the device's,
+ * and the check clears it, so let one thread of the process ask. */
 int q36_attn_status(void *stream);
 /* A 32-thread kernel that waits for what nobody completes, with a short limit, and
  * records that it gave up: lets a test see q36_attn_status report it. */

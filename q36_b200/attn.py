@@ -143,7 +143,8 @@ def kv_block_bytes(block_size: int, n_kv_head: int, head_dim: int) -> int:
 
 
 def check_device_status(device=None) -> None:
-    """Raises when a bounded wait of the attention or product kernels gave up on the device since the last check."""
+    """Raises when a bounded wait of the attention or product kernels gave up on the device since the last check (by anyone: for one
+    checking thread per device)."""
     with torch.cuda.device(device):
         check(lib.q36_attn_status(torch.cuda.current_stream().cuda_stream), "attn device status")
 

@@ -63,7 +63,7 @@ __device__ __forceinline__ void load8(const void *p, size_t e, int bf16, float (
     }
 }
 
-int launch_attention(AttnArgs a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st);
+int launch_attention(AttnArgs a, int max_q, void *ws, cudaStream_t st);
 uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q);
 int launch_kv_append(const void *k, const void *v, int bf16, long long ks, long long vs, const int *slots, KvGeom g, int T, cudaStream_t st);
 int launch_linear(const void *x, long long xs, const void *w, const float *bias, int act, const void *res, int res_bf16, long long rs,

@@ -258,8 +258,7 @@ uint64_t attention_ws_bytes(int Hq, int Hkv, int Dh, int max_q) {
     return rows < LONG_ROWS ? few : max(few, prefill_ws_bytes(Dh));      // (one after the other on the stream: the same memory)
 }
 
-int launch_attention(AttnArgs a, int max_q, void *ws, uint64_t ws_bytes, cudaStream_t st) {
-    (void)ws_bytes;
+int launch_attention(AttnArgs a, int max_q, void *ws, cudaStream_t st) {
     const long long all = (long long)a.T * a.G;
     const int rows = (int)min((long long)rows_of(a.Hq, a.kv.Hkv, max_q), all);      // of one request, at most
     a.long_work = all <= LONG_FEW_ROWS ? LONG_WORK_FEW : LONG_WORK;
@@ -324,7 +323,7 @@ int q36_kv_attention(const void *q, int x_is_bf16, int64_t q_stride, const void 
     a.o_stride = out_stride;
     a.o_bf16 = a.q_bf16;
     a.lse = lse;
-    return launch_attention(a, max_q, ws, ws_bytes, (cudaStream_t)stream);
+    return launch_attention(a, max_q, ws, (cudaStream_t)stream);
 }
 
 uint64_t q36_attn_block_workspace_bytes(int T, int n_head, int n_kv_head, int head_dim, int max_q) {
@@ -354,7 +353,7 @@ int q36_attn_block(const void *q, const void *k, const void *v, int x_is_bf16, i
     a.o_bf16 = 1;
     a.lse = nullptr;
     if ((rc = launch_kv_append(k, v, x_is_bf16, k_stride, v_stride, slots, a.kv, T, st))) return rc;
-    if ((rc = launch_attention(a, max_q, ws, at, st))) return rc;
+    if ((rc = launch_attention(a, max_q, ws, st))) return rc;
     return launch_linear(a.out, K, w_o, bias_o, Q36_ACT_NONE, h, 0, D, h, 0, D, T, D, K, cu_q + n_seq, st);
 }
 

@@ -20,8 +20,9 @@
 // Work.  A unit is 16 tokens of one (request, kv head, row tile).  The units of all requests, in order, are cut into equal
 // ranges, one per CTA, so that ragged lengths load every SM alike.  A range's first and last pieces may be parts of what a
 // neighbour has the rest of: they go to the workspace and k_attn_join adds them up in a fixed order.
-// With the join, 16 heads of 128 on 2: 64 requests of 266,000 tokens together 35 us, of 524,000 49 (5.0 TB/s between the two; the first 20 us
-// are launches, plan, the first reads of a page, of its data, and the join), one of 700 tokens 10, one of 131,072 32.
+// With the join, 16 heads of 128 on 2, from HBM: 64 requests of 266,000 tokens together 36 us, of 533,000 53, of 1,065,000 86 (4.2 to 4.4 TB/s
+// between them; the first 20 us are launches, plan, the first reads of a page, of its data, and the join), one of 131,072 32; one of 700
+// tokens 10.  Tokens all in the second form: 266,000 43.
 #include <math.h>
 
 #include "attn_plan.cuh"
@@ -222,7 +223,7 @@ struct DecSmem {
 
 template <int DH, int NT, bool F32>
 // What bounds it: instructions, 350 per warp and 16 tokens of 128 dims.  16 warps per SM at 128 registers are better than 20 at 102
-// (64 requests, 266,000 tokens: 35 against 39 us) and 12 at 168 (43); wider accumulators (256 dims, or 16 rows of 128) keep 8 warps at 255
+// (64 requests, 266,000 tokens: 35 against 39 us, when these were chosen) and 12 at 168 (43); wider accumulators (256 dims, or 16 rows of 128) keep 8 warps at 255
 // (37 us at 112,000 tokens of 256; 38 with 12 warps).  Tokens come by asynchronous copies one group ahead (35 us; 38 with loads into
 // registers behind their last use), two ahead gain nothing.  The stages share their place with the results: with a place of their own, 35.3,
 // and 33.2 against 32.0 for one request of 131,072, since more shared memory leaves less of L1.

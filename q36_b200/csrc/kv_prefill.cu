@@ -11,8 +11,8 @@
 // Every row tile has two S, so that the products of a tile run while the softmax is at the one before.
 // m is a lagging maximum: O is rescaled (in TMEM) only when a row would pass 2^8.
 //
-// What bounds it: nothing alone.  A tile takes 2300 cycles (2048 tokens behind 32,768, 16 heads of 128 on 2: 584 us, 970 TFLOP/s; prompt of
-// 8192 336 us, 819).  The tensor pipe needs 1320 of them (an MMA of 128 x 64 x 16 with both operands in shared memory takes 50 cycles,
+// What bounds it: nothing alone.  A tile takes 2300 cycles (2048 tokens behind 32,768, 16 heads of 128 on 2: 589 us, 962 TFLOP/s; prompt of
+// 8192 339 us, 811).  The tensor pipe needs 1320 of them (an MMA of 128 x 64 x 16 with both operands in shared memory takes 50 cycles,
 // shared memory's rate, one of 128 x 128 x 16 with P in TMEM 65), the exponentials 1070, the ALU 1330, issue slots two thirds.  Without the
 // exponentials the time stays, with twice the widening warps too, with both it falls by a tenth.  Tried without gain: a polynomial for
 // some of the exponentials, turns between the two row tiles' exponentials, sleeping waits, other register splits.
@@ -46,8 +46,9 @@ constexpr float PF_LARGE = 1 << 20;
 // V is widened 2^32 lower than it is, so that weights of up to 2^8 on as many tokens as memory holds stay in f32 at any of its exponents
 // (infinities are stored as 6 * 2^125); what falls out is below 2^-92.
 constexpr int PF_V_DOWN = 32;
-// What a span costs beside its tokens (Q in, results out, the pipeline's start), in tokens.  Prompt of 8192, 2 x 256 spans: us at 1
-// 577, 192 450, 384 373, 512 374, 768 379.
+// What a span costs beside its tokens (Q in, results out, the pipeline's start), in tokens.  us at 192 / 320 / 448 / 640 / 768: prompt of 8192,
+// 128-wide heads (2 x 256 spans) 414 / 359 / 338 / 343 / 346, 64-wide 301 / 283 / 285 / 290 / 292; of 4096, 256-wide (2 x 256 spans of half the
+// rows) 318 / 268 / 260 / 267 / 271.
 constexpr int PF_SPAN = 448;
 constexpr int PF_MIN = 1024;        // the smallest range of a CTA
 // Places for the bad pages of a tile, which go from the group that widens K to the softmax without a barrier of their own.  K runs up to 9

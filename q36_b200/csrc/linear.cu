@@ -112,7 +112,8 @@ __device__ __forceinline__ void finish(const Epilogue &e, int n, float bias, int
 }
 
 // ---------------------------------------------------------------- few rows: the weights' stream
-// Up to 8 rows: the stream of W bounds it, and below 10 MB the latency of one round trip (1 x 2048 x 2048, 8.4 MB, 5.9 us).  A block has
+// Up to 8 rows: the stream of W bounds it, and below 10 MB the latency of one round trip (1 x 2048 x 2048, 8.4 MB: 5.2 us behind one
+// another with W in L2, 7.8 cold).  A block has
 // 16 columns of y (rows of W) and splits K over its warps; a lane reads 16 bytes of two rows of W
 // and of one row of x, which is a fragment of m16n8k16 with k permuted alike on both sides.
 constexpr int LS_WARPS = 8, LS_THREADS = 32 * LS_WARPS, LS_COLS = 16;
@@ -176,8 +177,9 @@ k_linear_few(const uint16_t *x, long long xs, const uint16_t *__restrict__ w, Ep
 // ---------------------------------------------------------------- tiles on tcgen05
 // A tile is 128 columns of y (rows of W, the 128 lanes of the accumulator) by BN rows (its columns): in the epilogue a thread is
 // one column of y, so that bias is a register and a warp's accesses to residual and y are 32 neighbours.
-// The tensor pipe bounds large products (4096 x 4096 x 4096 102 us, 1352 TFLOP/s; 8000 x 4100 x 2048 107 us alone, 112 with gelu_tanh, 122
-// with a bf16 residual, 135 with both and bias: 16 epilogue warps, 143 with 8), the loads from L2 those of few rows.
+// The tensor pipe bounds large products, the loads from L2 those of few rows.  At 1965 MHz, short bursts: 4096 x 4096 x 4096 102 us, 1347
+// TFLOP/s; 8000 x 4100 x 2048 108 plain, 115 with silu, 116 with gelu or gelu_tanh, 122 with a bf16 residual, 128 with gelu_tanh, bias and
+// residual (16 epilogue warps; 8 took 8 us more).  A second of the last is under the power cap: 153 at 1470 MHz, 130 of the plain one.
 // SPLIT > 1: a cluster shares a tile, each CTA a part of K; the parts are added in rank order over distributed shared memory.
 constexpr int LT_M = 128, LT_K = 64;
 template <int BN, int SPLIT>

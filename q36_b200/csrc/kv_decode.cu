@@ -10,7 +10,8 @@
 // bf16's 2^-8 of the output) and block b uses it times 2^(vs[t][b] - anchor), which is exact: mm keeps weights at 2^7 and
 // below 2^11, so the strongest token of any block of dims has at least 2^-1 there and f16 is precise down to 2^-14.
 // When an exponent leaves the window (a block of V 2^8 times weaker, 2^4 times stronger than the first tokens'), the warp goes over
-// to a reference per row and block of dims and rounds the weights of every block by themselves, which holds for any exponents.
+// to a reference per row and block of dims and rounds the weights of every block by themselves: f16 keeps them to 2^-36 of the block's
+// strongest (weight times 2^exponent), whatever the other blocks' exponents.
 // It does so too at K exponents of 65 and more, whose sums with q as it is in f16 would not all fit f32: there they are kept 2^23 lower.
 // Blocks of scale byte 1 need no place in the window: zeros, or values up to 6 * 2^-126, which count as zeros beside an anchor 2^9 or more above.
 // The normaliser is the sum of the unrounded weights in f32.
@@ -528,13 +529,20 @@ k_attn_decode(AttnArgs a, int all, AttnPart *__restrict__ desc, float *__restric
         }
         const bool wide = k < n_mine;
         if (wide) {
-            // the sums so far count 2^(m + anchor - 127)
+            // The sums so far count 2^(m + anchor - 127).  What they are makes the reference, not the anchor, which may be another block's or a
+            // weak token's, far above what comes here; where they are nothing, the next token does.
 #pragma unroll
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int c = 0; c < 2; c++)
-                    for (int b = g; b < NB; b += 8)
-                        sm.M[warp][b][nt * 8 + 2 * j + c] = m[nt][c] == DEC_NONE ? DEC_NONE : (float)(anchor - 127) + DEC_WIDE_TOP;
+#pragma unroll
+                    for (int b = 0; b < NB; b++) {
+                        float (&r0)[4] = o[nt][b][0], (&r1)[4] = o[nt][b][1];
+                        const float most = column_max(fmaxf(fmaxf(fabsf(r0[c]), fabsf(r0[c + 2])), fmaxf(fabsf(r1[c]), fabsf(r1[c + 2]))));
+                        const float e = (float)max((int)(__float_as_uint(most) >> 23) - 127, -100), f = ex2(DEC_WIDE_TOP - e);
+                        r0[c] *= f; r0[c + 2] *= f; r1[c] *= f; r1[c + 2] *= f;
+                        if (lane < 4) sm.M[warp][b][nt * 8 + 2 * j + c] = most > 0.f ? (float)(anchor - 127) + e : DEC_NONE;
+                    }
             __syncwarp();
 #pragma unroll 1
             for (bool fresh = true; k < n_mine; k++, fresh = false) {

@@ -247,3 +247,19 @@ def test_values_up_to_the_largest(attn, lens, Dh, x, e):
     own_rows(s, rng.standard_normal((len(s.k), 2, Dh)), v)
     assert np.abs(s.v).max() >= 2.0 ** e and (e < 124 or np.abs(s.v).max() == 6 * 2.0 ** 125)
     s.check(s.run())
+
+
+@pytest.mark.parametrize("x", ["bf16", "f32"])
+@pytest.mark.parametrize("Dh", [64, 128, 256])
+def test_blocks_of_dims_far_apart_in_turn(attn, Dh, x):
+    """V in one block of dims at 2^12 (one token of 16, then 16 without any), in another at 2^-20 (those 16), zeros everywhere else: what
+    the first one is must not set the precision of the second.  Requests so many that a warp goes through several groups of 16."""
+    rng = np.random.default_rng(23)
+    s = Setup(attn, rng, [(1, int(n)) for n in rng.integers(1500, 2500, 64)], 16, 2, Dh, 32, x)
+    v = np.zeros((len(s.k), 2, Dh))
+    t = np.concatenate([np.arange(n) for _, n in s.lens])
+    odd = t // 16 % 2 == 1
+    v[t % 32 == 3, :, 32:64] = rng.standard_normal(((t % 32 == 3).sum(), 2, 32)) * 2.0 ** 12
+    v[odd, :, :32] = rng.standard_normal((odd.sum(), 2, 32)) * 2.0 ** -20
+    own_rows(s, s.k, v)
+    s.check(s.run())
